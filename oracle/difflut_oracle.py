@@ -179,11 +179,11 @@ def efd_transform(luts: torch.Tensor, alpha: float, beta: float) -> torch.Tensor
     """
     N, O, L = luts.shape
     n = int(math.log2(L))
-    a = torch.arange(L)
     k = torch.arange(L)
     out = torch.empty(N, O, L, n, dtype=torch.float64)
     l64 = luts.double()
     for i in range(n):
+        a = k[((k >> i) & 1) == 0]  # the value does not depend on bit i: one product serves both addresses
         mask = (L - 1) & ~(1 << i)
         x = (a[:, None] ^ k[None, :]) & mask
         ham = torch.zeros_like(x)
@@ -191,7 +191,9 @@ def efd_transform(luts: torch.Tensor, alpha: float, beta: float) -> torch.Tensor
             ham += (x >> bit) & 1
         sign = torch.where(((k >> i) & 1) == 0, -1.0, 1.0).double()
         M = (float(beta) ** ham.double()) * sign[None, :]  # (a, k)
-        out[..., i] = float(alpha) * torch.einsum("ak,jok->joa", M, l64)
+        half = float(alpha) * torch.einsum("ak,jok->joa", M, l64)
+        out[:, :, a, i] = half
+        out[:, :, a ^ (1 << i), i] = half
     return out
 
 
