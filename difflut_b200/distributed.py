@@ -5,6 +5,7 @@ blocks; every rank holds the full tables and index maps; the only exchange per s
 all-reduce of the flat table-gradient buffer.  Inference shards rows with no communication.
 """
 
+import atexit
 import datetime
 import os
 from typing import Optional, Tuple
@@ -31,9 +32,19 @@ def init_from_env(backend: Optional[str] = None, timeout_s: float = 180.0) -> Tu
                                     timeout=datetime.timedelta(seconds=timeout_s))
         else:
             dist.init_process_group(backend, timeout=datetime.timedelta(seconds=timeout_s))
+            atexit.register(_leave_group)
     elif torch.cuda.is_available():
         torch.cuda.set_device(local)
     return rank, world, local
+
+
+def _leave_group() -> None:
+    """A gloo group's threads end before the interpreter does (a rank that exits with them running aborts)."""
+    try:
+        if dist.is_initialized():
+            dist.destroy_process_group()
+    except Exception:
+        pass  # the peers may be gone already
 
 
 def shard_rows(total_rows: int, rank: int, world: int) -> Tuple[int, int]:
