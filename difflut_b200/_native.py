@@ -6,6 +6,7 @@ into RuntimeError (the reference's bindings raise RuntimeError through TORCH_CHE
 difflut/nodes/cuda/efd_cuda.cpp:18-40).
 """
 
+import contextlib
 import ctypes
 import os
 
@@ -86,6 +87,11 @@ SIGNATURES = {
     "dl_adam_advance": "pff s",
     "dl_adam_apply": "ppppplfffff s",
     "dl_adam_step_groups": "ppllpppplfffff s",
+    "dl_dropout": "pplldllp s",
+    "dl_counter_draw": "pp s",
+    "dl_embedding": "plppllllf s",
+    "dl_embedding_bwd_scratch_bytes": "llll",
+    "dl_embedding_bwd": "plppllllflp s",
 }
 
 _CT = {"p": ctypes.c_void_p, "l": ctypes.c_int64, "i": ctypes.c_int, "f": ctypes.c_float, "d": ctypes.c_double}
@@ -112,6 +118,7 @@ def lib():
             args.append(ctypes.c_void_p)
         fn.argtypes = args
         fn.restype = ctypes.c_int
+    handle.dl_embedding_bwd_scratch_bytes.restype = ctypes.c_int64
     handle.dl_version.restype = ctypes.c_int
     handle.dl_error_string.restype = ctypes.c_char_p
     handle.dl_error_string.argtypes = [ctypes.c_int]
@@ -153,6 +160,39 @@ def _ptr(a):
             raise RuntimeError("difflut_b200 kernels take contiguous tensors")
         return a.data_ptr()
     return int(a)
+
+
+# element types of the entry points that take more than fp32 (DL_DTYPE_* of the header)
+DTYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def dtype_code(t: torch.Tensor, what: str) -> int:
+    code = DTYPE_CODES.get(t.dtype)
+    if code is None:
+        raise TypeError(f"{what} must be float32, bfloat16 or float16, got {t.dtype}")
+    return code
+
+
+def require_cuda(what: str, *tensors) -> None:
+    """Every given tensor is on one CUDA device (None is skipped); RuntimeError otherwise."""
+    device = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise RuntimeError(f"difflut_b200.{what} runs on CUDA tensors only (no CPU fallback)")
+        if device is None:
+            device = t.device
+        elif t.device != device:
+            raise RuntimeError(f"difflut_b200.{what}: tensors are on {device} and {t.device}")
+
+
+_SAME_DEVICE = contextlib.nullcontext()
+
+
+def device_of(t: torch.Tensor):
+    """Context in which t's device is the current one (free when it already is)."""
+    return _SAME_DEVICE if torch.cuda.current_device() == t.device.index else torch.cuda.device(t.device)
 
 
 def host_floats(values):

@@ -1,6 +1,8 @@
-"""Encoders of the hot path: the thermometer encoder and its base class."""
+"""Encoders: thermometer (real features), embedding (token ids) and their base class."""
 
 from .base_encoder import BaseEncoder
+from .embedding import EmbeddingEncoder, embedding_lookup
 from .thermometer import DistributiveThermometerEncoder, GaussianThermometerEncoder, ThermometerEncoder
 
-__all__ = ["BaseEncoder", "ThermometerEncoder", "GaussianThermometerEncoder", "DistributiveThermometerEncoder"]
+__all__ = ["BaseEncoder", "ThermometerEncoder", "GaussianThermometerEncoder", "DistributiveThermometerEncoder",
+           "EmbeddingEncoder", "embedding_lookup"]

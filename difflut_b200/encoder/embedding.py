@@ -1,0 +1,122 @@
+"""Embedding encoder: token ids -> `num_bits` learned features per token.
+
+The thermometer encoders turn real features into bits; for token ids or other categorical features the features
+themselves are learned.  LUT nodes read them the way they read any layer input (`value >= 0.5` for DWN-type nodes,
+a probability for Probabilistic nodes) and their input gradient trains the table.  No counterpart in the reference
+(its encoders take real features; the interface is difflut/encoder/base_encoder.py:18-137).
+"""
+
+from typing import Optional
+
+import torch
+import torch.nn as nn
+from torch.autograd.function import once_differentiable
+
+from .. import _native
+from ..registry import register_encoder
+from .base_encoder import BaseEncoder
+
+DEFAULT_EMBEDDING_NUM_BITS: int = 8
+
+
+def _forward(ids: torch.Tensor, weight: torch.Tensor, scale: float) -> torch.Tensor:
+    V, D = weight.shape
+    out = torch.empty(*ids.shape, D, device=weight.device, dtype=weight.dtype)
+    with _native.device_of(weight):
+        _native.call("dl_embedding", ids, 64 if ids.dtype == torch.int64 else 32, weight, out, ids.numel(), V, D,
+                     _native.DTYPE_CODES[weight.dtype], scale)
+    return out
+
+
+class _EmbeddingFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, ids, weight, scale, padding):
+        ctx.save_for_backward(ids)
+        ctx.spec = (weight.shape, weight.dtype, scale, padding)
+        return _forward(ids, weight, scale)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        (ids,) = ctx.saved_tensors
+        (V, D), dtype, scale, padding = ctx.spec
+        g = g.contiguous()
+        code, tokens = _native.DTYPE_CODES[dtype], ids.numel()
+        gw = torch.empty(V, D, device=g.device, dtype=dtype)
+        size = int(_native.lib().dl_embedding_bwd_scratch_bytes(tokens, V, D, code))
+        if size == 0:
+            raise RuntimeError(f"embedding gradient of {tokens} tokens into a {V} x {D} table is not supported")
+        with _native.device_of(g):
+            scratch = torch.empty(size, device=g.device, dtype=torch.uint8)
+            _native.call("dl_embedding_bwd", ids, 64 if ids.dtype == torch.int64 else 32, g, gw, tokens, V, D, code,
+                         scale, padding, scratch)
+        return None, gw, None, None
+
+
+def embedding_lookup(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0,
+                     padding_idx: Optional[int] = None) -> torch.Tensor:
+    """`scale * weight[ids]`, shape `ids.shape + (D,)`, in weight's type (float32, bfloat16 or float16).
+
+    The gradient of `weight` sums the rows of equal ids in the order of their positions, in fp32, rounded once: the
+    same bits on every run.  `padding_idx` takes no gradient.  An id outside [0, V) gives a NaN row and takes no
+    gradient (torch raises a device assertion; nothing is read outside the table here)."""
+    if not isinstance(ids, torch.Tensor) or ids.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"ids must be an int32 or int64 tensor, got {getattr(ids, 'dtype', type(ids))}")
+    if weight.dim() != 2 or weight.shape[0] == 0 or weight.shape[1] == 0:
+        raise ValueError(f"weight must be a non-empty (num_embeddings, features) matrix, got shape {tuple(weight.shape)}")
+    _native.dtype_code(weight, "weight")
+    _native.require_cuda("embedding_lookup", ids, weight)
+    V = weight.shape[0]
+    padding = -1
+    if padding_idx is not None:
+        if not -V <= padding_idx < V:
+            raise ValueError(f"padding_idx must be within [-{V}, {V}), got {padding_idx}")
+        padding = int(padding_idx) % V
+    ids, weight = ids.contiguous(), weight.contiguous()
+    if weight.requires_grad and torch.is_grad_enabled():
+        return _EmbeddingFn.apply(ids, weight, float(scale), padding)
+    return _forward(ids, weight, float(scale))
+
+
+@register_encoder("embedding")
+class EmbeddingEncoder(BaseEncoder):
+    """Token ids (B, T) -> (B, T * num_bits) if `flatten` else (B, T, num_bits); a 1-D input is one sample.
+
+    `weight` (num_embeddings, num_bits) starts uniform such that the scaled features lie in [0, 1), half of them
+    above the 0.5 that DWN-type nodes threshold at.  There is nothing to fit: `fit` only returns the encoder."""
+
+    def __init__(self, num_embeddings: int, num_bits: int = DEFAULT_EMBEDDING_NUM_BITS, scale: float = 1.0,
+                 padding_idx: Optional[int] = None, flatten: bool = True,
+                 dtype: torch.dtype = torch.float32) -> None:
+        super().__init__(num_bits=num_bits, flatten=flatten)
+        if not isinstance(num_embeddings, int) or num_embeddings <= 0:
+            raise ValueError(f"num_embeddings must be a positive integer, got {num_embeddings}")
+        if not isinstance(scale, (int, float)) or not scale > 0:
+            raise ValueError(f"scale must be a positive number, got {scale}")
+        if padding_idx is not None and not -num_embeddings <= padding_idx < num_embeddings:
+            raise ValueError(f"padding_idx must be within [-{num_embeddings}, {num_embeddings}), got {padding_idx}")
+        if dtype not in _native.DTYPE_CODES:
+            raise TypeError(f"dtype must be float32, bfloat16 or float16, got {dtype}")
+        self.num_embeddings, self.scale, self.padding_idx = num_embeddings, float(scale), padding_idx
+        self.weight = nn.Parameter((torch.rand(num_embeddings, self.num_bits) / self.scale).to(dtype))
+        if padding_idx is not None:
+            with torch.no_grad():
+                self.weight[padding_idx] = 0.0
+        self._is_fitted = True
+
+    def fit(self, x=None) -> "EmbeddingEncoder":
+        return self
+
+    def encode(self, x) -> torch.Tensor:
+        ids = self._to_tensor(x)
+        out = embedding_lookup(ids, self.weight, self.scale, self.padding_idx)
+        if not self.flatten:
+            return out
+        return out.reshape(-1) if ids.dim() <= 1 else out.reshape(ids.shape[0], -1)
+
+    def to(self, *args, **kwargs) -> "EmbeddingEncoder":
+        return nn.Module.to(self, *args, **kwargs)  # the table is a parameter, not a plain attribute
+
+    def __repr__(self) -> str:
+        return (f"EmbeddingEncoder(num_embeddings={self.num_embeddings}, num_bits={self.num_bits}, "
+                f"scale={self.scale}, padding_idx={self.padding_idx}, flatten={self.flatten})")

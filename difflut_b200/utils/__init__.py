@@ -1,5 +1,6 @@
-"""Utility modules (GroupSum) and warning helpers."""
+"""Utility modules (GroupSum, Dropout) and warning helpers."""
 
+from .dropout import Dropout, dropout
 from .modules import GroupSum
 from .warnings import (
     ConfigurationWarning,

@@ -44,6 +44,9 @@ enum {
 #define DL_MAX_FAST_N 6    /* n <= 6: tables are 64-bit words / 32-lane shuffles */
 #define DL_STATIC_SCRATCH_BYTES (16 << 20) /* built-in scratch of dl_dwn_fwd_groupsum_noalloc_t */
 
+/* element types of the entry points that take more than fp32 */
+enum { DL_DTYPE_F32 = 0, DL_DTYPE_BF16 = 1, DL_DTYPE_F16 = 2 };
+
 int dl_version(void);
 const char* dl_error_string(int code);
 int64_t dl_padded_batch(int64_t B);
@@ -526,6 +529,36 @@ int dl_adam_step_groups(float* p, const float* partial, int64_t stride, int64_t 
  * (difflut/nodes/dwn_node.py:457-483, difflut/utils/modules.py:158-163).                   */
 int dl_popcount_groupsum_t(const uint32_t* bits_t, int32_t* counts, int64_t N, int64_t k, int64_t B,
                            int64_t Bp, dl_stream_t stream);
+
+/* ------------------------------------------------------------------ dropout
+ * No counterpart in the reference (its only random regulariser is the bit flip,
+ * difflut/layers/base_layer.py:189-262).  out[i] = x[i] / (1 - p), or 0 when word i % 4 of
+ * Philox4x32-10(counter = (i / 4, offset), key = seed) is below p * 2^32 (rounded).  Products in
+ * fp32, rounded once.  The mask is never stored: the gradient of the input is the same call on the
+ * gradient of the output.  `counter` (optional, one int64) is added to `offset` when the kernel
+ * runs, so a captured graph can draw a new mask per replay: dl_counter_draw writes *counter to
+ * *drawn and increments it.  x == out is allowed; no alignment beyond the element's own is needed. */
+int dl_dropout(const void* x, void* out, int64_t count, int64_t dtype, double p, int64_t seed, int64_t offset,
+               const int64_t* counter, dl_stream_t stream);
+int dl_counter_draw(int64_t* counter, int64_t* drawn, dl_stream_t stream);
+
+/* ------------------------------------------------------------------ embedding
+ * No counterpart in the reference (its encoders take real features).
+ * ids (tokens) int32 or int64 (id_bits 32 or 64), weight (V, D), out / g (tokens, D), gw (V, D), all of
+ * one element type; products and sums in fp32, rounded once.
+ *   dl_embedding       out[t] = scale * weight[ids[t]]; an id outside [0, V) gives a NaN row.
+ *   dl_embedding_bwd   gw[v] = scale * sum of g[t] over ids[t] == v in ascending t; every row of gw is
+ *                      written, 0 where no token has that id; ids outside [0, V) and `padding_idx`
+ *                      (-1: none) take no gradient.  The order of the additions is a function of the
+ *                      sizes and ids alone: run-to-run the same bits.  scratch:
+ *                      dl_embedding_bwd_scratch_bytes bytes (0 = sizes not supported), 256-byte aligned;
+ *                      tokens, V and D below 2^31.                                              */
+int dl_embedding(const void* ids, int64_t id_bits, const void* weight, void* out, int64_t tokens, int64_t V,
+                 int64_t D, int64_t dtype, float scale, dl_stream_t stream);
+int64_t dl_embedding_bwd_scratch_bytes(int64_t tokens, int64_t V, int64_t D, int64_t dtype);
+int dl_embedding_bwd(const void* ids, int64_t id_bits, const void* g, void* gw, int64_t tokens, int64_t V,
+                     int64_t D, int64_t dtype, float scale, int64_t padding_idx, void* scratch,
+                     dl_stream_t stream);
 
 #ifdef __cplusplus
 }

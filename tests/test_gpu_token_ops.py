@@ -1,0 +1,318 @@
+"""Token-path operators on the GPU against plain 64-bit forms, at the sizes and values where they can go wrong.
+
+Bounds: a rounding to type t is off by at most half a step (eps / 2 relative); fp32 sums of n terms by at most
+n * 2^-24 of the sum of absolute terms.
+"""
+
+import copy
+
+import pytest
+import torch
+
+from difflut_b200.encoder import EmbeddingEncoder, embedding_lookup
+from difflut_b200.utils import Dropout, dropout
+from token_util import TYPES, check, dropped, embedding_grad, half_step, smallest
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+U32 = 2.0 ** -24
+
+
+def _normal(*shape, dtype=torch.float32, seed=0):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed)).to(dtype).to(DEV)
+
+
+# ---------------------------------------------------------------------------------------------- dropout
+def _check_dropout(y, x, p, seed, offset, what):
+    gone = dropped(x.numel(), p, seed, offset).view(x.shape)
+    scale = 1.0 / (1.0 - p) if p < 1.0 else 0.0
+    ref = torch.where(gone, torch.zeros((), dtype=torch.float64), x.detach().double().cpu() * scale)
+    # scale and product are rounded to fp32, the result to the type
+    check(y, ref, ref.abs() * (half_step(x.dtype) + 2 * U32 * 1.01) + smallest(x.dtype), what)
+    assert bool((y.detach().cpu()[gone] == 0).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("numel", [1, 3, 4, 5, 31, 255, 2048, 2049, 4096 + 7, 100003])
+def test_dropout_forward_and_gradient(dtype, numel):
+    x = _normal(numel, dtype=dtype, seed=numel).requires_grad_(True)
+    seed, offset = 0x1234567890ABCDEF, (3 << 32) + 5
+    y = dropout(x, 0.3, seed=seed, offset=offset)
+    _check_dropout(y, x, 0.3, seed, offset, "forward")
+    g = _normal(numel, dtype=dtype, seed=numel + 1)
+    (gx,) = torch.autograd.grad(y, x, g)
+    _check_dropout(gx, g, 0.3, seed, offset, "gradient")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shift", [1, 2, 3, 5])
+def test_dropout_at_any_alignment(dtype, shift):
+    """The mask belongs to the element's index in the tensor, not to its address."""
+    x = _normal(1000 + shift, dtype=dtype)[shift:]
+    _check_dropout(dropout(x, 0.5, seed=9), x, 0.5, 9, 0, "shifted")
+
+
+@pytest.mark.parametrize("p", [0.0, 2.0 ** -34, 1e-9, 0.999999, 1.0 - 2.0 ** -40, 1.0])
+def test_dropout_extreme_probabilities(p):
+    x = _normal(4099).requires_grad_(True)
+    y = dropout(x, p, seed=1)
+    _check_dropout(y, x, p, 1, 0, f"p={p}")
+    (gx,) = torch.autograd.grad(y, x, torch.ones_like(y))
+    _check_dropout(gx, torch.ones(4099), p, 1, 0, f"gradient p={p}")
+
+
+def test_dropout_of_values_that_are_not_numbers():
+    """Dropped positions are exactly 0 whatever they held; kept ones keep infinities and NaN."""
+    x = torch.tensor([float("inf"), float("-inf"), float("nan"), 1.0], device=DEV).repeat(256)
+    y = dropout(x, 0.5, seed=3).cpu()
+    gone = dropped(1024, 0.5, 3, 0)
+    assert bool((y[gone] == 0).all())
+    kept = torch.tensor([float("inf"), float("-inf"), float("nan"), 2.0]).repeat(256)[~gone]
+    assert torch.equal(torch.nan_to_num(y[~gone], nan=7.0), torch.nan_to_num(kept, nan=7.0))
+
+
+def test_dropout_strides_and_empty():
+    x = _normal(64, 48)
+    _check_dropout(dropout(x.t(), 0.25, seed=2), x.t().contiguous(), 0.25, 2, 0, "transposed")
+    e = torch.empty(0, 5, device=DEV, requires_grad=True)
+    assert torch.autograd.grad(dropout(e, 0.5), e, e.detach())[0].shape == (0, 5)
+    xg = x.clone().requires_grad_(True)  # an expanded gradient
+    (gx,) = torch.autograd.grad(dropout(xg, 0.25, seed=2).sum(), xg)
+    _check_dropout(gx, torch.ones(64, 48), 0.25, 2, 0, "expanded gradient")
+
+
+def test_dropout_second_derivative_is_the_same_mask():
+    x = _normal(500).requires_grad_(True)
+    (gx,) = torch.autograd.grad(dropout(x, 0.5, seed=4).pow(2).sum(), x, create_graph=True)
+    (gg,) = torch.autograd.grad(gx.sum(), x)
+    gone = dropped(500, 0.5, 4, 0)
+    assert torch.equal(gg.cpu(), torch.where(gone, 0.0, 8.0))
+
+
+def test_dropout_word_index_past_32_bits():
+    """The high counter word: elements from 2^34 on take other words than the ones 2^34 below (bytes would be 32 GB, so
+    the counter is moved instead: the offset's words sit beside it in the same block)."""
+    x = torch.ones(4096, device=DEV)
+    a, b = dropout(x, 0.5, seed=5, offset=1), dropout(x, 0.5, seed=5, offset=1 << 32)
+    assert not torch.equal(a, b)
+    _check_dropout(b, x, 0.5, 5, 1 << 32, "high offset")
+
+
+def test_dropout_counter_on_the_device():
+    x = _normal(4096).requires_grad_(True)
+    counter = torch.tensor([7], device=DEV, dtype=torch.int64)
+    y = dropout(x, 0.5, seed=6, offset=10, counter=counter)
+    _check_dropout(y, x, 0.5, 6, 17, "counter")
+    (gx,) = torch.autograd.grad(y, x, torch.ones_like(y))
+    _check_dropout(gx, torch.ones(4096), 0.5, 6, 17, "counter gradient")
+    with pytest.raises(TypeError):
+        dropout(x, 0.5, counter=counter.int())
+    z = dropout(x, 0.5, seed=6, counter=counter)
+    counter.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(z, x, torch.ones_like(z))
+
+
+def test_dropout_module_draws_a_mask_per_call_and_repeats_under_a_seed():
+    d, x = Dropout(0.5).train(), torch.ones(4096, device=DEV)
+    torch.manual_seed(11)
+    a, b = d(x), d(x)
+    assert not torch.equal(a, b)
+    torch.manual_seed(11)
+    e = copy.deepcopy(Dropout(0.5).train())
+    first = e(x)  # also creates the counter, from a draw of its own
+    assert 0.4 < float((a == 0).float().mean()) < 0.6 and 0.4 < float((first == 0).float().mean()) < 0.6
+
+
+def test_dropout_module_in_a_captured_graph_draws_a_mask_per_replay():
+    d, x = Dropout(0.5).train(), torch.ones(4096, device=DEV, requires_grad=True)
+    fresh = Dropout(0.5).train()
+    d(x)
+    with torch.no_grad():
+        fresh_error = None
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        try:
+            fresh(x)
+        except RuntimeError as e:
+            fresh_error = str(e)
+        y = d(x)
+        (gx,) = torch.autograd.grad(y, x, torch.ones_like(y))
+    assert "before capturing" in fresh_error
+    seen = []
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal((y == 0), (gx == 0))
+        seen.append(y.detach().clone())
+    assert not torch.equal(seen[0], seen[1]) and not torch.equal(seen[1], seen[2])
+
+
+def test_dropout_on_another_stream():
+    x = _normal(1 << 20)
+    want = dropout(x, 0.5, seed=8)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = dropout(x, 0.5, seed=8)
+    s.synchronize()
+    assert torch.equal(got, want)
+
+
+# ---------------------------------------------------------------------------------------------- embedding
+def _ids(T, V, seed, kind="zipf"):
+    g = torch.Generator().manual_seed(seed)
+    if kind == "one":
+        return torch.full((T,), V // 2)
+    if kind == "runs":  # segments of many lengths
+        return (torch.arange(T) * torch.arange(T) // max(1, T)) % V
+    u = torch.rand(T, generator=g, dtype=torch.float64)
+    if kind == "uniform":
+        return (u * V).long()
+    return (torch.exp(u * torch.log(torch.tensor(V + 1.0, dtype=torch.float64))) - 1).long().clamp(0, V - 1)
+
+
+def _check_embedding(T, V, D, dtype, kind="zipf", scale=1.7, padding=None, ids=None, ids_dtype=torch.int64):
+    ids = (_ids(T, V, T + V, kind) if ids is None else ids).to(ids_dtype).to(DEV)
+    W = _normal(V, D, dtype=dtype, seed=1).requires_grad_(True)
+    g = _normal(*ids.shape, D, dtype=dtype, seed=2)
+    s32 = float(torch.tensor(scale, dtype=torch.float32))
+    out = embedding_lookup(ids, W, scale=scale, padding_idx=padding)
+    ok = (ids >= 0) & (ids < V)
+    ref = W.detach().double()[torch.where(ok, ids, 0).long()] * s32
+    check(out[ok], ref[ok], ref[ok].abs().cpu() * (half_step(dtype) + U32 * 1.01) + smallest(dtype), "lookup")
+    assert bool(torch.isnan(out[~ok]).all())
+    (gW,) = torch.autograd.grad(out, W, g)
+    want, size, n = embedding_grad(ids, g, V, s32, padding)
+    # n additions and one product in fp32, then the rounding to the type
+    check(gW, want, size * (n + 1) * U32 * 1.01 + want.abs() * half_step(dtype) * 1.01 + smallest(dtype), "table gradient")
+    assert bool((gW.cpu()[(n == 0).reshape(-1)] == 0).all())
+    return ids, W, g, gW
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,V,D", [(1, 1, 1), (1, 7, 8), (2, 300, 3), (33, 5, 16), (257, 1000, 36), (1000, 255, 130),
+                                   (1000, 256, 64), (5000, 65535, 24), (700, 40, 515), (37, 10, 1100)])
+def test_embedding_sizes(T, V, D, dtype):
+    _check_embedding(T, V, D, dtype)
+
+
+@pytest.mark.parametrize("kind", ["one", "runs", "uniform"])
+@pytest.mark.parametrize("T", [31, 4096, 4097, 9001, 33000])
+def test_embedding_distributions(kind, T):
+    """One id for all tokens (a segment over every range), segments of many lengths, and mostly single tokens; one
+    sorting block, two, and the whole cluster with several tiles per block."""
+    _check_embedding(T, 700, 16, torch.float32, kind)
+
+
+def test_embedding_long_ranges_of_one_id():
+    """So many tokens that a range holds more than 32 of them."""
+    _check_embedding(60000, 3, 520, torch.bfloat16, "uniform")
+
+
+@pytest.mark.parametrize("ids_dtype", [torch.int32, torch.int64])
+def test_embedding_ids_that_do_not_exist(ids_dtype):
+    """They give NaN rows, take no gradient, and nothing else changes; padding keeps its row and takes none either."""
+    ids = torch.tensor([3, -1, 0, 10, 9, 2147483647, -2147483648, 3, 0, 5])
+    _check_embedding(0, 10, 12, torch.float32, ids=ids, padding=0, ids_dtype=ids_dtype)
+    _check_embedding(0, 10, 12, torch.float32, ids=torch.full((50,), -7), ids_dtype=ids_dtype)
+    if ids_dtype == torch.int64:
+        _check_embedding(0, 10, 12, torch.float32, ids=torch.tensor([1 << 32, (1 << 32) + 3, 3, -(1 << 40)]))
+
+
+def test_embedding_no_tokens():
+    W = _normal(5, 4).requires_grad_(True)
+    out = embedding_lookup(torch.empty(2, 0, device=DEV, dtype=torch.int64), W)
+    assert out.shape == (2, 0, 4)
+    assert torch.equal(torch.autograd.grad(out, W, out.detach())[0], torch.zeros_like(W))
+
+
+def test_embedding_strided_inputs_and_shifted_table():
+    ids = _ids(600, 50, 3).view(20, 30).t().to(DEV)
+    big = _normal(50, 33)
+    table = big[:, 1:]  # rows that start at odd offsets
+    out = embedding_lookup(ids, table, scale=2.0)
+    assert torch.equal(out, table[ids] * 2.0)
+    flat = _normal(50 * 16 + 1)
+    shifted = flat[1:].view(50, 16)  # contiguous, 4-byte aligned only
+    assert torch.equal(embedding_lookup(ids, shifted), shifted[ids])
+    W = big.clone().requires_grad_(True)
+    (gW,) = torch.autograd.grad(embedding_lookup(ids, W).sum(), W)  # an expanded gradient
+    count = torch.bincount(ids.reshape(-1), minlength=50).float()
+    assert torch.equal(gW, count[:, None].expand(50, 33))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_embedding_gradient_is_the_same_on_every_run(dtype):
+    ids, W, g, first = _check_embedding(20000, 900, 72, dtype)
+    for _ in range(3):
+        (again,) = torch.autograd.grad(embedding_lookup(ids, W, scale=1.7), W, g)
+        assert torch.equal(first, again)
+
+
+def test_embedding_gradient_against_differences():
+    """The lookup is linear in the table: a step in one entry moves the loss by gradient * step exactly."""
+    ids = _ids(200, 30, 1).to(DEV)
+    W = (_normal(30, 8) * 8).round().requires_grad_(True)
+    g = (_normal(200, 8, seed=3) * 8).round()
+    (gW,) = torch.autograd.grad(embedding_lookup(ids, W, scale=0.5), W, g)
+    with torch.no_grad():
+        base = (embedding_lookup(ids, W, scale=0.5).double() * g).sum()
+        for v, d in ((0, 0), (3, 5), (29, 7)):
+            W2 = W.clone()
+            W2[v, d] += 1.0
+            assert float((embedding_lookup(ids, W2, scale=0.5).double() * g).sum() - base) == float(gW[v, d])
+
+
+def test_embedding_captured_and_replayed():
+    ids, W = _ids(3000, 400, 5).to(DEV), _normal(400, 40).requires_grad_(True)
+    g = _normal(3000, 40, seed=6)
+
+    def step():
+        out = embedding_lookup(ids, W, scale=1.5)
+        return out, torch.autograd.grad(out, W, g)[0]
+
+    want = [t.detach().clone() for t in step()]
+    torch.cuda.synchronize()
+    graphs, results = [], []
+    for _ in range(2):  # two graphs, each with a workspace of its own
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            results.append(step())
+        graphs.append(graph)
+    for graph in graphs + graphs:
+        graph.replay()
+    torch.cuda.synchronize()
+    for out, gW in results:
+        assert torch.equal(out, want[0]) and torch.equal(gW, want[1])
+    ids.copy_(ids.flip(0))  # new ids in place: the replay reads them
+    new = [t.detach().clone() for t in step()]
+    graphs[0].replay()
+    torch.cuda.synchronize()
+    assert torch.equal(results[0][0], new[0]) and torch.equal(results[0][1], new[1])
+
+
+def test_embedding_two_streams_at_once():
+    ids, W = _ids(20000, 4000, 5).to(DEV), _normal(4000, 64).requires_grad_(True)
+    g = _normal(20000, 64, seed=6)
+    want = torch.autograd.grad(embedding_lookup(ids, W), W, g)[0]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    got = []
+    for s in streams:
+        with torch.cuda.stream(s):
+            got.append(torch.autograd.grad(embedding_lookup(ids, W), W, g)[0])
+    torch.cuda.synchronize()
+    for x in got:
+        assert torch.equal(x, want)
+
+
+def test_embedding_encoder_trains():
+    enc = EmbeddingEncoder(20, num_bits=6, scale=3.0, padding_idx=0).to(DEV)
+    ids = torch.randint(0, 20, (5, 7), device=DEV)
+    x = enc(ids)
+    assert x.shape == (5, 42) and EmbeddingEncoder(20, num_bits=6, flatten=False).to(DEV)(ids).shape == (5, 7, 6)
+    assert enc(ids[0]).shape == (42,)
+    x.sum().backward()
+    assert float(enc.weight.grad[0].abs().max()) == 0.0 and float(enc.weight.grad[1:].abs().max()) > 0.0

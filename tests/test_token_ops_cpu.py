@@ -1,0 +1,117 @@
+"""Token-path operators without a GPU: refusals, registry, and the plain forms the GPU tests compare against."""
+
+import numpy as np
+import pytest
+import torch
+
+import difflut_b200 as difflut
+from difflut_b200 import _native
+from difflut_b200.encoder import EmbeddingEncoder, embedding_lookup
+from difflut_b200.utils import Dropout, dropout
+from difflut_b200.utils.warnings import DefaultValueWarning
+from token_util import philox
+
+
+def test_philox_known_answers():
+    """The published known-answer vectors of Philox4x32-10."""
+    cases = [((0, 0, 0, 0), (0, 0), (0x6627E8D5, 0xE169C58D, 0xBC57AC4C, 0x9B00DBD8)),
+             ((0xFFFFFFFF,) * 4, (0xFFFFFFFF,) * 2, (0x408F276D, 0x41C83B0E, 0xA20BC7C6, 0x6D5451FD)),
+             ((0x243F6A88, 0x85A308D3, 0x13198A2E, 0x03707344), (0xA4093822, 0x299F31D0),
+              (0xD16CFE09, 0x94FDCCEB, 0x5001E420, 0x24126EA1))]
+    for counter, key, want in cases:
+        got = philox(np.array([counter], dtype=np.uint64), key)[0]
+        assert tuple(int(w) for w in got) == want
+
+
+# ---------------------------------------------------------------------------------------------- embedding
+def test_embedding_encoder_is_registered_and_has_nothing_to_fit():
+    assert difflut.REGISTRY.get_encoder("embedding") is EmbeddingEncoder
+    enc = EmbeddingEncoder(10, num_bits=4, scale=2.0, padding_idx=-1)
+    assert enc.is_fitted and enc.fit(None) is enc
+    assert list(enc.state_dict()) == ["weight"] and enc.weight.shape == (10, 4)
+    assert float(enc.weight[-1].detach().abs().max()) == 0.0
+    scaled = enc.weight.detach()[:-1] * 2.0
+    assert float(scaled.min()) >= 0.0 and float(scaled.max()) < 1.0
+    assert enc.to("cpu") is enc and isinstance(enc.weight, torch.nn.Parameter)
+    assert "padding_idx=-1" in repr(enc)
+
+
+@pytest.mark.parametrize("kwargs", [{"num_embeddings": 0}, {"num_embeddings": 2.5}, {"num_embeddings": 4, "scale": 0.0},
+                                    {"num_embeddings": 4, "scale": float("nan")},
+                                    {"num_embeddings": 4, "padding_idx": 4}, {"num_embeddings": 4, "padding_idx": -5}])
+def test_embedding_encoder_refuses(kwargs):
+    with pytest.raises(ValueError):
+        EmbeddingEncoder(**kwargs)
+
+
+def test_embedding_lookup_refuses():
+    ids, weight = torch.zeros(3, dtype=torch.int64), torch.zeros(4, 2)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        embedding_lookup(ids, weight)
+    with pytest.raises(TypeError, match="int32 or int64"):
+        embedding_lookup(ids.float(), weight)
+    with pytest.raises(TypeError, match="int32 or int64"):
+        embedding_lookup([1, 2], weight)
+    with pytest.raises(TypeError, match="float32, bfloat16 or float16"):
+        embedding_lookup(ids, weight.double())
+    with pytest.raises(ValueError, match="non-empty"):
+        embedding_lookup(ids, weight[0])
+    with pytest.raises(ValueError, match="non-empty"):
+        embedding_lookup(ids, weight[:0])
+    with pytest.raises(TypeError):
+        EmbeddingEncoder(4, dtype=torch.float64)
+
+
+def test_embedding_entry_points_refuse_bad_sizes():
+    lib = _native.lib()
+    assert lib.dl_embedding_bwd_scratch_bytes(100, 10, 8, 0) > 0
+    for bad in ((-1, 10, 8, 0), (100, 0, 8, 0), (100, 10, 0, 0), (100, 10, 8, 3), (1 << 31, 10, 8, 0),
+                (100, 1 << 31, 8, 0)):
+        assert lib.dl_embedding_bwd_scratch_bytes(*bad) == 0
+    assert lib.dl_embedding(None, 64, None, None, 3, 4, 2, 0, 1.0, None) == -1
+    assert lib.dl_embedding(None, 64, None, None, 0, 4, 2, 0, 1.0, None) == 0
+    assert lib.dl_embedding(None, 16, None, None, 0, 4, 2, 0, 1.0, None) == -1
+    assert lib.dl_embedding(8, 64, 18, 16, 3, 4, 2, 0, 1.0, None) == -4  # fp32 table at an odd half word
+    assert lib.dl_embedding_bwd(8, 64, 16, 16, 3, 4, 2, 0, 1.0, -1, 64, None) == -4  # scratch not 256-byte aligned
+    assert lib.dl_embedding_bwd(8, 64, 16, 16, 1 << 31, 4, 2, 0, 1.0, -1, 256, None) == -5
+
+
+# ---------------------------------------------------------------------------------------------- dropout
+def test_dropout_refuses():
+    x = torch.zeros(8)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        dropout(x, 0.5)
+    for p in (-0.1, 1.5, float("nan"), "0.5", True):
+        with pytest.raises(ValueError, match="probability"):
+            dropout(x, p)
+    for name in ("seed", "offset"):
+        for value in (-1, 1 << 63, 0.5, True):
+            with pytest.raises(ValueError, match=name):
+                dropout(x, 0.5, **{name: value})
+    with pytest.raises(TypeError, match="float32, bfloat16 or float16"):
+        dropout(x.double(), 0.5)
+
+
+def test_dropout_module_host_side():
+    import copy
+
+    with pytest.warns(DefaultValueWarning):
+        assert Dropout().p == 0.5
+    with pytest.raises(ValueError):
+        Dropout(2.0)
+    d = Dropout(0.3)
+    x = torch.ones(3)
+    assert d.eval()(x) is x and Dropout(0.0).train()(x) is x
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        d.train()(x)
+    assert copy.deepcopy(d).p == 0.3 and list(d.state_dict()) == []
+
+
+def test_dropout_entry_points_refuse():
+    lib = _native.lib()
+    assert lib.dl_dropout(None, None, 0, 0, 0.5, 1, 0, None, None) == 0
+    assert lib.dl_dropout(None, None, 4, 0, 0.5, 1, 0, None, None) == -1
+    assert lib.dl_dropout(None, None, 0, 0, 1.5, 1, 0, None, None) == -1
+    assert lib.dl_dropout(None, None, 0, 7, 0.5, 1, 0, None, None) == -1
+    assert lib.dl_dropout(6, 8, 4, 0, 0.5, 1, 0, None, None) == -4
+    assert lib.dl_counter_draw(None, None, None) == -1
