@@ -89,9 +89,10 @@ SIGNATURES = {
     "dl_adam_step_groups": "ppllpppplfffff s",
     "dl_dropout": "pplldllp s",
     "dl_counter_draw": "pp s",
-    "dl_embedding": "plppllllf s",
+    "dl_embedding_order_bytes": "llll",
+    "dl_embedding": "plppllllflp s",
     "dl_embedding_bwd_scratch_bytes": "llll",
-    "dl_embedding_bwd": "plppllllflp s",
+    "dl_embedding_bwd": "pppllllfp s",
 }
 
 _CT = {"p": ctypes.c_void_p, "l": ctypes.c_int64, "i": ctypes.c_int, "f": ctypes.c_float, "d": ctypes.c_double}
@@ -118,6 +119,7 @@ def lib():
             args.append(ctypes.c_void_p)
         fn.argtypes = args
         fn.restype = ctypes.c_int
+    handle.dl_embedding_order_bytes.restype = ctypes.c_int64
     handle.dl_embedding_bwd_scratch_bytes.restype = ctypes.c_int64
     handle.dl_version.restype = ctypes.c_int
     handle.dl_error_string.restype = ctypes.c_char_p
@@ -221,7 +223,8 @@ def call(name: str, *args, stream=None):
         raise TypeError(f"{name}: expected {len(kinds)} arguments, got {len(args)}")
     conv = [_ptr(a) if kind == "p" else (int(a) if kind in ("l", "i") else float(a)) for kind, a in zip(kinds, args)]
     if has_stream:
-        conv.append(torch.cuda.current_stream().cuda_stream if stream is None else stream)
+        # the current stream of the current device, without building a Stream object around it (3 us of a call)
+        conv.append(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()) if stream is None else stream)
     code = fn(*conv)
     if code != 0:
         raise RuntimeError(f"{name} failed: {lib().dl_error_string(code).decode()} (code {code})")

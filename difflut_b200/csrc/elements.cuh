@@ -5,9 +5,9 @@
 
 #include "common.cuh"
 
-// N elements of T that are loaded and stored as one access (N * sizeof(T) is 2, 4, 8 or 16 bytes)
+// N elements of T that are loaded and stored as one access (N * sizeof(T) is 2, 4, 8 or 16 bytes; 32 are two)
 template <typename T, int N>
-struct __align__(sizeof(T) * N) DlVec {
+struct __align__(sizeof(T) * N < 16 ? sizeof(T) * N : 16) DlVec {
     T v[N];
 };
 
@@ -23,6 +23,70 @@ template <>
 __device__ __forceinline__ __nv_bfloat16 dl_from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 template <>
 __device__ __forceinline__ __half dl_from_float<__half>(float x) { return __float2half_rn(x); }
+
+// A whole vector to and from fp32; 16-bit types go through the two-element conversions (one instruction a pair).
+template <int N>
+__device__ __forceinline__ void dl_unpack(const DlVec<float, N>& x, float (&f)[N]) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) f[e] = x.v[e];
+}
+template <int N>
+__device__ __forceinline__ void dl_unpack(const DlVec<__nv_bfloat16, N>& x, float (&f)[N]) {
+    if constexpr (N == 1) {
+        f[0] = __bfloat162float(x.v[0]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; e += 2) {
+            const float2 p = __bfloat1622float2(__nv_bfloat162(x.v[e], x.v[e + 1]));
+            f[e] = p.x;
+            f[e + 1] = p.y;
+        }
+    }
+}
+template <int N>
+__device__ __forceinline__ void dl_unpack(const DlVec<__half, N>& x, float (&f)[N]) {
+    if constexpr (N == 1) {
+        f[0] = __half2float(x.v[0]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; e += 2) {
+            const float2 p = __half22float2(__half2(x.v[e], x.v[e + 1]));
+            f[e] = p.x;
+            f[e + 1] = p.y;
+        }
+    }
+}
+template <int N>
+__device__ __forceinline__ void dl_pack(const float (&f)[N], DlVec<float, N>& x) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) x.v[e] = f[e];
+}
+template <int N>
+__device__ __forceinline__ void dl_pack(const float (&f)[N], DlVec<__nv_bfloat16, N>& x) {
+    if constexpr (N == 1) {
+        x.v[0] = __float2bfloat16_rn(f[0]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; e += 2) {
+            const __nv_bfloat162 p = __floats2bfloat162_rn(f[e], f[e + 1]);
+            x.v[e] = p.x;
+            x.v[e + 1] = p.y;
+        }
+    }
+}
+template <int N>
+__device__ __forceinline__ void dl_pack(const float (&f)[N], DlVec<__half, N>& x) {
+    if constexpr (N == 1) {
+        x.v[0] = __float2half_rn(f[0]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; e += 2) {
+            const __half2 p = __floats2half2_rn(f[e], f[e + 1]);
+            x.v[e] = p.x;
+            x.v[e + 1] = p.y;
+        }
+    }
+}
 
 // element `i` of an array whose type is one of DL_DTYPE_*, as fp32
 __device__ __forceinline__ float dl_load_as_float(const void* p, int dtype, int64_t i) {

@@ -19,37 +19,42 @@ from .base_encoder import BaseEncoder
 DEFAULT_EMBEDDING_NUM_BITS: int = 8
 
 
-def _forward(ids: torch.Tensor, weight: torch.Tensor, scale: float) -> torch.Tensor:
+def _forward(ids, weight, scale, padding, sort):
+    """(looked-up rows, the sorted tokens that the backward pass wants or None)."""
     V, D = weight.shape
-    out = torch.empty(*ids.shape, D, device=weight.device, dtype=weight.dtype)
+    code, tokens = _native.DTYPE_CODES[weight.dtype], ids.numel()
+    out = torch.empty(ids.shape + (D,), device=weight.device, dtype=weight.dtype)
+    order = None
+    if sort:
+        size = int(_native.lib().dl_embedding_order_bytes(tokens, V, D, code))
+        if size == 0:
+            raise RuntimeError(f"the gradient of {tokens} tokens into a {V} x {D} table is not supported")
+        order = torch.empty(size, device=weight.device, dtype=torch.uint8)
     with _native.device_of(weight):
-        _native.call("dl_embedding", ids, 64 if ids.dtype == torch.int64 else 32, weight, out, ids.numel(), V, D,
-                     _native.DTYPE_CODES[weight.dtype], scale)
-    return out
+        _native.call("dl_embedding", ids, 64 if ids.dtype == torch.int64 else 32, weight, out, tokens, V, D, code, scale,
+                     padding, order)
+    return out, order
 
 
 class _EmbeddingFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, ids, weight, scale, padding):
-        ctx.save_for_backward(ids)
-        ctx.spec = (weight.shape, weight.dtype, scale, padding)
-        return _forward(ids, weight, scale)
+        out, order = _forward(ids, weight, scale, padding, True)
+        ctx.save_for_backward(order)
+        ctx.spec = (ids.numel(), weight.shape, weight.dtype, scale)
+        return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
-        (ids,) = ctx.saved_tensors
-        (V, D), dtype, scale, padding = ctx.spec
-        g = g.contiguous()
-        code, tokens = _native.DTYPE_CODES[dtype], ids.numel()
+        (order,) = ctx.saved_tensors
+        tokens, (V, D), dtype, scale = ctx.spec
+        code = _native.DTYPE_CODES[dtype]
         gw = torch.empty(V, D, device=g.device, dtype=dtype)
         size = int(_native.lib().dl_embedding_bwd_scratch_bytes(tokens, V, D, code))
-        if size == 0:
-            raise RuntimeError(f"embedding gradient of {tokens} tokens into a {V} x {D} table is not supported")
+        scratch = torch.empty(size, device=g.device, dtype=torch.uint8)
         with _native.device_of(g):
-            scratch = torch.empty(size, device=g.device, dtype=torch.uint8)
-            _native.call("dl_embedding_bwd", ids, 64 if ids.dtype == torch.int64 else 32, g, gw, tokens, V, D, code,
-                         scale, padding, scratch)
+            _native.call("dl_embedding_bwd", order, g.contiguous(), gw, tokens, V, D, code, scale, scratch)
         return None, gw, None, None
 
 
@@ -75,7 +80,7 @@ def embedding_lookup(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0
     ids, weight = ids.contiguous(), weight.contiguous()
     if weight.requires_grad and torch.is_grad_enabled():
         return _EmbeddingFn.apply(ids, weight, float(scale), padding)
-    return _forward(ids, weight, float(scale))
+    return _forward(ids, weight, float(scale), padding, False)[0]
 
 
 @register_encoder("embedding")

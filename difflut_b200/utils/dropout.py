@@ -35,9 +35,7 @@ class _DropoutFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, p, seed, offset, counter):
         ctx.rule = (p, seed, offset)
-        if counter is None:
-            ctx.counter = None
-        else:
+        if counter is not None:
             ctx.save_for_backward(counter)
         ctx.drawn = counter is not None
         return _apply_mask(x, p, seed, offset, counter)
@@ -46,7 +44,10 @@ class _DropoutFn(torch.autograd.Function):
     def backward(ctx, g):
         p, seed, offset = ctx.rule
         counter = ctx.saved_tensors[0] if ctx.drawn else None
-        return _DropoutFn.apply(g.contiguous(), p, seed, offset, counter), None, None, None, None
+        g = g.contiguous()
+        if torch.is_grad_enabled():  # create_graph
+            return _DropoutFn.apply(g, p, seed, offset, counter), None, None, None, None
+        return _apply_mask(g, p, seed, offset, counter), None, None, None, None
 
 
 def dropout(x: torch.Tensor, p: float = DEFAULT_DROPOUT_P, seed: int = 0, offset: int = 0,

@@ -546,19 +546,22 @@ int dl_counter_draw(int64_t* counter, int64_t* drawn, dl_stream_t stream);
  * No counterpart in the reference (its encoders take real features).
  * ids (tokens) int32 or int64 (id_bits 32 or 64), weight (V, D), out / g (tokens, D), gw (V, D), all of
  * one element type; products and sums in fp32, rounded once.
- *   dl_embedding       out[t] = scale * weight[ids[t]]; an id outside [0, V) gives a NaN row.
+ *   dl_embedding       out[t] = scale * weight[ids[t]]; an id outside [0, V) gives a NaN row.  With `order`
+ *                      (dl_embedding_order_bytes bytes, 256-byte aligned; null: lookup only) the same launch
+ *                      also sorts the tokens for the backward pass; padding_idx (-1: none) and ids outside
+ *                      [0, V) are sorted behind the others and take no gradient.
  *   dl_embedding_bwd   gw[v] = scale * sum of g[t] over ids[t] == v in ascending t; every row of gw is
- *                      written, 0 where no token has that id; ids outside [0, V) and `padding_idx`
- *                      (-1: none) take no gradient.  The order of the additions is a function of the
- *                      sizes and ids alone: run-to-run the same bits.  scratch:
- *                      dl_embedding_bwd_scratch_bytes bytes (0 = sizes not supported), 256-byte aligned;
- *                      tokens, V and D below 2^31.                                              */
+ *                      written, 0 where no token has that id.  `order` as dl_embedding left it for the same
+ *                      tokens, V (it is only read).  The order of the additions is a function of the sizes
+ *                      and ids alone: run-to-run the same bits.  scratch: dl_embedding_bwd_scratch_bytes
+ *                      bytes, 256-byte aligned.
+ * With `order`, tokens, V and D are below 2^31; the size functions return 0 for sizes not supported. */
+int64_t dl_embedding_order_bytes(int64_t tokens, int64_t V, int64_t D, int64_t dtype);
 int dl_embedding(const void* ids, int64_t id_bits, const void* weight, void* out, int64_t tokens, int64_t V,
-                 int64_t D, int64_t dtype, float scale, dl_stream_t stream);
+                 int64_t D, int64_t dtype, float scale, int64_t padding_idx, void* order, dl_stream_t stream);
 int64_t dl_embedding_bwd_scratch_bytes(int64_t tokens, int64_t V, int64_t D, int64_t dtype);
-int dl_embedding_bwd(const void* ids, int64_t id_bits, const void* g, void* gw, int64_t tokens, int64_t V,
-                     int64_t D, int64_t dtype, float scale, int64_t padding_idx, void* scratch,
-                     dl_stream_t stream);
+int dl_embedding_bwd(const void* order, const void* g, void* gw, int64_t tokens, int64_t V, int64_t D,
+                     int64_t dtype, float scale, void* scratch, dl_stream_t stream);
 
 #ifdef __cplusplus
 }

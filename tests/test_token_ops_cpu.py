@@ -64,16 +64,20 @@ def test_embedding_lookup_refuses():
 
 def test_embedding_entry_points_refuse_bad_sizes():
     lib = _native.lib()
-    assert lib.dl_embedding_bwd_scratch_bytes(100, 10, 8, 0) > 0
-    for bad in ((-1, 10, 8, 0), (100, 0, 8, 0), (100, 10, 0, 0), (100, 10, 8, 3), (1 << 31, 10, 8, 0),
-                (100, 1 << 31, 8, 0)):
-        assert lib.dl_embedding_bwd_scratch_bytes(*bad) == 0
-    assert lib.dl_embedding(None, 64, None, None, 3, 4, 2, 0, 1.0, None) == -1
-    assert lib.dl_embedding(None, 64, None, None, 0, 4, 2, 0, 1.0, None) == 0
-    assert lib.dl_embedding(None, 16, None, None, 0, 4, 2, 0, 1.0, None) == -1
-    assert lib.dl_embedding(8, 64, 18, 16, 3, 4, 2, 0, 1.0, None) == -4  # fp32 table at an odd half word
-    assert lib.dl_embedding_bwd(8, 64, 16, 16, 3, 4, 2, 0, 1.0, -1, 64, None) == -4  # scratch not 256-byte aligned
-    assert lib.dl_embedding_bwd(8, 64, 16, 16, 1 << 31, 4, 2, 0, 1.0, -1, 256, None) == -5
+    for size in (lib.dl_embedding_bwd_scratch_bytes, lib.dl_embedding_order_bytes):
+        assert size(100, 10, 8, 0) > 0 and size(0, 10, 8, 0) > 0
+        for bad in ((-1, 10, 8, 0), (100, 0, 8, 0), (100, 10, 0, 0), (100, 10, 8, 3), (1 << 31, 10, 8, 0),
+                    (100, 1 << 31, 8, 0)):
+            assert size(*bad) == 0
+    assert lib.dl_embedding(None, 64, None, None, 3, 4, 2, 0, 1.0, -1, None, None) == -1
+    assert lib.dl_embedding(None, 64, None, None, 0, 4, 2, 0, 1.0, -1, None, None) == 0
+    assert lib.dl_embedding(None, 16, None, None, 0, 4, 2, 0, 1.0, -1, None, None) == -1
+    assert lib.dl_embedding(8, 64, 18, 16, 3, 4, 2, 0, 1.0, -1, None, None) == -4  # fp32 table at an odd half word
+    assert lib.dl_embedding(8, 64, 16, 16, 3, 4, 2, 0, 1.0, -1, 64, None) == -4  # workspace not 256-byte aligned
+    assert lib.dl_embedding(8, 64, 16, 16, 1 << 31, 4, 2, 0, 1.0, -1, 256, None) == -5
+    assert lib.dl_embedding_bwd(256, 16, 16, 3, 4, 2, 0, 1.0, 64, None) == -4
+    assert lib.dl_embedding_bwd(None, 16, 16, 3, 4, 2, 0, 1.0, 256, None) == -1
+    assert lib.dl_embedding_bwd(256, 16, 16, 1 << 31, 4, 2, 0, 1.0, 256, None) == -5
 
 
 # ---------------------------------------------------------------------------------------------- dropout
