@@ -93,6 +93,9 @@ SIGNATURES = {
     "dl_embedding": "plppllllflp s",
     "dl_embedding_bwd_scratch_bytes": "llll",
     "dl_embedding_bwd": "pppllllfp s",
+    "dl_group_norm": "pppppplllllllf s",
+    "dl_group_norm_bwd_scratch_bytes": "lllll",
+    "dl_group_norm_bwd": "pppppppppplllllll s",
 }
 
 _CT = {"p": ctypes.c_void_p, "l": ctypes.c_int64, "i": ctypes.c_int, "f": ctypes.c_float, "d": ctypes.c_double}
@@ -119,6 +122,7 @@ def lib():
             args.append(ctypes.c_void_p)
         fn.argtypes = args
         fn.restype = ctypes.c_int
+    handle.dl_group_norm_bwd_scratch_bytes.restype = ctypes.c_int64
     handle.dl_embedding_order_bytes.restype = ctypes.c_int64
     handle.dl_embedding_bwd_scratch_bytes.restype = ctypes.c_int64
     handle.dl_version.restype = ctypes.c_int

@@ -1,7 +1,8 @@
-"""Utility modules (GroupSum, Dropout) and warning helpers."""
+"""Utility modules (GroupSum, GroupNorm, Dropout) and warning helpers."""
 
 from .dropout import Dropout, dropout
 from .modules import GroupSum
+from .normalization import GroupNorm, group_norm
 from .warnings import (
     ConfigurationWarning,
     CUDAWarning,

@@ -1,0 +1,143 @@
+"""Group norm with an activation over channels-last data.
+
+LUT nodes read their inputs as bits (`value >= 0.5`) or as probabilities; a norm followed by a sigmoid puts any layer's
+values there, half of them on either side of 0.5.  Channels last is how the package's own layers write: rows (B, F), and
+the memory behind ConvolutionalLayer's (B, C, H, W) output (difflut/layers/convolutional.py:199-240).
+"""
+
+from typing import Optional
+
+import torch
+import torch.nn as nn
+from torch.autograd.function import once_differentiable
+
+from .. import _native
+
+DEFAULT_GROUPNORM_EPS: float = 1e-5
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "sigmoid": 3}
+
+
+def _check_activation(activation) -> int:
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"activation must be one of {list(ACTIVATIONS)}, got {activation!r}")
+    return ACTIVATIONS[activation]
+
+
+def _forward(x, weight, bias, dims, eps, act, keep):
+    N, S, C, G, param_code = dims
+    y = torch.empty_like(x)
+    stats = torch.empty(2, N, G, device=x.device, dtype=torch.float32) if keep else None
+    with _native.device_of(x):
+        _native.call("dl_group_norm", x, weight, bias, y, stats, stats.data_ptr() + 4 * N * G if keep else None, N, S, C, G,
+                     _native.DTYPE_CODES[x.dtype], param_code, act, eps)
+    return y, stats
+
+
+class _GroupNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, dims, eps, act):
+        y, stats = _forward(x, weight, bias, dims, eps, act, True)
+        ctx.save_for_backward(x, weight, bias, stats)
+        ctx.dims, ctx.act = dims, act
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        x, weight, bias, stats = ctx.saved_tensors
+        N, S, C, G, param_code = ctx.dims
+        code = _native.DTYPE_CODES[x.dtype]
+        gx = torch.empty_like(x)
+        gw = torch.empty_like(weight) if weight is not None and ctx.needs_input_grad[1] else None
+        gb = torch.empty_like(bias) if bias is not None and ctx.needs_input_grad[2] else None
+        scratch = None
+        if gw is not None or gb is not None:
+            size = int(_native.lib().dl_group_norm_bwd_scratch_bytes(N, S, C, G, code))
+            scratch = torch.empty(size, device=x.device, dtype=torch.uint8)
+        with _native.device_of(x):
+            _native.call("dl_group_norm_bwd", x, g.contiguous(), weight, bias, stats, stats.data_ptr() + 4 * N * G, gx, gw,
+                         gb, scratch, N, S, C, G, code, param_code, ctx.act)
+        return gx, gw, gb, None, None, None
+
+
+def group_norm(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor] = None,
+               bias: Optional[torch.Tensor] = None, eps: float = DEFAULT_GROUPNORM_EPS,
+               activation: str = "none") -> torch.Tensor:
+    """`act(norm(x) * weight + bias)` for x (N, ..., C): every sample's group of C / num_groups channels is normalised
+    over all positions in between, by its mean and biased variance.
+
+    x is float32, bfloat16 or float16; weight and bias (C) are float32 or of x's type.  Statistics and sums are fp32, the
+    result is rounded once.  activation: "none", "relu", "silu" or "sigmoid"."""
+    act = _check_activation(activation)
+    _native.dtype_code(x, "group_norm input")
+    if x.dim() < 2:
+        raise ValueError(f"group_norm expects (N, ..., C) input, got shape {tuple(x.shape)}")
+    N, C = x.shape[0], x.shape[-1]
+    S = 1
+    for size in x.shape[1:-1]:
+        S *= size
+    if isinstance(num_groups, bool) or not isinstance(num_groups, int) or num_groups <= 0:
+        raise ValueError(f"num_groups must be a positive integer, got {num_groups}")
+    if C == 0 or C % num_groups != 0:
+        raise ValueError(f"{C} channels do not form {num_groups} groups of equal size")
+    if not eps >= 0.0:
+        raise ValueError(f"eps must not be negative, got {eps}")
+    param_dtype = None
+    for name, p in (("weight", weight), ("bias", bias)):
+        if p is None:
+            continue
+        if p.shape != (C,):
+            raise ValueError(f"{name} must have shape ({C},), got {tuple(p.shape)}")
+        if p.dtype not in (torch.float32, x.dtype):
+            raise TypeError(f"{name} must be float32 or of the input's type {x.dtype}, got {p.dtype}")
+        if param_dtype not in (None, p.dtype):
+            raise TypeError(f"weight and bias must be of one type, got {param_dtype} and {p.dtype}")
+        param_dtype = p.dtype
+    _native.require_cuda("group_norm", x, weight, bias)
+    if S == 0:
+        raise ValueError(f"group_norm needs at least one position per sample, got shape {tuple(x.shape)}")
+    x = x.contiguous()
+    weight = None if weight is None else weight.contiguous()
+    bias = None if bias is None else bias.contiguous()
+    dims = (N, S, C, num_groups, 0 if param_dtype is None else _native.DTYPE_CODES[param_dtype])
+    if _native.lib().dl_group_norm_bwd_scratch_bytes(N, S, C, num_groups, _native.DTYPE_CODES[x.dtype]) == 0:
+        raise ValueError(f"groups of {C // num_groups} channels are wider than group_norm supports")
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
+                                    or (bias is not None and bias.requires_grad)):
+        return _GroupNormFn.apply(x, weight, bias, dims, float(eps), act)
+    return _forward(x, weight, bias, dims, float(eps), act, False)[0]
+
+
+class GroupNorm(nn.Module):
+    """Group norm with an activation as a module: (N, ..., C), or with `channel_dim=1` (N, C, ...).
+
+    With `channel_dim=1` the memory still is channels last: the output of a ConvolutionalLayer and tensors in torch's
+    channels_last format are taken as they are, any other layout is copied first."""
+
+    def __init__(self, num_groups: int, num_channels: int, eps: float = DEFAULT_GROUPNORM_EPS, affine: bool = True,
+                 activation: str = "none", channel_dim: int = -1) -> None:
+        super().__init__()
+        if num_groups <= 0 or num_channels <= 0 or num_channels % num_groups != 0:
+            raise ValueError(f"{num_channels} channels do not form {num_groups} groups of equal size")
+        if not eps >= 0.0:
+            raise ValueError(f"eps must not be negative, got {eps}")
+        _check_activation(activation)
+        if channel_dim not in (-1, 1):
+            raise ValueError(f"channel_dim must be -1 or 1, got {channel_dim}")
+        self.num_groups, self.num_channels, self.eps = num_groups, num_channels, float(eps)
+        self.activation, self.channel_dim = activation, channel_dim
+        self.weight = nn.Parameter(torch.ones(num_channels)) if affine else None
+        self.bias = nn.Parameter(torch.zeros(num_channels)) if affine else None
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if x.dim() < 2 or x.shape[self.channel_dim] != self.num_channels:
+            raise ValueError(f"GroupNorm expects {self.num_channels} channels in dimension {self.channel_dim}, got shape "
+                             f"{tuple(x.shape)}")
+        if self.channel_dim == 1:
+            x = x.movedim(1, -1)
+        y = group_norm(x, self.num_groups, self.weight, self.bias, self.eps, self.activation)
+        return y.movedim(-1, 1) if self.channel_dim == 1 else y
+
+    def extra_repr(self) -> str:
+        return (f"{self.num_groups}, {self.num_channels}, eps={self.eps}, affine={self.weight is not None}, "
+                f"activation={self.activation!r}, channel_dim={self.channel_dim}")

@@ -563,6 +563,27 @@ int64_t dl_embedding_bwd_scratch_bytes(int64_t tokens, int64_t V, int64_t D, int
 int dl_embedding_bwd(const void* order, const void* g, void* gw, int64_t tokens, int64_t V, int64_t D,
                      int64_t dtype, float scale, void* scratch, dl_stream_t stream);
 
+/* ------------------------------------------------------------------ group norm with an activation
+ * No counterpart in the reference.  x, y, g, gx (N, S, C) channels last (S positions, 1 for plain rows),
+ * C = G groups of equal size, of one element type; weight, bias (C) or null, their gradients likewise,
+ * of type param_dtype; mean, rstd (N, G) fp32.  Statistics, sums and products in fp32, rounded once.
+ *   y = act((x - mean) * rstd * weight + bias), rstd = 1 / sqrt(var + eps), var the biased variance of
+ *   the S * C/G values of a sample's group; activation 0 none, 1 relu, 2 silu, 3 sigmoid.
+ *   dl_group_norm       mean / rstd may be null (both).
+ *   dl_group_norm_bwd   gx, and gweight / gbias where not null, from the mean / rstd of the forward call.
+ *                       scratch: dl_group_norm_bwd_scratch_bytes bytes, 16-byte aligned (not needed when
+ *                       both are null).  Fixed order of additions: run-to-run the same bits.
+ * A group may be up to 4096 vectors wide (the widest power-of-two vector up to 16 bytes that C/G and the
+ * addresses allow); wider ones return DL_ERR_TOO_LARGE (scratch size 0).                    */
+int dl_group_norm(const void* x, const void* weight, const void* bias, void* y, float* mean, float* rstd, int64_t N,
+                  int64_t S, int64_t C, int64_t G, int64_t dtype, int64_t param_dtype, int64_t activation, float eps,
+                  dl_stream_t stream);
+int64_t dl_group_norm_bwd_scratch_bytes(int64_t N, int64_t S, int64_t C, int64_t G, int64_t dtype);
+int dl_group_norm_bwd(const void* x, const void* g, const void* weight, const void* bias, const float* mean,
+                      const float* rstd, void* gx, void* gweight, void* gbias, void* scratch, int64_t N, int64_t S,
+                      int64_t C, int64_t G, int64_t dtype, int64_t param_dtype, int64_t activation,
+                      dl_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -10,8 +10,10 @@ import pytest
 import torch
 
 from difflut_b200.encoder import EmbeddingEncoder, embedding_lookup
-from difflut_b200.utils import Dropout, dropout
-from token_util import TYPES, check, dropped, embedding_grad, half_step, smallest
+from difflut_b200.layers import ConvolutionalLayer, ConvolutionConfig, RandomLayer
+from difflut_b200.nodes import NodeConfig, ProbabilisticNode
+from difflut_b200.utils import Dropout, GroupNorm, dropout, group_norm
+from token_util import TYPES, check, dropped, embedding_grad, half_step, norm_reference, smallest
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -316,3 +318,199 @@ def test_embedding_encoder_trains():
     assert enc(ids[0]).shape == (42,)
     x.sum().backward()
     assert float(enc.weight.grad[0].abs().max()) == 0.0 and float(enc.weight.grad[1:].abs().max()) > 0.0
+
+
+# ---------------------------------------------------------------------------------------------- group norm
+def _rounded(pair, dtype):
+    ref, bound = pair
+    return bound + ref.abs() * half_step(dtype) * 1.01 + smallest(dtype)
+
+
+def _check_norm(N, S, C, G, dtype, act="silu", affine=True, param_dtype=torch.float32, eps=1e-5, shift=0.0, x=None, seed=0):
+    if x is None:
+        x = _normal(N, S, C, seed=seed) * 1.5 + _normal(C, seed=seed + 1) + shift
+    x = x.to(dtype).requires_grad_(True)
+    w = (1 + 0.3 * _normal(C, seed=seed + 2)).to(param_dtype).requires_grad_(True) if affine else None
+    b = (0.2 * _normal(C, seed=seed + 3)).to(param_dtype).requires_grad_(True) if affine else None
+    g = _normal(N, S, C, seed=seed + 4)
+    z = norm_reference(x, G, w, b, eps, act)["z"].to(DEV)
+    g = torch.where(z.abs() < 1e-3, 0.0, g).to(dtype) if act == "relu" else g.to(dtype)  # away from relu's corner
+    ref = norm_reference(x, G, w, b, eps, act, g)
+    y = group_norm(x, G, w, b, eps=eps, activation=act)
+    check(y, ref["y"][0], _rounded(ref["y"], dtype), "y")
+    with torch.no_grad():
+        assert torch.equal(group_norm(x, G, w, b, eps=eps, activation=act), y)
+    wanted = [t for t in (x, w, b) if t is not None]
+    grads = torch.autograd.grad(y, wanted, g, retain_graph=True)
+    check(grads[0], ref["gx"][0], _rounded(ref["gx"], dtype), "gx")
+    if affine:
+        check(grads[1], ref["gw"][0], _rounded(ref["gw"], param_dtype), "gweight")
+        check(grads[2], ref["gb"][0], _rounded(ref["gb"], param_dtype), "gbias")
+    for first, again in zip(grads, torch.autograd.grad(y, wanted, g)):
+        assert torch.equal(first, again)
+    return x, w, b, g, y, grads
+
+
+NORM_SIZES = [(1, 1, 16, 1), (3, 1, 30, 3), (300, 1, 96, 12), (5, 1, 1024, 32), (700, 1, 64, 2), (9, 1, 513, 9), (4, 1, 2048, 2),
+              (2, 7, 12, 4), (2, 100, 6, 6), (3, 65, 40, 4), (2, 576, 32, 8), (1, 1517, 120, 12), (2, 333, 8, 8),
+              (1, 4097, 64, 4), (2, 50, 1000, 1), (1, 3, 1, 1), (1, 40, 3, 1), (2, 19, 1030, 2)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N,S,C,G", NORM_SIZES)
+def test_group_norm_sizes(N, S, C, G, dtype):
+    _check_norm(N, S, C, G, dtype, seed=N + S + C)
+
+
+@pytest.mark.parametrize("act", ["none", "relu", "silu", "sigmoid"])
+@pytest.mark.parametrize("N,S,C,G", [(64, 1, 128, 8), (3, 130, 48, 6)])
+def test_group_norm_activations(N, S, C, G, act):
+    for dtype in TYPES:
+        _check_norm(N, S, C, G, dtype, act=act)
+        _check_norm(N, S, C, G, dtype, act=act, affine=False)
+        _check_norm(N, S, C, G, dtype, act=act, param_dtype=dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("N,S,C,G", [
+    (1, 9000, 64, 2),       # a unit over a cluster of blocks
+    (1, 30000, 128, 1),     # larger than the shared memory of a cluster: part of it is read twice
+    (2, 3, 8192, 1),        # a group over several blocks of channels
+    (1, 2, 5000, 1),        # the same with lanes left over
+    (1, 40, 12000, 1),      # and too many positions for the shared memory
+    (600, 3, 64, 4),        # several samples per block in the backward pass
+])
+def test_group_norm_large_units(N, S, C, G, dtype):
+    _check_norm(N, S, C, G, dtype, act="sigmoid")
+
+
+@pytest.mark.parametrize("S", [1, 37, 5000])
+def test_group_norm_far_from_zero(S):
+    """A mean a thousand times the spread: squares are taken around the mean."""
+    _check_norm(3, S, 32, 2, torch.float32, shift=1500.0)
+
+
+def test_group_norm_constant_group():
+    """No spread at all: the output is act(bias), the gradient is finite."""
+    x = torch.full((2, 33, 16), 3.0, device=DEV)
+    _check_norm(2, 33, 16, 4, torch.float32, x=x)
+    _check_norm(2, 1, 16, 4, torch.float32, x=x[:, :1].contiguous())
+
+
+@pytest.mark.parametrize("S", [1, 50])
+def test_group_norm_values_that_are_not_numbers_stay_in_their_group(S):
+    x = _normal(4, S, 32)
+    x[1, 0, 3], x[2, S - 1, 20] = float("nan"), float("inf")
+    want = torch.nn.functional.group_norm(x.transpose(1, 2).double(), 4).transpose(1, 2)
+    y = group_norm(x, 4)
+    assert torch.equal(torch.isnan(y), torch.isnan(want))
+    ok = ~torch.isnan(want)
+    assert float((y[ok] - want[ok]).abs().max()) < 1e-5
+    clean = group_norm(torch.nan_to_num(x, nan=0.0, posinf=0.0), 4)
+    assert torch.equal(y[0], clean[0]) and torch.equal(y[3], clean[3])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_group_norm_alignment_and_strides(dtype):
+    flat = _normal(2 * 50 * 24 + 1, dtype=dtype)
+    shifted, plain = flat[1:].view(2, 50, 24), flat[1:].clone().view(2, 50, 24)
+    a, b = group_norm(shifted, 3, activation="silu"), group_norm(plain, 3, activation="silu")
+    assert float((a.float() - b.float()).abs().max()) <= 4 * half_step(dtype) * float(b.float().abs().max())
+    strided = _normal(2, 24, 50, dtype=dtype).transpose(1, 2)
+    assert torch.equal(group_norm(strided, 3), group_norm(strided.contiguous(), 3))
+    x = plain.float().requires_grad_(True)  # an expanded gradient
+    (gx,) = torch.autograd.grad(group_norm(x, 3).sum(), x)
+    assert float(gx.abs().max()) < 1e-4  # a constant on every element of a group has no effect
+
+
+def test_group_norm_gradient_against_differences():
+    x = _normal(2, 9, 12).requires_grad_(True)
+    w, b = (1 + 0.1 * _normal(12, seed=1)).requires_grad_(True), _normal(12, seed=2).requires_grad_(True)
+    g = _normal(2, 9, 12, seed=3)
+    grads = torch.autograd.grad(group_norm(x, 3, w, b, activation="sigmoid"), (x, w, b), g)
+    for t, grad in zip((x, w, b), grads):
+        d = _normal(*t.shape, seed=7)
+        h = 1e-2
+        with torch.no_grad():
+            def loss(step):
+                args = [v + step * d if v is t else v for v in (x, w, b)]
+                return (group_norm(args[0], 3, args[1], args[2], activation="sigmoid").double() * g).sum()
+            # fourth-order differences: error h^4 times the fifth derivative (below 10) plus rounding / h
+            slope = (8 * (loss(h) - loss(-h)) - (loss(2 * h) - loss(-2 * h))) / (12 * h)
+        want = float((grad.double() * d).sum())
+        assert abs(float(slope) - want) <= 2e-3 * max(1.0, abs(want))
+
+
+def test_group_norm_empty_batch():
+    x = torch.empty(0, 5, 8, device=DEV, requires_grad=True)
+    w = torch.ones(8, device=DEV, requires_grad=True)
+    gx, gw = torch.autograd.grad(group_norm(x, 2, w), (x, w), torch.empty(0, 5, 8, device=DEV))
+    assert gx.shape == (0, 5, 8) and torch.equal(gw, torch.zeros_like(w))
+    with pytest.raises(ValueError, match="position"):
+        group_norm(torch.empty(2, 0, 8, device=DEV), 2)
+    with pytest.raises(ValueError, match="wider"):
+        group_norm(torch.empty(2, 4097, device=DEV, dtype=torch.bfloat16), 1)
+
+
+def test_group_norm_partial_gradients():
+    x, w, b = _normal(3, 20, 16), torch.ones(16, device=DEV, requires_grad=True), torch.zeros(16, device=DEV)
+    (gw,) = torch.autograd.grad(group_norm(x, 4, w, b, activation="silu").sum(), w)
+    xg, bg = x.clone().requires_grad_(True), b.clone().requires_grad_(True)
+    both = torch.autograd.grad(group_norm(xg, 4, w, bg, activation="silu").sum(), (xg, w, bg))
+    assert torch.equal(gw, both[1])
+    (gx,) = torch.autograd.grad(group_norm(xg, 4, w.detach(), b, activation="silu").sum(), xg)
+    assert torch.equal(gx, both[0])
+
+
+def test_group_norm_captured_and_replayed():
+    x, w, b = (t.requires_grad_(True) for t in (_normal(4, 700, 64), _normal(64, seed=1), _normal(64, seed=2)))
+    g = _normal(4, 700, 64, seed=3)
+
+    def step():
+        y = group_norm(x, 8, w, b, activation="silu")
+        return (y.detach(),) + torch.autograd.grad(y, (x, w, b), g)
+
+    want = step()
+    torch.cuda.synchronize()
+    graphs, results = [], []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            results.append(step())
+        graphs.append(graph)
+    for graph in graphs + graphs:
+        graph.replay()
+    torch.cuda.synchronize()
+    for got in results:
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+def test_group_norm_streams_at_once():
+    x, g = _normal(8, 2000, 64).requires_grad_(True), _normal(8, 2000, 64, seed=1)
+    want = torch.autograd.grad(group_norm(x, 4), x, g)[0]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(3):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got.append(torch.autograd.grad(group_norm(x, 4), x, g)[0])
+    torch.cuda.synchronize()
+    assert all(torch.equal(t, want) for t in got)
+
+
+def test_group_norm_module_behind_a_convolutional_layer():
+    """(B, C, H, W) over the layer's channels-last memory: no copy in, the same view out."""
+    torch.manual_seed(0)
+    conv = ConvolutionalLayer(ConvolutionConfig(tree_depth=1, in_channels=2, out_channels=8, receptive_field=3),
+                              ProbabilisticNode, NodeConfig(input_dim=4, output_dim=1), RandomLayer,
+                              n_inputs_per_node=4, flip_probability=0.0).to(DEV)
+    norm = GroupNorm(2, 8, activation="sigmoid", channel_dim=1).to(DEV)
+    h = conv(torch.rand(3, 2, 9, 9, device=DEV))
+    assert h.movedim(1, -1).is_contiguous()
+    y = norm(h)
+    want = torch.sigmoid(torch.nn.functional.group_norm(h.detach().double(), 2))
+    assert y.shape == h.shape and y.movedim(1, -1).is_contiguous()
+    assert float((y - want).abs().max()) < 1e-5
+    y.square().sum().backward()
+    assert float(norm.weight.grad.abs().max()) > 0 and float(conv.first_layer_chunks[0].raw_weights.grad.abs().max()) > 0
+    rows = GroupNorm(2, 8).to(DEV)
+    assert rows(torch.rand(5, 8, device=DEV)).shape == (5, 8)

@@ -7,7 +7,7 @@ import torch
 import difflut_b200 as difflut
 from difflut_b200 import _native
 from difflut_b200.encoder import EmbeddingEncoder, embedding_lookup
-from difflut_b200.utils import Dropout, dropout
+from difflut_b200.utils import Dropout, GroupNorm, dropout, group_norm
 from difflut_b200.utils.warnings import DefaultValueWarning
 from token_util import philox
 
@@ -119,3 +119,60 @@ def test_dropout_entry_points_refuse():
     assert lib.dl_dropout(None, None, 0, 7, 0.5, 1, 0, None, None) == -1
     assert lib.dl_dropout(6, 8, 4, 0, 0.5, 1, 0, None, None) == -4
     assert lib.dl_counter_draw(None, None, None) == -1
+
+
+# ---------------------------------------------------------------------------------------------- group norm
+def test_group_norm_refuses():
+    x, w = torch.zeros(2, 3, 8), torch.ones(8)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        group_norm(x, 2)
+    for groups in (0, 3, -2, 2.0, True):
+        with pytest.raises(ValueError):
+            group_norm(x, groups)
+    with pytest.raises(ValueError, match="activation"):
+        group_norm(x, 2, activation="tanh")
+    with pytest.raises(ValueError, match="eps"):
+        group_norm(x, 2, eps=float("nan"))
+    with pytest.raises(ValueError, match="weight"):
+        group_norm(x, 2, w[:7])
+    with pytest.raises(ValueError, match="bias"):
+        group_norm(x, 2, w, w.view(1, 8))
+    with pytest.raises(TypeError, match="weight"):
+        group_norm(x, 2, w.half())
+    with pytest.raises(TypeError, match="one type"):
+        group_norm(x.half(), 2, w, w.half())
+    with pytest.raises(TypeError, match="float32, bfloat16 or float16"):
+        group_norm(x.double(), 2)
+    with pytest.raises(ValueError, match="shape"):
+        group_norm(x[0, 0], 2)
+
+
+def test_group_norm_module_host_side():
+    for kwargs in ({"num_groups": 3}, {"num_groups": 0}, {"eps": -1.0}, {"activation": "gelu"}, {"channel_dim": 2}):
+        with pytest.raises(ValueError):
+            GroupNorm(**{"num_groups": 2, "num_channels": 8, **kwargs})
+    m = GroupNorm(2, 8, activation="sigmoid", channel_dim=1)
+    assert list(m.state_dict()) == ["weight", "bias"] and GroupNorm(2, 8, affine=False).weight is None
+    with pytest.raises(ValueError, match="8 channels"):
+        m(torch.zeros(2, 3, 8))
+    assert "sigmoid" in repr(m)
+
+
+def test_group_norm_entry_points_refuse():
+    lib = _native.lib()
+    size = lib.dl_group_norm_bwd_scratch_bytes
+    assert size(2, 3, 8, 2, 0) > 0 and size(0, 3, 8, 2, 0) > 0
+    # 4096 vectors of 16 bytes are the widest group, whatever the positions
+    assert size(2, 1, 16384, 1, 0) > 0 and size(2, 5, 32768, 1, 1) > 0
+    for bad in ((-1, 3, 8, 2, 0), (2, 0, 8, 2, 0), (2, 3, 0, 2, 0), (2, 3, 8, 3, 0), (2, 3, 8, 2, 5), (2, 1, 16385, 1, 0),
+                (2, 1, 32768, 1, 0), (2, 1, 4097, 1, 1)):
+        assert size(*bad) == 0
+    zeros = [None] * 6
+    assert lib.dl_group_norm(*zeros, 2, 3, 8, 2, 0, 0, 0, 1e-5, None) == -1
+    assert lib.dl_group_norm(*zeros, 0, 3, 8, 2, 0, 0, 0, 1e-5, None) == 0
+    assert lib.dl_group_norm(*zeros, 0, 3, 8, 2, 0, 0, 4, 1e-5, None) == -1
+    assert lib.dl_group_norm(16, None, None, 18, None, None, 2, 3, 8, 2, 0, 0, 0, 1e-5, None) == -4
+    assert lib.dl_group_norm(16, None, None, 16, 16, None, 2, 3, 8, 2, 0, 0, 0, 1e-5, None) == -1
+    assert lib.dl_group_norm(16, None, None, 16, None, None, 2, 1, 16385, 1, 0, 0, 0, 1e-5, None) == -5
+    assert lib.dl_group_norm_bwd(*([16] * 10), 2, 3, 8, 2, 0, 0, 9, None) == -1
+    assert lib.dl_group_norm_bwd(16, 16, None, None, None, 16, 16, 16, 16, 16, 2, 3, 8, 2, 0, 0, 0, None) == -1

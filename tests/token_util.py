@@ -67,3 +67,52 @@ def embedding_grad(ids, g, V, scale, padding=None):
         size[ids[t]] += g[t].abs()
         count[ids[t]] += 1
     return total * scale, size * abs(scale), count
+
+
+# ---------------------------------------------------------------------------------------------- group norm
+def norm_reference(x, G, weight, bias, eps, act, g=None, depth=400):
+    """Float64 results of x (N, S, C) and the bounds of their errors, as pairs.
+
+    With u = 2^-24 and `depth` the longest chain of additions of a sum: the mean is off by depth * u * mean|x|, the
+    variance by depth * u relative (its squares are centred), hence xh by `e_xh`, z by `e_z` and so on through the
+    formulas; exponential and quotient of the sigmoid are a few u, the slopes change by at most half as much as z."""
+    u = 2.0 ** -24
+    N, S, C = x.shape
+    x = x.detach().double().cpu()
+    w = torch.ones(C, dtype=torch.float64) if weight is None else weight.detach().double().cpu()
+    b = torch.zeros(C, dtype=torch.float64) if bias is None else bias.detach().double().cpu()
+
+    def groups(t):
+        return t.reshape(N, S, G, C // G)
+
+    def mean(t):  # over a sample's group, spread over its elements
+        return groups(t).mean(dim=(1, 3), keepdim=True).expand(N, S, G, C // G).reshape(N, S, C)
+
+    mu = mean(x)
+    rstd = torch.rsqrt(mean((x - mu) ** 2) + eps)
+    xh = (x - mu) * rstd
+    z = xh * w + b
+    e_xh = depth * u * mean(x.abs()) * rstd + 2 * u * mu.abs() * rstd + xh.abs() * (depth / 2 + 4) * u
+    e_z = e_xh * w.abs() + 2 * u * ((xh * w).abs() + b.abs())
+    s = torch.sigmoid(z)
+    y, slope = {"none": (z, torch.ones_like(z)), "relu": (z.clamp_min(0), (z > 0).double()),
+                "silu": (z * s, s * (1 + z * (1 - s))), "sigmoid": (s, s * (1 - s))}[act]
+    e_y = 1.1 * e_z + (10 + z.abs()) * u * (y.abs() + s)
+    out = {"z": z, "y": (y, e_y)}
+    if g is None:
+        return out
+    g = g.detach().double().cpu()
+    dz = g * slope
+    e_dz = g.abs() * ((0 if act in ("none", "relu") else 0.5) * e_z + (10 + z.abs()) * u)
+    wdz = dz * w
+    s1, s2 = mean(wdz), mean(wdz * xh)
+    e_s1 = mean(e_dz * w.abs()) + (depth + 4) * u * mean(wdz.abs())
+    e_s2 = mean(e_dz * (w * xh).abs() + wdz.abs() * e_xh) + (depth + 4) * u * mean((wdz * xh).abs())
+    gx = rstd * (wdz - s1 - xh * s2)
+    size = rstd * (wdz.abs() + s1.abs() + (xh * s2).abs())
+    e_gx = rstd * (w.abs() * e_dz + e_s1 + xh.abs() * e_s2 + e_xh * s2.abs()) + size * (8 + depth / 2) * u
+    gw, gb = (dz * xh).sum(dim=(0, 1)), dz.sum(dim=(0, 1))
+    e_gw = (e_dz * xh.abs() + dz.abs() * e_xh + depth * u * (dz * xh).abs()).sum(dim=(0, 1))
+    e_gb = (e_dz + depth * u * dz.abs()).sum(dim=(0, 1))
+    out.update(gx=(gx, e_gx), gw=(gw, e_gw), gb=(gb, e_gb))
+    return out
