@@ -96,6 +96,7 @@ SIGNATURES = {
     "dl_group_norm": "pppppplllllllf s",
     "dl_group_norm_bwd_scratch_bytes": "lllll",
     "dl_group_norm_bwd": "pppppppppplllllll s",
+    "dl_sample_rows": "plplpdplpdpdplll s",
 }
 
 _CT = {"p": ctypes.c_void_p, "l": ctypes.c_int64, "i": ctypes.c_int, "f": ctypes.c_float, "d": ctypes.c_double}

@@ -29,6 +29,7 @@ from .distributed import allreduce_sum_
 from .encoder.thermometer import ThermometerEncoder
 from .layers.random_layer import RandomLayer
 from .utils.modules import GroupSum
+from .utils.sampling import sample_logits
 
 
 class DWNNetwork:
@@ -531,6 +532,15 @@ class DWNNetwork:
             out = torch.empty(B, self.k, device=self.device, dtype=torch.float32)
             _native.call("dl_f32_t_to_rows", self.logits_t, out, B, self.k, self.Bp)
         return out
+
+    def sample(self, x: torch.Tensor, u: Optional[torch.Tensor] = None, temperature=1.0, top_k=0, top_p=1.0,
+               min_p=0.0) -> torch.Tensor:
+        """A class id per sample (B,) int64, drawn from the training-mode logits by the random numbers u (B,) in [0, 1)
+        (drawn from torch's generator of the device when left out); settings as in `utils.sample_logits`."""
+        logits = self.logits(x)
+        if u is None:
+            u = torch.rand(logits.shape[0], device=self.device)
+        return sample_logits(logits, u, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
 
     @torch.no_grad()
     def hard_counts(self, x: Optional[torch.Tensor] = None, packed_rows: Optional[torch.Tensor] = None,

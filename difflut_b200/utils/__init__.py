@@ -1,8 +1,9 @@
-"""Utility modules (GroupSum, GroupNorm, Dropout) and warning helpers."""
+"""Utility modules (GroupSum, GroupNorm, Dropout), sampling from logits, and warning helpers."""
 
 from .dropout import Dropout, dropout
 from .modules import GroupSum
 from .normalization import GroupNorm, group_norm
+from .sampling import sample_logits
 from .warnings import (
     ConfigurationWarning,
     CUDAWarning,

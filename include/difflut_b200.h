@@ -584,6 +584,25 @@ int dl_group_norm_bwd(const void* x, const void* g, const void* weight, const vo
                       int64_t C, int64_t G, int64_t dtype, int64_t param_dtype, int64_t activation,
                       dl_stream_t stream);
 
+/* ------------------------------------------------------------------ sampling from logits
+ * No counterpart in the reference.  Per row of logits (R rows of V classes, `pitch` elements apart; one of the
+ * DL_DTYPE_* types) one class id into out (int64): temperature, then top-k, top-p, min-p, then the first
+ * class in ascending order whose running sum of kept weights exceeds u * (their total), w_i =
+ * exp((l_i - max) / T).  Equal logits count as lower the higher their index.  Weights are fixed point
+ * (62 - log2 V fractional bits, at most 50) from exp in double: exact sums, the same id on every run.
+ *   u                  (R) random numbers in [0, 1), fp32 or (u_double != 0) fp64
+ *   temperature        > 0; 0 takes the largest logit (lowest index)
+ *   top_k              0 (or >= V): all        top_p   1: all        min_p   0: all; keeps w_i >= min_p
+ * Each setting is an array (R) or null, then its scalar `_all` holds for all rows.  In the arrays a
+ * temperature that is not positive takes the largest logit, a top_k that is not positive and a top_p that
+ * is not below 1 keep all, a top_p that is not positive keeps the first class, min_p is clamped to [0, 1].
+ * NaN and -inf are never taken; a row without any other logit gives -1.  With logits of +inf only those
+ * have weight.  V below 2^30.                                                                */
+int dl_sample_rows(const void* logits, int64_t pitch, const void* u, int64_t u_double, const float* temperature,
+                   double temperature_all, const int32_t* top_k, int64_t top_k_all, const float* top_p,
+                   double top_p_all, const float* min_p, double min_p_all, int64_t* out, int64_t R, int64_t V,
+                   int64_t dtype, dl_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

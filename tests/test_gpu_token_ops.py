@@ -5,15 +5,18 @@ n * 2^-24 of the sum of absolute terms.
 """
 
 import copy
+import math
 
+import numpy as np
 import pytest
 import torch
 
 from difflut_b200.encoder import EmbeddingEncoder, embedding_lookup
 from difflut_b200.layers import ConvolutionalLayer, ConvolutionConfig, RandomLayer
 from difflut_b200.nodes import NodeConfig, ProbabilisticNode
-from difflut_b200.utils import Dropout, GroupNorm, dropout, group_norm
-from token_util import TYPES, check, dropped, embedding_grad, half_step, norm_reference, smallest
+from difflut_b200.utils import Dropout, GroupNorm, dropout, group_norm, sample_logits
+from token_util import (TYPES, check, dropped, embedding_grad, half_step, kept_weights, norm_reference, sample_row,
+                        smallest)
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -514,3 +517,179 @@ def test_group_norm_module_behind_a_convolutional_layer():
     assert float(norm.weight.grad.abs().max()) > 0 and float(conv.first_layer_chunks[0].raw_weights.grad.abs().max()) > 0
     rows = GroupNorm(2, 8).to(DEV)
     assert rows(torch.rand(5, 8, device=DEV)).shape == (5, 8)
+
+
+# ---------------------------------------------------------------------------------------------- sampling
+def _check_samples(x, u, T=1.0, k=0, p=1.0, m=0.0):
+    """Every id equals the plain 64-bit form's, with numbers or per-row tensors as settings."""
+    got = sample_logits(x, u, temperature=T, top_k=k, top_p=p, min_p=m).cpu().tolist()
+    rows, us = x.double().cpu().numpy(), u.double().cpu().numpy()
+    per = [v.cpu().tolist() if isinstance(v, torch.Tensor) else [v] * len(rows) for v in (T, k, p, m)]
+    want = [sample_row(rows[r], us[r], *(v[r] for v in per)) for r in range(len(rows))]
+    assert got == want, [(r, a, b) for r, (a, b) in enumerate(zip(got, want)) if a != b][:5]
+    return got
+
+
+def _logits(R, V, dtype, seed=0, spread=2.5):
+    x = _normal(R, V, seed=seed) * spread
+    g = torch.Generator().manual_seed(seed + 1)
+    return (x + 6.0 * (torch.rand(R, V, generator=g) < min(0.5, 4.0 / V)).to(DEV)).to(dtype)
+
+
+def _u(R, seed=0):
+    return torch.rand(R, generator=torch.Generator().manual_seed(seed + 77)).to(DEV)
+
+
+SETTINGS = [(1.0, 0, 1.0, 0.0), (0.7, 40, 1.0, 0.0), (1.3, 0, 0.9, 0.0), (1.0, 0, 1.0, 0.05), (0.8, 50, 0.95, 0.02),
+            (0.0, 0, 1.0, 0.0), (1.0, 1, 0.5, 0.5), (2.0, 3, 0.3, 0.0), (1.0, 1000, 0.999, 0.0)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [1, 2, 3, 31, 32, 33, 64, 65, 200, 256, 257, 511, 512, 513, 1000, 4097, 8192, 16384, 40003])
+def test_sampling_sizes(V, dtype):
+    R = 24 if V < 5000 else 6
+    for i, (T, k, p, m) in enumerate(SETTINGS):
+        _check_samples(_logits(R, V, dtype, seed=V + i), _u(R, i), T, k, p, m)
+
+
+@pytest.mark.parametrize("R,V", [(1, 131072), (700, 700), (1, 600), (130, 9000)])
+def test_sampling_rows_and_clusters(R, V):
+    """One row over the largest cluster, many rows over one block each."""
+    for i, (T, k, p, m) in enumerate(SETTINGS[:5]):
+        _check_samples(_logits(R, V, torch.float32, seed=i), _u(R, i), T, k, p, m)
+
+
+@pytest.mark.parametrize("V", [5, 300, 513, 3000, 30000])
+@pytest.mark.parametrize("levels", [1, 2, 7])
+def test_sampling_equal_logits(V, levels):
+    """Few distinct values: the cuts fall inside runs of equal logits and go by index."""
+    x = torch.randint(0, levels, (8, V), generator=torch.Generator().manual_seed(V)).float().to(DEV)
+    for i, (T, k, p, m) in enumerate([(1.0, 0, 1.0, 0.0), (1.0, 3, 1.0, 0.0), (1.0, V // 2, 1.0, 0.0), (1.0, 0, 0.31, 0.0),
+                                      (0.5, V // 3, 0.77, 0.0), (1.0, 0, 0.6, 0.5), (0.0, 0, 1.0, 0.0), (1.0, 0, 1.0, 1.0)]):
+        _check_samples(x, _u(8, i), T, k, p, m)
+
+
+@pytest.mark.parametrize("V", [400, 3000, 30000])
+@pytest.mark.parametrize("spread", [1e-3, 1e-6, 1e-30])
+def test_sampling_logits_close_together(V, spread):
+    """All logits within one step of the histogram: their keys are narrowed down bit by bit."""
+    x = _normal(6, V, seed=V) * spread
+    x[3] += 8.0  # here most of them become equal
+    x[4, ::2] *= -1e-8
+    for i, (T, k, p, m) in enumerate([(1.0, V // 3, 1.0, 0.0), (1.0, 0, 0.4, 0.0), (0.9, V // 2, 0.9, 0.0), (1.0, 0, 1.0, 0.0)]):
+        _check_samples(x, _u(6, i), T, k, p, m)
+
+
+@pytest.mark.parametrize("V", [7, 300, 2000, 20000])
+def test_sampling_masked_and_extreme_logits(V):
+    low, big = torch.finfo(torch.float32).min, 3.0e38
+    x = _logits(12, V, torch.float32, seed=V)
+    x[0] = -math.inf                       # nothing left
+    x[1] = math.nan
+    x[2, 1:] = -math.inf                   # one left
+    x[3, : V - 1] = low                    # masked by the type's lowest value
+    x[4] = low                             # every logit is that value
+    x[5, ::2] = math.nan
+    x[6, V // 2] = math.inf
+    x[7, ::3] = math.inf
+    x[8, 0], x[8, V - 1] = big, -big
+    x[9, ::2] = 0.0
+    x[9, 1::2] = -0.0
+    x[10] = -math.inf
+    x[10, V - 1] = -5.0
+    x[11, : V // 2] = -math.inf
+    for i, (T, k, p, m) in enumerate(SETTINGS):
+        got = _check_samples(x, _u(12, i), T, k, p, m)
+        assert got[0] == got[1] == -1 and got[2] == 0 and got[10] == V - 1
+
+
+@pytest.mark.parametrize("V", [200, 3000])
+@pytest.mark.parametrize("T", [1e-30, 1e-3, 50.0, 1e30, math.inf, 5e-324])
+def test_sampling_extreme_temperatures(V, T):
+    x, u = _logits(10, V, torch.float32), _u(10)
+    if T == 5e-324:  # 1 / T is not a number of the type: the largest logit
+        assert sample_logits(x, u, temperature=T).tolist() == x.argmax(1).tolist()
+        return
+    for k, p in ((0, 1.0), (20, 1.0), (0, 0.9), (20, 0.5)):
+        _check_samples(x, u, T, k, p)
+
+
+@pytest.mark.parametrize("V", [300, 3000])
+def test_sampling_ends_of_the_random_numbers(V):
+    """u = 0 takes the first kept class, the largest u below 1 the last; numbers outside [0, 1) and NaN are pulled in."""
+    x = _logits(6, V, torch.float32)
+    u = torch.tensor([0.0, 1.0 - 2.0 ** -24, 1.0, 7.0, -1.0, math.nan], device=DEV)
+    got = sample_logits(x, u, top_p=0.9).tolist()
+    for r, (id, first) in enumerate(zip(got, (True, False, False, False, True, True))):
+        ids, w = kept_weights(x[r].cpu().numpy(), p=0.9)
+        assert id == (ids[0] if first else ids[-1])
+    u64 = torch.tensor([1.0 - 2.0 ** -53, 2.0 ** -60] * 3, device=DEV, dtype=torch.float64)
+    _check_samples(x, u64, 1.0, 0, 0.9)
+
+
+@pytest.mark.parametrize("V", [100, 2000])
+def test_sampling_settings_per_row(V):
+    R = 40
+    x, u = _logits(R, V, torch.bfloat16), _u(R)
+    i = torch.arange(R, device=DEV)
+    T = torch.where(i % 5 == 3, 0.0, 0.5 + 0.1 * (i % 7)).float()
+    k = torch.where(i % 4 == 1, 0, 1 + i * 3).int()
+    p = torch.where(i % 3 == 2, 1.0, 0.3 + 0.015 * i).float()
+    m = torch.where(i % 6 == 0, 0.1, 0.0).float()
+    _check_samples(x, u, T, k, p, m)
+    # what numbers may not be, per row: not positive temperatures and counts, shares outside (0, 1], ratios outside [0, 1]
+    T[0], k[1], p[2], p[3], m[4], m[5] = -1.0, -5, 0.0, 2.0, 3.0, -1.0
+    got = sample_logits(x, u, temperature=T, top_k=k, top_p=p, min_p=m).tolist()
+    rows = x.double().cpu().numpy()
+    for r in range(R):
+        a = [float(v[r]) for v in (T, k, p, m)]
+        a[2] = 1e-12 if a[2] <= 0 else a[2]
+        assert got[r] == sample_row(rows[r], float(u[r]), a[0], max(int(a[1]), 0), a[2], min(max(a[3], 0.0), 1.0))
+    assert sample_logits(x, u, temperature=T.double(), top_k=k.long(), top_p=p, min_p=m).tolist() == got
+
+
+@pytest.mark.parametrize("V", [200, 2000, 20000])
+def test_sampling_frequencies(V):
+    """Random numbers on an even grid: every class comes up as often as its weight says, give or take one at each end."""
+    n = 4096
+    x = (_normal(1, V, seed=V) * 2).expand(n, V)  # rows at distance zero
+    u = ((torch.arange(n, dtype=torch.float64) + 0.5) / n).to(DEV)
+    got = np.bincount(sample_logits(x, u, temperature=0.8, top_p=0.95).cpu().numpy(), minlength=V)
+    ids, w = kept_weights(x[0].cpu().numpy(), 0.8, 0, 0.95)
+    want = np.zeros(V)
+    want[ids] = w / w.sum() * n
+    assert np.abs(got - want).max() <= 1.0 + 1e-6
+
+
+def test_sampling_strided_rows_and_views():
+    big = _logits(10, 900, torch.float32)
+    u = _u(10)
+    view = big[:, 100:801]  # rows 900 apart, odd start
+    assert sample_logits(view, u, top_p=0.9).tolist() == sample_logits(view.contiguous(), u, top_p=0.9).tolist()
+    last = big.view(5, 2, 900)[:, -1]
+    assert sample_logits(last, u[:5]).tolist() == sample_logits(last.contiguous(), u[:5]).tolist()
+    t = big[:, :10].t()
+    assert sample_logits(t, u).tolist() == sample_logits(t.contiguous(), u).tolist()
+    assert sample_logits(big, u.expand(2, 10).t()[:, 0]).tolist() == sample_logits(big, u).tolist()
+    assert sample_logits(big[:0], u[:0]).shape == (0,)
+
+
+def test_sampling_captured_and_on_streams():
+    x, u = _logits(20, 5000, torch.float32), _u(20)
+    want = sample_logits(x, u, temperature=0.9, top_k=100, top_p=0.9)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = sample_logits(x, u, temperature=0.9, top_k=100, top_p=0.9)
+    graph.replay()
+    assert torch.equal(got, want)
+    u.copy_(_u(20, 5))
+    graph.replay()
+    assert torch.equal(got, sample_logits(x, u, temperature=0.9, top_k=100, top_p=0.9))
+    torch.cuda.synchronize()
+    outs = []
+    for _ in range(3):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            outs.append(sample_logits(x, u, temperature=0.9, top_k=100, top_p=0.9))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, got) for o in outs)

@@ -7,9 +7,9 @@ import torch
 import difflut_b200 as difflut
 from difflut_b200 import _native
 from difflut_b200.encoder import EmbeddingEncoder, embedding_lookup
-from difflut_b200.utils import Dropout, GroupNorm, dropout, group_norm
+from difflut_b200.utils import Dropout, GroupNorm, dropout, group_norm, sample_logits
 from difflut_b200.utils.warnings import DefaultValueWarning
-from token_util import philox
+from token_util import philox, sample_row
 
 
 def test_philox_known_answers():
@@ -176,3 +176,53 @@ def test_group_norm_entry_points_refuse():
     assert lib.dl_group_norm(16, None, None, 16, None, None, 2, 1, 16385, 1, 0, 0, 0, 1e-5, None) == -5
     assert lib.dl_group_norm_bwd(*([16] * 10), 2, 3, 8, 2, 0, 0, 9, None) == -1
     assert lib.dl_group_norm_bwd(16, 16, None, None, None, 16, 16, 16, 16, 16, 2, 3, 8, 2, 0, 0, 0, None) == -1
+
+
+# ---------------------------------------------------------------------------------------------- sampling
+def test_sample_logits_refuses():
+    x, u = torch.zeros(3, 5), torch.zeros(3)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        sample_logits(x, u)
+    with pytest.raises(TypeError, match="float32, bfloat16 or float16"):
+        sample_logits(x.double(), u)
+    with pytest.raises(ValueError, match="classes"):
+        sample_logits(x[0], u)
+    with pytest.raises(ValueError, match="classes"):
+        sample_logits(x[:, :0], u)
+    with pytest.raises(TypeError, match="u must"):
+        sample_logits(x, u.half())
+    with pytest.raises(TypeError, match="u must"):
+        sample_logits(x, [0.0] * 3)
+    with pytest.raises(ValueError, match="u must"):
+        sample_logits(x, u[:2])
+    nan = float("nan")
+    for name, values in (("temperature", (-1.0, nan, "1", True, torch.ones(2))), ("top_k", (-1, 1.5, True, torch.ones(3, 1))),
+                         ("top_p", (0.0, 1.1, nan, -0.5)), ("min_p", (-0.1, 1.5, nan))):
+        for value in values:
+            with pytest.raises(ValueError, match=name):
+                sample_logits(x, u, **{name: value})
+
+
+def test_sample_entry_point_refuses():
+    f = _native.lib().dl_sample_rows
+
+    def call(logits=16, u=16, out=16, T=1.0, k=0, p=1.0, m=0.0, R=2, V=4, dtype=0):
+        return f(logits, 4, u, 0, None, T, None, k, None, p, None, m, out, R, V, dtype, None)
+
+    assert call(R=0) == 0 and call(logits=None) == -1 and call(u=None) == -1 and call(out=None) == -1
+    assert call(V=0) == -1 and call(R=-1) == -1 and call(dtype=3) == -1 and call(V=1 << 30) == -5
+    assert call(T=-1.0) == -1 and call(T=float("nan")) == -1 and call(k=-1) == -1
+    assert call(p=0.0) == -1 and call(p=float("nan")) == -1 and call(m=-1.0) == -1 and call(m=1.5) == -1
+    assert call(logits=18) == -4 and call(u=18) == -4
+
+
+def test_plain_sampling_form_on_known_answers():
+    x = np.log(np.array([0.1, 0.4, 0.2, 0.3]))
+    assert [sample_row(x, u) for u in (0.0, 0.0999, 0.1001, 0.4999, 0.5001, 0.6999, 0.7001)] == [0, 0, 1, 1, 2, 2, 3]
+    assert sample_row(x, 0.99, k=1) == 1 and sample_row(x, 0.0, k=2) == 1 and sample_row(x, 0.9, k=2) == 3
+    assert sample_row(x, 0.0, p=0.39) == 1 and sample_row(x, 0.9, p=0.41) == 3 and sample_row(x, 0.99, p=0.69) == 3
+    assert sample_row(x, 0.0, min_p=0.6) == 1 and sample_row(x, 0.99, min_p=0.6) == 3
+    assert sample_row(np.array([1.0, 2.0, 2.0]), 0.7, T=0) == 1
+    assert sample_row(np.array([-np.inf, np.nan]), 0.5) == -1
+    assert sample_row(np.array([0.0, np.inf, 1.0, np.inf]), 0.6) == 3
+    assert sample_row(np.array([5.0, 5.0, 5.0]), 0.99, k=2) == 1 and sample_row(np.array([5.0, 5.0, 5.0]), 0.9, p=0.5) == 1

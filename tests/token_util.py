@@ -116,3 +116,34 @@ def norm_reference(x, G, weight, bias, eps, act, g=None, depth=400):
     e_gb = (e_dz + depth * u * dz.abs()).sum(dim=(0, 1))
     out.update(gx=(gx, e_gx), gw=(gw, e_gw), gb=(gb, e_gb))
     return out
+
+
+# ---------------------------------------------------------------------------------------------- sampling
+def kept_weights(x, T=1.0, k=0, p=1.0, min_p=0.0):
+    """(ids in ascending order, their weights) that survive temperature, top-k, top-p and min-p, in float64."""
+    x = np.asarray(x, dtype=np.float64)
+    ids = np.flatnonzero(x > -np.inf)
+    if len(ids) == 0:
+        return ids, np.zeros(0)
+    ids = ids[np.lexsort((ids, -x[ids]))]
+    if T <= 0:
+        return ids[:1], np.ones(1)
+    if k > 0:
+        ids = ids[:k]
+    top = x[ids[0]]
+    w = (x[ids] == np.inf).astype(np.float64) if top == np.inf else np.exp((x[ids] - top) / T)
+    if p < 1.0:
+        ahead = np.concatenate(([0.0], np.cumsum(w)[:-1]))
+        inside = ahead < max(p * w.sum(), 1e-300)
+        ids, w = ids[inside], w[inside]
+    ids, w = ids[w >= min_p], w[w >= min_p]
+    order = np.argsort(ids)
+    return ids[order], w[order]
+
+
+def sample_row(x, u, T=1.0, k=0, p=1.0, min_p=0.0) -> int:
+    ids, w = kept_weights(x, T, k, p, min_p)
+    if len(ids) == 0:
+        return -1
+    upto = np.cumsum(w)
+    return int(ids[min(int(np.searchsorted(upto, u * upto[-1], side="right")), int(np.flatnonzero(w)[-1]))])
