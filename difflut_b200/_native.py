@@ -182,24 +182,38 @@ def dtype_code(t: torch.Tensor, what: str) -> int:
 
 def require_cuda(what: str, *tensors) -> None:
     """Every given tensor is on one CUDA device (None is skipped); RuntimeError otherwise."""
-    device = None
+    device = -1
     for t in tensors:
         if t is None:
             continue
         if not t.is_cuda:
             raise RuntimeError(f"difflut_b200.{what} runs on CUDA tensors only (no CPU fallback)")
-        if device is None:
-            device = t.device
-        elif t.device != device:
-            raise RuntimeError(f"difflut_b200.{what}: tensors are on {device} and {t.device}")
+        index = t.get_device()
+        if device < 0:
+            device = index
+        elif index != device:
+            raise RuntimeError(f"difflut_b200.{what}: tensors are on devices {device} and {index}")
+
+
+def once_differentiable_backward(backward):
+    """A Function's backward whose result cannot be differentiated again: an error says so if it is.  torch's own wrapper
+    costs several microseconds a call and only matters while a graph of the backward pass is being built."""
+    from torch.autograd.function import once_differentiable
+
+    guarded = once_differentiable(backward)
+
+    def chosen(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return chosen
 
 
 _SAME_DEVICE = contextlib.nullcontext()
 
 
 def device_of(t: torch.Tensor):
-    """Context in which t's device is the current one (free when it already is)."""
-    return _SAME_DEVICE if torch.cuda.current_device() == t.device.index else torch.cuda.device(t.device)
+    """Context in which the device of CUDA tensor t is the current one (free when it already is)."""
+    return _SAME_DEVICE if torch._C._cuda_getDevice() == t.get_device() else torch.cuda.device(t.device)
 
 
 def host_floats(values):
@@ -219,6 +233,26 @@ def _call_plan(name: str):
         plan = (getattr(lib(), name), tuple(c for c in sig if c != "s"), sig.endswith("s"))
         _CALL_PLANS[name] = plan
     return plan
+
+
+_ENTRIES = {}
+
+
+def entry(name: str):
+    """Entry `name` as a function of plain addresses (0 or None: null) and numbers that appends the current stream and
+    raises on an error code: `call` without its conversions (a third of a short call), for callers that have checked
+    device, type and contiguity of their tensors themselves."""
+    found = _ENTRIES.get(name)
+    if found is None:
+        fn = _call_plan(name)[0]
+
+        def found(*args):
+            code = fn(*args, torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()))
+            if code != 0:
+                raise RuntimeError(f"{name} failed: {lib().dl_error_string(code).decode()} (code {code})")
+
+        _ENTRIES[name] = found
+    return found
 
 
 def call(name: str, *args, stream=None):

@@ -570,9 +570,8 @@ int launch_forward(const void* ids, const void* weight, void* out, int64_t token
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     const auto kernel = embedding_sorting_kernel<T, W, I>;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(SortShared)) != cudaSuccess ||
-        cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
-        return DL_ERR_LAUNCH;
+    static DlKernelLimits limits;
+    if (!dl_allow(reinterpret_cast<const void*>(kernel), limits, sizeof(SortShared), true)) return DL_ERR_LAUNCH;
     const cudaError_t e = cudaLaunchKernelEx(
         &cfg, kernel, look, padding, reinterpret_cast<uint2*>(order), reinterpret_cast<uint2*>(order + p.off_b),
         reinterpret_cast<uint8_t*>(order + p.off_present), p.passes, p.digit_bits, per, per_log2);

@@ -13,6 +13,8 @@
 // (count, mean, squares).  No atomics: the same bits on every run.
 #include <cooperative_groups.h>
 
+#include <type_traits>
+
 #include "elements.cuh"
 
 namespace cg = cooperative_groups;
@@ -24,27 +26,36 @@ constexpr int MAX_LANES = 512;  // threads across the channels of one block
 
 enum { ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_SIGMOID = 3 };
 
-// 1 / (1 + e^-z).  16-bit results have no use for the last bits of the exponential.
+// e^-z.  16-bit results have no use for the last bits of the exponential.
 template <typename T>
-__device__ __forceinline__ float sigmoid_of(float z) {
-    const float e = sizeof(T) == 4 ? expf(-z) : __expf(-z);
-    return __fdividef(1.0f, 1.0f + e);
+__device__ __forceinline__ float exp_minus(float z) {
+    return sizeof(T) == 4 ? expf(-z) : __expf(-z);
 }
 
-template <typename T>
-__device__ __forceinline__ float activate(float z, int act) {
-    if (act == ACT_NONE) return z;
-    if (act == ACT_RELU) return z < 0.0f ? 0.0f : z;  // NaN stays
-    const float s = sigmoid_of<T>(z);
-    return act == ACT_SILU ? z * s : s;
+template <typename T, int ACT>
+__device__ __forceinline__ float activate(float z) {
+    if (ACT == ACT_NONE) return z;
+    if (ACT == ACT_RELU) return z < 0.0f ? 0.0f : z;  // NaN stays
+    const float s = __fdividef(1.0f, 1.0f + exp_minus<T>(z));
+    return ACT == ACT_SILU ? z * s : s;
 }
 
-template <typename T>
-__device__ __forceinline__ float slope(float z, int act) {
-    if (act == ACT_NONE) return 1.0f;
-    if (act == ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
-    const float s = sigmoid_of<T>(z);
-    return act == ACT_SILU ? s * (1.0f + z * (1.0f - s)) : s * (1.0f - s);
+template <typename T, int ACT>
+__device__ __forceinline__ float slope(float z) {
+    if (ACT == ACT_NONE) return 1.0f;
+    if (ACT == ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
+    const float s = __fdividef(1.0f, 1.0f + exp_minus<T>(z)), rest = 1.0f - s;
+    return ACT == ACT_SILU ? s * fmaf(z, rest, 1.0f) : s * rest;
+}
+
+// calls f with the activation as a compile-time constant: inside the loops over rows the switch would cost a branch
+// per value
+template <typename F>
+__device__ __forceinline__ void with_activation(int act, F f) {
+    if (act == ACT_SILU) f(std::integral_constant<int, ACT_SILU>());
+    else if (act == ACT_SIGMOID) f(std::integral_constant<int, ACT_SIGMOID>());
+    else if (act == ACT_RELU) f(std::integral_constant<int, ACT_RELU>());
+    else f(std::integral_constant<int, ACT_NONE>());
 }
 
 struct Norm {
@@ -58,13 +69,24 @@ struct Norm {
     int act;
 };
 
+// parameters c .. c + W - 1, c a multiple of W; by vectors where their addresses allow
+template <int W>
+__device__ __forceinline__ void load_param(const void* p, int dtype, float missing, int c, float (&f)[W]) {
+    constexpr int BYTES32 = W * 4 < 16 ? W * 4 : 16;
+    if (p == nullptr) {
+#pragma unroll
+        for (int e = 0; e < W; ++e) f[e] = missing;
+    } else if (dtype == DL_DTYPE_F32 && reinterpret_cast<uintptr_t>(p) % BYTES32 == 0) {
+        dl_unpack(*reinterpret_cast<const DlVec<float, W>*>(static_cast<const float*>(p) + c), f);
+    } else {
+#pragma unroll
+        for (int e = 0; e < W; ++e) f[e] = dl_load_as_float(p, dtype, c + e);
+    }
+}
 template <int W>
 __device__ __forceinline__ void load_params(const Norm& p, int c, float (&w)[W], float (&b)[W]) {
-#pragma unroll
-    for (int e = 0; e < W; ++e) {
-        w[e] = p.weight ? dl_load_as_float(p.weight, p.param_dtype, c + e) : 1.0f;
-        b[e] = p.bias ? dl_load_as_float(p.bias, p.param_dtype, c + e) : 0.0f;
-    }
+    load_param<W>(p.weight, p.param_dtype, 1.0f, c, w);
+    load_param<W>(p.bias, p.param_dtype, 0.0f, c, b);
 }
 
 template <typename T, int W>
@@ -239,19 +261,28 @@ norm_unit_kernel(const T* __restrict__ x, T* __restrict__ y, float* __restrict__
         }
         __syncthreads();
         if (at.live) {
+            // z = a * x + c
             const float mean = stats[at.group], rstd = stats[k.groups + at.group];
-            for (int r = at.ty; r < at.rows; r += k.ty) {
-                float f[W];
-                if (r < cached)
-                    dl_unpack(tile[r * k.tx + at.tx], f);
-                else
-                    dl_unpack(*reinterpret_cast<const DlVec<T, W>*>(src + r * pitch), f);
+            float a[W], c[W];
 #pragma unroll
-                for (int e = 0; e < W; ++e) f[e] = activate<T>((f[e] - mean) * rstd * w[e] + b[e], p.act);
-                DlVec<T, W> out;
-                dl_pack(f, out);
-                *reinterpret_cast<DlVec<T, W>*>(dst + r * pitch) = out;
+            for (int e = 0; e < W; ++e) {
+                a[e] = rstd * w[e];
+                c[e] = fmaf(-mean, a[e], b[e]);
             }
+            with_activation(p.act, [&](auto act) {
+                for (int r = at.ty; r < at.rows; r += k.ty) {
+                    float f[W];
+                    if (r < cached)
+                        dl_unpack(tile[r * k.tx + at.tx], f);
+                    else
+                        dl_unpack(*reinterpret_cast<const DlVec<T, W>*>(src + r * pitch), f);
+#pragma unroll
+                    for (int e = 0; e < W; ++e) f[e] = activate<T, act.value>(fmaf(f[e], a[e], c[e]));
+                    DlVec<T, W> out;
+                    dl_pack(f, out);
+                    *reinterpret_cast<DlVec<T, W>*>(dst + r * pitch) = out;
+                }
+            });
         }
     }
     if (k.cluster > 1) cluster.sync();  // nobody leaves while others read its sums
@@ -284,32 +315,42 @@ norm_unit_bwd_kernel(const T* __restrict__ x, const T* __restrict__ gy, const fl
     for (int64_t n = team; n < p.N; n += k.teams, parity ^= 1) {
         const int64_t from = (n * p.S + at.row0) * pitch + at.channel;
         const T *src = x + from, *src_g = gy + from;
-        float part[2] = {0.0f, 0.0f}, mean = 0.0f, rstd = 0.0f;
+        float part[2] = {0.0f, 0.0f}, rstd = 0.0f, off = 0.0f;  // xh = rstd * x + off
         if (at.live) {
             for (int r = at.ty; r < cached; r += k.ty) {
                 copy_async<T, W>(&tile[r * k.tx + at.tx], reinterpret_cast<const DlVec<T, W>*>(src + r * pitch));
                 copy_async<T, W>(&tile_g[r * k.tx + at.tx], reinterpret_cast<const DlVec<T, W>*>(src_g + r * pitch));
             }
-            mean = mean_in[n * p.G + group0 + at.group];
             rstd = rstd_in[n * p.G + group0 + at.group];
-            copy_wait_all();
-            for (int r = at.ty; r < at.rows; r += k.ty) {
-                float f[W], d[W];
-                if (r < cached) {
-                    dl_unpack(tile[r * k.tx + at.tx], f);
-                    dl_unpack(tile_g[r * k.tx + at.tx], d);
-                } else {
-                    dl_unpack(*reinterpret_cast<const DlVec<T, W>*>(src + r * pitch), f);
-                    dl_unpack(*reinterpret_cast<const DlVec<T, W>*>(src_g + r * pitch), d);
-                }
+            off = -mean_in[n * p.G + group0 + at.group] * rstd;
+            float unit_dz[W], unit_dzx[W];
 #pragma unroll
-                for (int e = 0; e < W; ++e) {
-                    const float xh = (f[e] - mean) * rstd, dz = d[e] * slope<T>(xh * w[e] + b[e], p.act);
-                    sum_dz[e] += dz;
-                    sum_dzx[e] += dz * xh;
-                    part[0] += dz * w[e];
-                    part[1] += dz * w[e] * xh;
+            for (int e = 0; e < W; ++e) unit_dz[e] = unit_dzx[e] = 0.0f;
+            copy_wait_all();
+            with_activation(p.act, [&](auto act) {
+                for (int r = at.ty; r < at.rows; r += k.ty) {
+                    float f[W], d[W];
+                    if (r < cached) {
+                        dl_unpack(tile[r * k.tx + at.tx], f);
+                        dl_unpack(tile_g[r * k.tx + at.tx], d);
+                    } else {
+                        dl_unpack(*reinterpret_cast<const DlVec<T, W>*>(src + r * pitch), f);
+                        dl_unpack(*reinterpret_cast<const DlVec<T, W>*>(src_g + r * pitch), d);
+                    }
+#pragma unroll
+                    for (int e = 0; e < W; ++e) {
+                        const float xh = fmaf(f[e], rstd, off), dz = d[e] * slope<T, act.value>(fmaf(xh, w[e], b[e]));
+                        unit_dz[e] += dz;
+                        unit_dzx[e] = fmaf(dz, xh, unit_dzx[e]);
+                    }
                 }
+            });
+#pragma unroll
+            for (int e = 0; e < W; ++e) {
+                part[0] = fmaf(unit_dz[e], w[e], part[0]);
+                part[1] = fmaf(unit_dzx[e], w[e], part[1]);
+                sum_dz[e] += unit_dz[e];
+                sum_dzx[e] += unit_dzx[e];
             }
         }
         float* mine = k.cluster > 1 ? shared_sums + parity * 2 * k.groups : sums;
@@ -327,27 +368,32 @@ norm_unit_bwd_kernel(const T* __restrict__ x, const T* __restrict__ gy, const fl
             s2 = mine[k.groups + at.group];
         }
         if (at.live) {
-            s1 *= over_m;
-            s2 *= over_m;
-            T* dst = gx + from;
-            for (int r = at.ty; r < at.rows; r += k.ty) {
-                float f[W], d[W];
-                if (r < cached) {
-                    dl_unpack(tile[r * k.tx + at.tx], f);
-                    dl_unpack(tile_g[r * k.tx + at.tx], d);
-                } else {
-                    dl_unpack(*reinterpret_cast<const DlVec<T, W>*>(src + r * pitch), f);
-                    dl_unpack(*reinterpret_cast<const DlVec<T, W>*>(src_g + r * pitch), d);
-                }
+            // gx = rstd * w * dz - rstd * (s1 + xh * s2)
+            const float k1 = -rstd * s1 * over_m, k2 = -rstd * s2 * over_m;
+            float rw[W];
 #pragma unroll
-                for (int e = 0; e < W; ++e) {
-                    const float xh = (f[e] - mean) * rstd, dz = d[e] * slope<T>(xh * w[e] + b[e], p.act);
-                    f[e] = rstd * (dz * w[e] - (s1 + xh * s2));
+            for (int e = 0; e < W; ++e) rw[e] = rstd * w[e];
+            T* dst = gx + from;
+            with_activation(p.act, [&](auto act) {
+                for (int r = at.ty; r < at.rows; r += k.ty) {
+                    float f[W], d[W];
+                    if (r < cached) {
+                        dl_unpack(tile[r * k.tx + at.tx], f);
+                        dl_unpack(tile_g[r * k.tx + at.tx], d);
+                    } else {
+                        dl_unpack(*reinterpret_cast<const DlVec<T, W>*>(src + r * pitch), f);
+                        dl_unpack(*reinterpret_cast<const DlVec<T, W>*>(src_g + r * pitch), d);
+                    }
+#pragma unroll
+                    for (int e = 0; e < W; ++e) {
+                        const float xh = fmaf(f[e], rstd, off), dz = d[e] * slope<T, act.value>(fmaf(xh, w[e], b[e]));
+                        f[e] = fmaf(dz, rw[e], fmaf(xh, k2, k1));
+                    }
+                    DlVec<T, W> out;
+                    dl_pack(f, out);
+                    *reinterpret_cast<DlVec<T, W>*>(dst + r * pitch) = out;
                 }
-                DlVec<T, W> out;
-                dl_pack(f, out);
-                *reinterpret_cast<DlVec<T, W>*>(dst + r * pitch) = out;
-            }
+            });
         }
     }
     if (k.cluster > 1) cluster.sync();  // nobody leaves while others read its sums
@@ -399,8 +445,9 @@ norm_rows_kernel(const T* __restrict__ x, T* __restrict__ y, float* __restrict__
     const bool live = group < p.G && j < k.lanes && ty < k.ty;
     const int channel = group * p.per_group + j * W;
     float w[W], b[W];
-    if (live) load_params<W>(p, channel, w, b);
+    bool first = true;
     const float over_m = 1.0f / (float)p.per_group;
+    with_activation(p.act, [&](auto act) {
     for (int64_t n0 = (int64_t)blockIdx.x * k.ty * ITEMS; n0 < p.N; n0 += (int64_t)gridDim.x * k.ty * ITEMS) {
         DlVec<T, W> in[ITEMS];
 #pragma unroll
@@ -408,6 +455,8 @@ norm_rows_kernel(const T* __restrict__ x, T* __restrict__ y, float* __restrict__
             const int64_t n = n0 + i * k.ty + ty;
             if (live && n < p.N) in[i] = *reinterpret_cast<const DlVec<T, W>*>(x + n * p.C + channel);
         }
+        if (first && live) load_params<W>(p, channel, w, b);  // behind the first rows' loads
+        first = false;
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
             const int64_t n = n0 + i * k.ty + ty;
@@ -421,7 +470,10 @@ norm_rows_kernel(const T* __restrict__ x, T* __restrict__ y, float* __restrict__
             const float mean = sum_lanes(sum, k.lanes_log2) * over_m;
             if (here) {
 #pragma unroll
-                for (int e = 0; e < W; ++e) squares += (f[e] - mean) * (f[e] - mean);
+                for (int e = 0; e < W; ++e) {
+                    f[e] -= mean;
+                    squares = fmaf(f[e], f[e], squares);
+                }
             }
             const float rstd = rsqrtf(sum_lanes(squares, k.lanes_log2) * over_m + p.eps);
             if (!here) continue;
@@ -430,12 +482,13 @@ norm_rows_kernel(const T* __restrict__ x, T* __restrict__ y, float* __restrict__
                 rstd_out[n * p.G + group] = rstd;
             }
 #pragma unroll
-            for (int e = 0; e < W; ++e) f[e] = activate<T>((f[e] - mean) * rstd * w[e] + b[e], p.act);
+            for (int e = 0; e < W; ++e) f[e] = activate<T, act.value>(fmaf(f[e] * rstd, w[e], b[e]));
             DlVec<T, W> out;
             dl_pack(f, out);
             *reinterpret_cast<DlVec<T, W>*>(y + n * p.C + channel) = out;
         }
     }
+    });
 }
 
 template <typename T, int W, int ITEMS>
@@ -449,10 +502,11 @@ norm_rows_bwd_kernel(const T* __restrict__ x, const T* __restrict__ gy, const fl
     const bool live = group < p.G && j < k.lanes && ty < k.ty;
     const int channel = group * p.per_group + j * W;
     float w[W], b[W], sum_dz[W], sum_dzx[W];
-    if (live) load_params<W>(p, channel, w, b);
+    bool first = true;
 #pragma unroll
     for (int e = 0; e < W; ++e) sum_dz[e] = sum_dzx[e] = 0.0f;
     const float over_m = 1.0f / (float)p.per_group;
+    with_activation(p.act, [&](auto act) {
     for (int64_t n0 = (int64_t)blockIdx.x * k.ty * ITEMS; n0 < p.N; n0 += (int64_t)gridDim.x * k.ty * ITEMS) {
         DlVec<T, W> in[ITEMS], in_g[ITEMS];
         float mean[ITEMS], rstd[ITEMS];
@@ -466,35 +520,39 @@ norm_rows_bwd_kernel(const T* __restrict__ x, const T* __restrict__ gy, const fl
                 rstd[i] = rstd_in[n * p.G + group];
             }
         }
+        if (first && live) load_params<W>(p, channel, w, b);  // behind the first rows' loads
+        first = false;
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
             const int64_t n = n0 + i * k.ty + ty;
             const bool here = live && n < p.N;
             float xh[W], dzw[W], s1 = 0.0f, s2 = 0.0f;
             if (here) {
+                const float off = -mean[i] * rstd[i];
                 dl_unpack(in[i], xh);
                 dl_unpack(in_g[i], dzw);
 #pragma unroll
                 for (int e = 0; e < W; ++e) {
-                    xh[e] = (xh[e] - mean[i]) * rstd[i];
-                    const float dz = dzw[e] * slope<T>(xh[e] * w[e] + b[e], p.act);
+                    xh[e] = fmaf(xh[e], rstd[i], off);
+                    const float dz = dzw[e] * slope<T, act.value>(fmaf(xh[e], w[e], b[e]));
                     sum_dz[e] += dz;
-                    sum_dzx[e] += dz * xh[e];
+                    sum_dzx[e] = fmaf(dz, xh[e], sum_dzx[e]);
                     dzw[e] = dz * w[e];
                     s1 += dzw[e];
-                    s2 += dzw[e] * xh[e];
+                    s2 = fmaf(dzw[e], xh[e], s2);
                 }
             }
             s1 = sum_lanes(s1, k.lanes_log2) * over_m;
             s2 = sum_lanes(s2, k.lanes_log2) * over_m;
             if (!here) continue;
 #pragma unroll
-            for (int e = 0; e < W; ++e) xh[e] = rstd[i] * (dzw[e] - (s1 + xh[e] * s2));
+            for (int e = 0; e < W; ++e) xh[e] = rstd[i] * (dzw[e] - fmaf(xh[e], s2, s1));
             DlVec<T, W> out;
             dl_pack(xh, out);
             *reinterpret_cast<DlVec<T, W>*>(gx + n * p.C + channel) = out;
         }
     }
+    });
     if (partial == nullptr) return;
 #pragma unroll
     for (int v = 0; v < 2; ++v) {
@@ -540,7 +598,8 @@ norm_params_kernel(const float* __restrict__ partial, int64_t parts, int C, void
 }
 
 // ------------------------------------------------------------------------------------------ host
-constexpr size_t SHARED_LIMIT = 190 * 1024;   // for tiles; a block may have 227 KB in all
+constexpr size_t SHARED_MOST = 227 * 1024;    // of a block
+constexpr size_t SHARED_LIMIT = 190 * 1024;   // of these for tiles
 constexpr size_t SHARED_WANTED = 64 * 1024;   // so that about three blocks share an SM and overlap their phases
 
 // false: the groups are too wide.  `tensors` are held at once (1 forward, 2 backward).
@@ -554,8 +613,14 @@ bool cut_units(const Norm& p, int W, int64_t esize, int tensors, bool accumulate
         k.groups = 1;
         k.tx = (int)dl_ceil_div(k.lanes, k.cluster);
     } else {
-        k.groups = 1;  // the fewest groups that are 128 bytes wide together
-        while (k.groups < p.G && (p.G % k.groups != 0 || (int64_t)k.groups * p.per_group * esize < 128)) ++k.groups;
+        // the fewest groups that are 128 bytes wide together; 64 or 32 when the unit would not fit a cluster at the
+        // wanted size, or when there would be too few units for the SMs
+        for (int64_t width = 128; width >= 32; width /= 2) {
+            k.groups = 1;
+            while (k.groups < p.G && (p.G % k.groups != 0 || (int64_t)k.groups * p.per_group * esize < width)) ++k.groups;
+            const int64_t unit = p.S * k.groups * p.per_group * esize * tensors;
+            if (unit <= (int64_t)SHARED_WANTED * MAX_CLUSTER && p.N * (p.G / k.groups) * MAX_CLUSTER >= DL_NUM_SMS) break;
+        }
         // all groups of a block need a lane each; wide groups of one-element vectors may not fit
         while (k.groups * k.lanes > MAX_LANES) {
             --k.groups;
@@ -611,8 +676,7 @@ bool cut_rows(const Norm& p, int W, int items, int64_t most_blocks, RowCut& k) {
 constexpr int ROW_ITEMS = 4, ROW_ITEMS_BWD = 2;
 constexpr int64_t ROW_BLOCKS = DL_NUM_SMS * 16, ROW_BLOCKS_BWD = DL_NUM_SMS * 4;
 
-template <typename K>
-cudaError_t launch_unit(K kernel, const Cut& k, cudaLaunchConfig_t& cfg, cudaLaunchAttribute* attr, cudaStream_t s) {
+void unit_config(const Cut& k, cudaLaunchConfig_t& cfg, cudaLaunchAttribute* attr, cudaStream_t s) {
     cfg.gridDim = dim3((unsigned)(k.teams * k.blocks_c * k.cluster));
     cfg.blockDim = dim3((unsigned)k.threads);
     cfg.dynamicSmemBytes = k.shared;
@@ -622,7 +686,6 @@ cudaError_t launch_unit(K kernel, const Cut& k, cudaLaunchConfig_t& cfg, cudaLau
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)k.shared);
 }
 
 template <typename T, int W>
@@ -641,7 +704,9 @@ int launch_forward(const void* x, void* y, float* mean, float* rstd, const Norm&
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1];
     const auto kernel = norm_unit_kernel<T, W>;
-    if (launch_unit(kernel, k, cfg, attr, s) != cudaSuccess) return DL_ERR_LAUNCH;
+    static DlKernelLimits limits;
+    if (!dl_allow(reinterpret_cast<const void*>(kernel), limits, SHARED_MOST, false)) return DL_ERR_LAUNCH;
+    unit_config(k, cfg, attr, s);
     return cudaLaunchKernelEx(&cfg, kernel, src, dst, mean, rstd, p, k) == cudaSuccess ? dl_launch_status()
                                                                                       : DL_ERR_LAUNCH;
 }
@@ -674,7 +739,9 @@ int launch_backward(const void* x, const void* g, const float* mean, const float
         cudaLaunchConfig_t cfg = {};
         cudaLaunchAttribute attr[1];
         const auto kernel = norm_unit_bwd_kernel<T, W>;
-        if (launch_unit(kernel, k, cfg, attr, s) != cudaSuccess) return DL_ERR_LAUNCH;
+        static DlKernelLimits limits;
+        if (!dl_allow(reinterpret_cast<const void*>(kernel), limits, SHARED_MOST, false)) return DL_ERR_LAUNCH;
+        unit_config(k, cfg, attr, s);
         if (cudaLaunchKernelEx(&cfg, kernel, src, src_g, mean, rstd, dst, partial, p, k) != cudaSuccess)
             return DL_ERR_LAUNCH;
     }

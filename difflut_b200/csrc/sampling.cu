@@ -662,8 +662,8 @@ int launch_sample(const void* logits, const Job& job, cudaStream_t s) {
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     const auto kernel = sample_kernel<T>;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Shared)) != cudaSuccess)
-        return DL_ERR_LAUNCH;
+    static DlKernelLimits limits;
+    if (!dl_allow(reinterpret_cast<const void*>(kernel), limits, sizeof(Shared), false)) return DL_ERR_LAUNCH;
     return cudaLaunchKernelEx(&cfg, kernel, src, job, ranks) == cudaSuccess ? dl_launch_status() : DL_ERR_LAUNCH;
 }
 

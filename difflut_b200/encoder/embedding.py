@@ -6,11 +6,11 @@ a probability for Probabilistic nodes) and their input gradient trains the table
 (its encoders take real features; the interface is difflut/encoder/base_encoder.py:18-137).
 """
 
+import functools
 from typing import Optional
 
 import torch
 import torch.nn as nn
-from torch.autograd.function import once_differentiable
 
 from .. import _native
 from ..registry import register_encoder
@@ -19,20 +19,26 @@ from .base_encoder import BaseEncoder
 DEFAULT_EMBEDDING_NUM_BITS: int = 8
 
 
+@functools.lru_cache(maxsize=1024)
+def _sizes(tokens, V, D, code):
+    """Bytes of (the sorted tokens, the backward pass's workspace)."""
+    lib = _native.lib()
+    order = int(lib.dl_embedding_order_bytes(tokens, V, D, code))
+    if order == 0:
+        raise RuntimeError(f"the gradient of {tokens} tokens into a {V} x {D} table is not supported")
+    return order, int(lib.dl_embedding_bwd_scratch_bytes(tokens, V, D, code))
+
+
 def _forward(ids, weight, scale, padding, sort):
     """(looked-up rows, the sorted tokens that the backward pass wants or None)."""
     V, D = weight.shape
     code, tokens = _native.DTYPE_CODES[weight.dtype], ids.numel()
-    out = torch.empty(ids.shape + (D,), device=weight.device, dtype=weight.dtype)
-    order = None
-    if sort:
-        size = int(_native.lib().dl_embedding_order_bytes(tokens, V, D, code))
-        if size == 0:
-            raise RuntimeError(f"the gradient of {tokens} tokens into a {V} x {D} table is not supported")
-        order = torch.empty(size, device=weight.device, dtype=torch.uint8)
+    out = weight.new_empty(ids.shape + (D,))
+    order = weight.new_empty(_sizes(tokens, V, D, code)[0], dtype=torch.uint8) if sort else None
     with _native.device_of(weight):
-        _native.call("dl_embedding", ids, 64 if ids.dtype == torch.int64 else 32, weight, out, tokens, V, D, code, scale,
-                     padding, order)
+        _native.entry("dl_embedding")(ids.data_ptr(), 64 if ids.dtype == torch.int64 else 32, weight.data_ptr(),
+                                      out.data_ptr(), tokens, V, D, code, scale, padding,
+                                      order.data_ptr() if sort else None)
     return out, order
 
 
@@ -45,16 +51,17 @@ class _EmbeddingFn(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
+    @_native.once_differentiable_backward
     def backward(ctx, g):
         (order,) = ctx.saved_tensors
         tokens, (V, D), dtype, scale = ctx.spec
         code = _native.DTYPE_CODES[dtype]
-        gw = torch.empty(V, D, device=g.device, dtype=dtype)
-        size = int(_native.lib().dl_embedding_bwd_scratch_bytes(tokens, V, D, code))
-        scratch = torch.empty(size, device=g.device, dtype=torch.uint8)
+        g = g.contiguous()
+        gw = g.new_empty((V, D))
+        scratch = order.new_empty(_sizes(tokens, V, D, code)[1])
         with _native.device_of(g):
-            _native.call("dl_embedding_bwd", order, g.contiguous(), gw, tokens, V, D, code, scale, scratch)
+            _native.entry("dl_embedding_bwd")(order.data_ptr(), g.data_ptr(), gw.data_ptr(), tokens, V, D, code, scale,
+                                              scratch.data_ptr())
         return None, gw, None, None
 
 

@@ -23,9 +23,10 @@ def _check_p(p) -> float:
 
 
 def _apply_mask(x, p, seed, offset, counter):
-    out = torch.empty_like(x, memory_format=torch.contiguous_format)
+    out = torch.empty_like(x)  # x is contiguous
     with _native.device_of(x):
-        _native.call("dl_dropout", x, out, x.numel(), _native.DTYPE_CODES[x.dtype], p, seed, offset, counter)
+        _native.entry("dl_dropout")(x.data_ptr(), out.data_ptr(), x.numel(), _native.DTYPE_CODES[x.dtype], p, seed, offset,
+                                    None if counter is None else counter.data_ptr())
     return out
 
 

@@ -5,11 +5,11 @@ values there, half of them on either side of 0.5.  Channels last is how the pack
 the memory behind ConvolutionalLayer's (B, C, H, W) output (difflut/layers/convolutional.py:199-240).
 """
 
+import functools
 from typing import Optional
 
 import torch
 import torch.nn as nn
-from torch.autograd.function import once_differentiable
 
 from .. import _native
 
@@ -23,13 +23,24 @@ def _check_activation(activation) -> int:
     return ACTIVATIONS[activation]
 
 
+@functools.lru_cache(maxsize=1024)
+def _scratch_bytes(N, S, C, G, code):
+    return int(_native.lib().dl_group_norm_bwd_scratch_bytes(N, S, C, G, code))
+
+
+def _address(t):
+    return None if t is None else t.data_ptr()
+
+
 def _forward(x, weight, bias, dims, eps, act, keep):
     N, S, C, G, param_code = dims
     y = torch.empty_like(x)
-    stats = torch.empty(2, N, G, device=x.device, dtype=torch.float32) if keep else None
+    stats = x.new_empty((2, N, G), dtype=torch.float32) if keep else None
+    mean = _address(stats)
     with _native.device_of(x):
-        _native.call("dl_group_norm", x, weight, bias, y, stats, stats.data_ptr() + 4 * N * G if keep else None, N, S, C, G,
-                     _native.DTYPE_CODES[x.dtype], param_code, act, eps)
+        _native.entry("dl_group_norm")(x.data_ptr(), _address(weight), _address(bias), y.data_ptr(), mean,
+                                       mean + 4 * N * G if keep else None, N, S, C, G, _native.DTYPE_CODES[x.dtype],
+                                       param_code, act, eps)
     return y, stats
 
 
@@ -38,25 +49,27 @@ class _GroupNormFn(torch.autograd.Function):
     def forward(ctx, x, weight, bias, dims, eps, act):
         y, stats = _forward(x, weight, bias, dims, eps, act, True)
         ctx.save_for_backward(x, weight, bias, stats)
-        ctx.dims, ctx.act = dims, act
+        ctx.spec = (dims, act)
         return y
 
     @staticmethod
-    @once_differentiable
+    @_native.once_differentiable_backward
     def backward(ctx, g):
         x, weight, bias, stats = ctx.saved_tensors
-        N, S, C, G, param_code = ctx.dims
+        (N, S, C, G, param_code), act = ctx.spec
         code = _native.DTYPE_CODES[x.dtype]
+        g = g.contiguous()
         gx = torch.empty_like(x)
         gw = torch.empty_like(weight) if weight is not None and ctx.needs_input_grad[1] else None
         gb = torch.empty_like(bias) if bias is not None and ctx.needs_input_grad[2] else None
         scratch = None
         if gw is not None or gb is not None:
-            size = int(_native.lib().dl_group_norm_bwd_scratch_bytes(N, S, C, G, code))
-            scratch = torch.empty(size, device=x.device, dtype=torch.uint8)
+            scratch = x.new_empty(_scratch_bytes(N, S, C, G, code), dtype=torch.uint8)
+        mean = stats.data_ptr()
         with _native.device_of(x):
-            _native.call("dl_group_norm_bwd", x, g.contiguous(), weight, bias, stats, stats.data_ptr() + 4 * N * G, gx, gw,
-                         gb, scratch, N, S, C, G, code, param_code, ctx.act)
+            _native.entry("dl_group_norm_bwd")(x.data_ptr(), g.data_ptr(), _address(weight), _address(bias), mean,
+                                               mean + 4 * N * G, gx.data_ptr(), _address(gw), _address(gb),
+                                               _address(scratch), N, S, C, G, code, param_code, act)
         return gx, gw, gb, None, None, None
 
 
@@ -100,7 +113,7 @@ def group_norm(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor] 
     weight = None if weight is None else weight.contiguous()
     bias = None if bias is None else bias.contiguous()
     dims = (N, S, C, num_groups, 0 if param_dtype is None else _native.DTYPE_CODES[param_dtype])
-    if _native.lib().dl_group_norm_bwd_scratch_bytes(N, S, C, num_groups, _native.DTYPE_CODES[x.dtype]) == 0:
+    if _scratch_bytes(*dims[:4], _native.DTYPE_CODES[x.dtype]) == 0:
         raise ValueError(f"groups of {C // num_groups} channels are wider than group_norm supports")
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
                                     or (bias is not None and bias.requires_grad)):

@@ -51,9 +51,12 @@ def sample_logits(logits: torch.Tensor, u: torch.Tensor, temperature: Union[floa
     if logits.stride(1) != 1 and V > 1:
         logits = logits.contiguous()
     u = u.contiguous()
-    out = torch.empty(R, device=logits.device, dtype=torch.int64)
+    out = logits.new_empty(R, dtype=torch.int64)
     with _native.device_of(logits):
-        _native.call("dl_sample_rows", logits.data_ptr(), logits.stride(0), u, u.dtype == torch.float64, t,
-                     1.0 if t_all is None else t_all, k, 0 if k_all is None else k_all, p, 1.0 if p_all is None else p_all,
-                     m, 0.0 if m_all is None else m_all, out, R, V, code)
+        _native.entry("dl_sample_rows")(
+            logits.data_ptr(), logits.stride(0), u.data_ptr(), u.dtype == torch.float64,
+            None if t is None else t.data_ptr(), 1.0 if t_all is None else t_all,
+            None if k is None else k.data_ptr(), 0 if k_all is None else k_all,
+            None if p is None else p.data_ptr(), 1.0 if p_all is None else p_all,
+            None if m is None else m.data_ptr(), 0.0 if m_all is None else m_all, out.data_ptr(), R, V, code)
     return out
