@@ -93,7 +93,8 @@ SIGNATURES = {
     "dl_embedding": "plppllllflp s",
     "dl_embedding_bwd_scratch_bytes": "llll",
     "dl_embedding_bwd": "pppllllfp s",
-    "dl_group_norm": "pppppplllllllf s",
+    "dl_group_norm_scratch_bytes": "lllll",
+    "dl_group_norm": "ppppppplllllllf s",
     "dl_group_norm_bwd_scratch_bytes": "lllll",
     "dl_group_norm_bwd": "pppppppppplllllll s",
     "dl_sample_rows": "plplpdplpdpdplll s",
@@ -123,6 +124,7 @@ def lib():
             args.append(ctypes.c_void_p)
         fn.argtypes = args
         fn.restype = ctypes.c_int
+    handle.dl_group_norm_scratch_bytes.restype = ctypes.c_int64
     handle.dl_group_norm_bwd_scratch_bytes.restype = ctypes.c_int64
     handle.dl_embedding_order_bytes.restype = ctypes.c_int64
     handle.dl_embedding_bwd_scratch_bytes.restype = ctypes.c_int64

@@ -275,7 +275,10 @@ __device__ __forceinline__ bool reaches_far(const uint2* sorted, int64_t at, int
 template <typename T, int W>
 __device__ __forceinline__ void copy_async(DlVec<T, W>* dst, const DlVec<T, W>* src) {
     constexpr int BYTES = (int)sizeof(T) * W;
-    if constexpr (BYTES >= 4)
+    if constexpr (BYTES == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src)
+                     : "memory");
+    else if constexpr (BYTES >= 4)
         asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)),
                      "l"(src), "n"(BYTES)
                      : "memory");

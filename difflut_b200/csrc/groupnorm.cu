@@ -4,39 +4,44 @@
 //   dz = gy * act'(z);  gbias = sum dz;  gweight = sum dz * xh;
 //   gx = rstd * (weight * dz - (s1 + xh * s2) / m),  s1 = sum weight * dz,  s2 = sum weight * dz * xh,  m = S * C / G
 //
-// Both directions are bound by memory, so every tensor is read once: a unit (one sample, a block of whole groups at
-// least 128 bytes wide) is held in the shared memory of a thread block, or of a cluster when it is larger, while its sums
-// are formed; the blocks of a cluster exchange their sums through distributed shared memory.  What does not fit is read
-// twice.  Every thread keeps to its own channels (a vector of W) and to its own slots of shared memory.  Rows without
-// positions (S = 1) take kernels of their own, in which a group is a few lanes of a warp and stays in registers.
-// Statistics are centred sums in fp32: the mean first, then the squares around it; parts are combined by
-// (count, mean, squares).  No atomics: the same bits on every run.
-#include <cooperative_groups.h>
-
+// Both directions read their tensors twice, first for the sums, then to write the result.  A sample is cut into chunks of
+// rows, one thread block each, such that all blocks are resident at once: one launch leaves every chunk's sums, the next
+// one adds up its sample's (a few hundred numbers) and writes.  Where samples alone fill the GPU a chunk is a sample and
+// one launch does both.  The second reading comes from L2 as far as the tensor fits there.  (Holding a sample in the shared
+// memory of a cluster, so that it is read once, was slower: all blocks load, then all compute, then all store, and each
+// sample costs a cluster barrier; 51 us instead of 38 us for 16 x 4096 x 512 bf16 forward.)
+// A thread keeps to its own channels (a vector of W).  Rows without positions (S = 1) take kernels of their own, in which a
+// group is a few lanes of a warp and stays in registers.
+//
+// A thread sums its values and their squares relative to its first one, which is a value of the group: the squares of these
+// offsets add up to no more than the group's own, so what cancels is at most (values per thread) * 2^-24 of the variance.
+// Threads and chunks are joined by their means and squares around them.  No atomics: the same bits on every run.
 #include <type_traits>
 
 #include "elements.cuh"
 
-namespace cg = cooperative_groups;
-
 namespace {
 
-constexpr int MAX_CLUSTER = 8;
-constexpr int MAX_LANES = 512;  // threads across the channels of one block
+constexpr int MAX_LANES = 256;  // threads across the channels of one block
 
 enum { ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_SIGMOID = 3 };
 
-// e^-z.  16-bit results have no use for the last bits of the exponential.
+// 1 / (1 + e^-z).  The approximate exponential (2^x with x rounded to fp32: its error grows with |z|, where the sigmoid
+// no longer depends on it) is for 16-bit results.  Results below 2^-126 become 0.
 template <typename T>
-__device__ __forceinline__ float exp_minus(float z) {
-    return sizeof(T) == 4 ? expf(-z) : __expf(-z);
+__device__ __forceinline__ float sigmoid_of(float z) {
+    float e, s;
+    if (sizeof(T) == 4) e = expf(-z);
+    else asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z * -1.4426950408889634f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(1.0f + e));
+    return s;
 }
 
 template <typename T, int ACT>
 __device__ __forceinline__ float activate(float z) {
     if (ACT == ACT_NONE) return z;
     if (ACT == ACT_RELU) return z < 0.0f ? 0.0f : z;  // NaN stays
-    const float s = __fdividef(1.0f, 1.0f + exp_minus<T>(z));
+    const float s = sigmoid_of<T>(z);
     return ACT == ACT_SILU ? z * s : s;
 }
 
@@ -44,7 +49,7 @@ template <typename T, int ACT>
 __device__ __forceinline__ float slope(float z) {
     if (ACT == ACT_NONE) return 1.0f;
     if (ACT == ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
-    const float s = __fdividef(1.0f, 1.0f + exp_minus<T>(z)), rest = 1.0f - s;
+    const float s = sigmoid_of<T>(z), rest = 1.0f - s;
     return ACT == ACT_SILU ? s * fmaf(z, rest, 1.0f) : s * rest;
 }
 
@@ -89,335 +94,352 @@ __device__ __forceinline__ void load_params(const Norm& p, int c, float (&w)[W],
     load_param<W>(p.bias, p.param_dtype, 0.0f, c, b);
 }
 
-template <typename T, int W>
-__device__ __forceinline__ void copy_async(DlVec<T, W>* dst, const DlVec<T, W>* src) {
-    constexpr int BYTES = (int)sizeof(T) * W;
-    if constexpr (BYTES >= 4)
-        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)),
-                     "l"(src), "n"(BYTES)
-                     : "memory");
-    else
-        *dst = *src;
-}
-__device__ __forceinline__ void copy_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+// ------------------------------------------------------------------------------------------ chunks of rows
+constexpr int CHUNK_THREADS = 256;
+constexpr int IN_FLIGHT = 4;  // rows a thread loads before it uses the first
 
-// ------------------------------------------------------------------------------------------ units in shared memory
 // How the tensor is cut; a function of sizes, type and alignment.
 struct Cut {
-    int groups;      // per block of channels (one unit)
-    int lanes;       // vectors across one group, all blocks of the cluster together
+    int lanes;       // vectors across one group
+    int groups;      // per block of channels, whole ones; 1 when a group is wider than a block
+    int split;       // blocks of channels per group
     int tx, ty;      // threads across channels and down the rows of one block
-    int threads;
-    int cluster;     // blocks per unit
-    int by_channel;  // the cluster splits the channels of a single group instead of the rows
-    int rows;        // of a unit per block
-    int cached;      // of them in shared memory
     int blocks_c;    // blocks of channels
-    int64_t teams;   // clusters per block of channels; each takes every teams-th sample
-    size_t shared;
+    int chunks;      // of rows per sample
+    int rows;        // per chunk
 };
 
-// What a thread of a unit works on.
+// What a thread works on.  A part is one (chunk, block of channels of the group): the partial sums of a sample's group are
+// chunks * split numbers.
 struct Place {
     int tx, ty;
-    int rank;
-    int group;      // of the block, 0 .. groups - 1
-    int channel;    // first of the thread's W
-    bool live;
-    int group_lanes;  // of a group in this block
+    int64_t n;
+    int chunk, piece;     // which of the group's blocks of channels
+    int group0, groups;   // first group of the block, how many it has
+    int group;            // of the thread, from group0
+    int group_lanes;      // of a group in this block
+    int channel;          // first of the thread's W
     int row0, rows;
+    bool live;
     __device__ __forceinline__ Place(const Norm& p, const Cut& k, int W) {
-        const int lanes_here = k.by_channel ? 0 : k.groups * k.lanes;
         tx = threadIdx.x % k.tx;
         ty = threadIdx.x / k.tx;
-        rank = blockIdx.x % k.cluster;
-        const int block_c = (int)(blockIdx.x / k.cluster % k.blocks_c);
-        const int lane = k.by_channel ? rank * k.tx + tx : tx;
-        live = ty < k.ty && lane < (k.by_channel ? k.lanes : lanes_here);
-        group = k.by_channel ? 0 : tx / k.lanes;
-        channel = (block_c * k.groups * k.lanes + lane) * W;
-        const int left = k.lanes - rank * k.tx;
-        group_lanes = k.by_channel ? (left < k.tx ? (left > 0 ? left : 0) : k.tx) : k.lanes;
-        row0 = k.by_channel ? 0 : rank * k.rows;
-        const int64_t behind = p.S - row0;
-        rows = (int)(behind < k.rows ? (behind > 0 ? behind : 0) : k.rows);
+        const int64_t unit = blockIdx.x / k.chunks;
+        chunk = (int)(blockIdx.x - unit * k.chunks);
+        n = unit / k.blocks_c;
+        const int block_c = (int)(unit - n * k.blocks_c), set = block_c / k.split;
+        piece = block_c - set * k.split;
+        group0 = set * k.groups;
+        groups = p.G - group0 < k.groups ? p.G - group0 : k.groups;
+        group_lanes = lanes_of(k, piece);
+        const int lane = piece * k.tx + tx;  // piece is 0 when the block holds whole groups
+        group = k.split > 1 ? 0 : tx / k.lanes;
+        live = ty < k.ty && (k.split > 1 ? lane < k.lanes : group < groups);
+        channel = (group0 * k.lanes + lane) * W;
+        row0 = chunk * k.rows;
+        rows = rows_of(p, k, chunk);
+    }
+    __device__ __forceinline__ static int lanes_of(const Cut& k, int piece) {
+        if (k.split == 1) return k.lanes;
+        const int left = k.lanes - piece * k.tx;
+        return left < k.tx ? left : k.tx;
+    }
+    __device__ __forceinline__ static int rows_of(const Norm& p, const Cut& k, int chunk) {
+        const int64_t behind = p.S - (int64_t)chunk * k.rows;
+        return (int)(behind < k.rows ? (behind > 0 ? behind : 0) : k.rows);
+    }
+    __device__ __forceinline__ int part(const Cut& k) const { return chunk * k.split + piece; }
+};
+
+// f(row, vectors...) for every row of the thread, IN_FLIGHT loads of every tensor ahead of their use
+template <typename T, int W, typename F, typename... Src>
+__device__ __forceinline__ void each_row(const Place& at, const Cut& k, int64_t pitch, F f, const Src*... src) {
+    int r = at.ty;
+    for (; r + (IN_FLIGHT - 1) * k.ty < at.rows; r += IN_FLIGHT * k.ty) {
+        DlVec<T, W> v[sizeof...(Src)][IN_FLIGHT];
+        const T* const from[] = {src...};
+#pragma unroll
+        for (int u = 0; u < IN_FLIGHT; ++u) {
+#pragma unroll
+            for (int s = 0; s < (int)sizeof...(Src); ++s)
+                v[s][u] = *reinterpret_cast<const DlVec<T, W>*>(from[s] + (r + u * k.ty) * pitch);
+        }
+#pragma unroll
+        for (int u = 0; u < IN_FLIGHT; ++u) {
+            if constexpr (sizeof...(Src) == 1) f(r + u * k.ty, v[0][u]);
+            else f(r + u * k.ty, v[0][u], v[1][u]);
+        }
+    }
+    for (; r < at.rows; r += k.ty) f(r, *reinterpret_cast<const DlVec<T, W>*>(src + r * pitch)...);
+}
+
+// Joins sets of values given by count, mean and squares around their means, one per call and lane, about the mean of one
+// of the sets, `centre`.  That lies within the spread: the sum of count * (mean - centre)^2 is at most (number of sets)
+// times the squares of all, so as many times 2^-24 cancels.
+struct Join {
+    float centre, moved = 0.0f, squares = 0.0f;
+    __device__ __forceinline__ Join(float centre) : centre(centre) {}
+    __device__ __forceinline__ void add(float count, float mean, float around) {
+        const float d = mean - centre;
+        moved = fmaf(count, d, moved);
+        squares += fmaf(count * d, d, around);
+    }
+    __device__ __forceinline__ void across_warp() {
+#pragma unroll
+        for (int s = 16; s > 0; s >>= 1) {
+            moved += __shfl_xor_sync(0xffffffffu, moved, s);
+            squares += __shfl_xor_sync(0xffffffffu, squares, s);
+        }
+    }
+    __device__ __forceinline__ void finish(float count, float& mean, float& around) const {
+        const float off = moved / count;
+        mean = centre + off;
+        around = squares - off * moved;
+        around = around < 0.0f ? 0.0f : around;  // NaN stays
     }
 };
 
-// out[v][g] = sum of value[v] over the threads of group g; all threads call it, `red` holds 2 * threads floats
-template <int NV>
-__device__ __forceinline__ void sum_groups(const float (&value)[NV], const Place& at, const Cut& k, float* red, float* out) {
-    __syncthreads();  // `red` and `out` may still be read from the last time
-#pragma unroll
-    for (int v = 0; v < NV; ++v) red[v * k.threads + threadIdx.x] = at.live ? value[v] : 0.0f;
-    __syncthreads();
-    const int lane = threadIdx.x & 31, warps = k.threads / 32;
-    const int entries = at.group_lanes * k.ty;
-    for (int g = threadIdx.x / 32; g < k.groups; g += warps) {
-        float sum[NV];
-#pragma unroll
-        for (int v = 0; v < NV; ++v) sum[v] = 0.0f;
+// calls f(group, entry) for every thread of every group of the block, a warp per group; then done(group) in every lane
+template <typename F, typename D, typename B>
+__device__ __forceinline__ void warp_per_group(const Place& at, const Cut& k, B begin, F f, D done) {
+    const int lane = threadIdx.x & 31, entries = at.group_lanes * k.ty;
+    for (int g = threadIdx.x / 32; g < at.groups; g += blockDim.x / 32) {
+        begin(g);
         for (int e = lane; e < entries; e += 32) {
-            const int y = e / at.group_lanes, i = y * k.tx + g * at.group_lanes + (e - y * at.group_lanes);
-#pragma unroll
-            for (int v = 0; v < NV; ++v) sum[v] += red[v * k.threads + i];
+            const int y = e / at.group_lanes;
+            f(g, y * k.tx + g * at.group_lanes + (e - y * at.group_lanes));
         }
-#pragma unroll
-        for (int v = 0; v < NV; ++v) {
-#pragma unroll
-            for (int s = 16; s > 0; s >>= 1) sum[v] += __shfl_xor_sync(0xffffffffu, sum[v], s);
-            if (lane == 0) out[v * k.groups + g] = sum[v];
-        }
+        done(g);
     }
-    __syncthreads();
 }
 
-template <typename T, int W>
-__global__ void __launch_bounds__(MAX_LANES)
-norm_unit_kernel(const T* __restrict__ x, T* __restrict__ y, float* __restrict__ mean_out, float* __restrict__ rstd_out,
-                 const __grid_constant__ Norm p, const __grid_constant__ Cut k) {
-    extern __shared__ __align__(16) unsigned char shared_bytes[];
-    DlVec<T, W>* tile = reinterpret_cast<DlVec<T, W>*>(shared_bytes);
-    float* red = reinterpret_cast<float*>(shared_bytes + (size_t)k.cached * k.tx * sizeof(DlVec<T, W>) / 16 * 16 + 16);
-    float* sums = red + 2 * k.threads;       // [2][groups]
-    float* stats = sums + 2 * k.groups;      // [2][groups] mean and rstd of the unit
-    float* shared_parts = stats + 2 * k.groups;  // [2][3][groups] count, mean, squares, read by the other blocks
-    cg::cluster_group cluster = cg::this_cluster();
+enum { SUMS = 1, WRITE = 2 };  // what a launch does; both when a chunk is a sample
+
+// sums (N, G, parts, 2): mean and squares around it of every part
+template <typename T, int W, int DO>
+__global__ void __launch_bounds__(CHUNK_THREADS, 4)
+norm_chunk_kernel(const T* __restrict__ x, T* __restrict__ y, float* __restrict__ mean_out, float* __restrict__ rstd_out,
+                  float* __restrict__ sums, const __grid_constant__ Norm p, const __grid_constant__ Cut k) {
+    __shared__ float red[3][CHUNK_THREADS];
+    __shared__ float stats[2][MAX_LANES];  // mean and rstd of the block's groups
     const Place at(p, k, W);
-    float w[W], b[W];
-    if (at.live) load_params<W>(p, at.channel, w, b);
-    const int cached = at.rows < k.cached ? at.rows : k.cached;
-    const int64_t team = blockIdx.x / k.cluster / k.blocks_c;
-    const int group0 = (int)(blockIdx.x / k.cluster % k.blocks_c) * k.groups;
-    const int64_t pitch = p.C;
-    int parity = 0;
-    for (int64_t n = team; n < p.N; n += k.teams, parity ^= 1) {
-        const T* src = x + (n * p.S + at.row0) * pitch + at.channel;
-        T* dst = y + (n * p.S + at.row0) * pitch + at.channel;
-        float part[2] = {0.0f, 0.0f};
-        if (at.live) {
-            for (int r = at.ty; r < cached; r += k.ty)
-                copy_async<T, W>(&tile[r * k.tx + at.tx], reinterpret_cast<const DlVec<T, W>*>(src + r * pitch));
-            copy_wait_all();
-            for (int r = at.ty; r < cached; r += k.ty) {
+    const int64_t pitch = p.C, first = (at.n * p.S + at.row0) * pitch + at.channel;
+    const int lane = threadIdx.x & 31, parts = k.chunks * k.split;
+    const float values = (float)p.S * (float)p.per_group;
+    if (DO & SUMS) {
+        float count = 0.0f, mean = 0.0f, squares = 0.0f;
+        if (at.live && at.ty < at.rows) {
+            const float zero = dl_to_float(x[first + at.ty * pitch]);
+            float s1 = 0.0f, s2 = 0.0f;
+            int rows = 0;
+            each_row<T, W>(at, k, pitch, [&](int, const DlVec<T, W>& v) {
                 float f[W];
-                dl_unpack(tile[r * k.tx + at.tx], f);
-#pragma unroll
-                for (int e = 0; e < W; ++e) part[0] += f[e];
-            }
-        }
-        {
-            const float one[1] = {part[0]};
-            sum_groups<1>(one, at, k, red, sums);
-        }
-        const float width = (float)(at.group_lanes * W);
-        const float centre = cached > 0 && at.group_lanes > 0 ? sums[at.group] / ((float)cached * width) : 0.0f;
-        part[0] = part[1] = 0.0f;
-        if (at.live) {
-            for (int r = at.ty; r < at.rows; r += k.ty) {
-                float f[W];
-                if (r < cached)
-                    dl_unpack(tile[r * k.tx + at.tx], f);
-                else
-                    dl_unpack(*reinterpret_cast<const DlVec<T, W>*>(src + r * pitch), f);
+                dl_unpack(v, f);
 #pragma unroll
                 for (int e = 0; e < W; ++e) {
-                    const float d = f[e] - centre;
-                    part[0] += d;
-                    part[1] += d * d;
+                    const float d = f[e] - zero;
+                    s1 += d;
+                    s2 = fmaf(d, d, s2);
                 }
-            }
+                ++rows;
+            }, x + first);
+            count = (float)rows * W;
+            const float off = s1 / count;
+            mean = zero + off;
+            squares = s2 - off * s1;
+            squares = squares < 0.0f ? 0.0f : squares;  // NaN stays
         }
-        float* parts = shared_parts + parity * 3 * k.groups;
-        // `centre` of a group is the same in all its threads; thread g of the block still needs that of group g
-        if (threadIdx.x < k.groups) parts[k.groups + threadIdx.x] = cached > 0 && at.group_lanes > 0 ? sums[threadIdx.x] / ((float)cached * width) : 0.0f;
-        sum_groups<2>(part, at, k, red, sums);
-        for (int g = threadIdx.x; g < k.groups; g += k.threads) {
-            const float count = (float)at.rows * width, off = count > 0.0f ? sums[g] / count : 0.0f;
-            parts[g] = count;
-            parts[k.groups + g] += off;
-            parts[2 * k.groups + g] = sums[k.groups + g] - off * sums[g];
-        }
-        if (k.cluster > 1) cluster.sync();
-        else __syncthreads();
-        for (int g = threadIdx.x; g < k.groups; g += k.threads) {
-            float count = 0.0f, mean = 0.0f, squares = 0.0f;
-            for (int r = 0; r < k.cluster; ++r) {
-                const float* other = k.cluster > 1 ? cluster.map_shared_rank(parts, r) : parts;
-                const float c = other[g], m = other[k.groups + g], q = other[2 * k.groups + g];
-                if (c == 0.0f) continue;
-                const float both = count + c, d = m - mean;
-                mean += d * (c / both);
-                squares += q + d * d * (count * (c / both));
-                count = both;
-            }
-            const float rstd = rsqrtf((squares < 0.0f ? 0.0f : squares / count) + p.eps);
-            stats[g] = mean;
-            stats[k.groups + g] = rstd;
-            if (at.rank == 0 && mean_out != nullptr) {
-                mean_out[n * p.G + group0 + g] = mean;
-                rstd_out[n * p.G + group0 + g] = rstd;
-            }
-        }
+        red[0][threadIdx.x] = count;
+        red[1][threadIdx.x] = mean;
+        red[2][threadIdx.x] = squares;
         __syncthreads();
-        if (at.live) {
-            // z = a * x + c
-            const float mean = stats[at.group], rstd = stats[k.groups + at.group];
-            float a[W], c[W];
-#pragma unroll
-            for (int e = 0; e < W; ++e) {
-                a[e] = rstd * w[e];
-                c[e] = fmaf(-mean, a[e], b[e]);
-            }
-            with_activation(p.act, [&](auto act) {
-                for (int r = at.ty; r < at.rows; r += k.ty) {
-                    float f[W];
-                    if (r < cached)
-                        dl_unpack(tile[r * k.tx + at.tx], f);
-                    else
-                        dl_unpack(*reinterpret_cast<const DlVec<T, W>*>(src + r * pitch), f);
-#pragma unroll
-                    for (int e = 0; e < W; ++e) f[e] = activate<T, act.value>(fmaf(f[e], a[e], c[e]));
-                    DlVec<T, W> out;
-                    dl_pack(f, out);
-                    *reinterpret_cast<DlVec<T, W>*>(dst + r * pitch) = out;
+        Join join(0.0f);
+        warp_per_group(at, k,
+            [&](int g) { join = Join(red[1][g * at.group_lanes]); },  // the group's first thread: it has the first row
+            [&](int, int i) { join.add(red[0][i], red[1][i], red[2][i]); },
+            [&](int g) {
+                join.across_warp();
+                if (lane != 0) return;
+                float m, q;
+                join.finish((float)at.rows * (float)(at.group_lanes * W), m, q);
+                if (DO & WRITE) {  // the only part
+                    stats[0][g] = m;
+                    stats[1][g] = q;
+                } else {
+                    float* out = sums + ((at.n * p.G + at.group0 + g) * parts + at.part(k)) * 2;
+                    out[0] = m;
+                    out[1] = q;
                 }
             });
+    }
+    if (!(DO & WRITE)) return;
+    float w[W], b[W];
+    if (at.live) load_params<W>(p, at.channel, w, b);
+    if (!(DO & SUMS)) {
+        for (int g = threadIdx.x / 32; g < at.groups; g += blockDim.x / 32) {
+            const float2* in = reinterpret_cast<const float2*>(sums) + (at.n * p.G + at.group0 + g) * parts;
+            Join join(in[0].x);
+            for (int i = lane; i < parts; i += 32) {
+                const int chunk = i / k.split;
+                join.add((float)Place::rows_of(p, k, chunk) * (float)(Place::lanes_of(k, i - chunk * k.split) * W), in[i].x,
+                         in[i].y);
+            }
+            join.across_warp();
+            if (lane == 0) join.finish(values, stats[0][g], stats[1][g]);
         }
     }
-    if (k.cluster > 1) cluster.sync();  // nobody leaves while others read its sums
+    __syncthreads();
+    if (at.chunk == 0 && at.piece == 0 && mean_out != nullptr) {
+        for (int g = threadIdx.x; g < at.groups; g += blockDim.x) {
+            mean_out[at.n * p.G + at.group0 + g] = stats[0][g];
+            rstd_out[at.n * p.G + at.group0 + g] = rsqrtf(stats[1][g] / values + p.eps);
+        }
+    }
+    if (!at.live) return;
+    // z = a * x + c
+    const float mean = stats[0][at.group], rstd = rsqrtf(stats[1][at.group] / values + p.eps);
+#pragma unroll
+    for (int e = 0; e < W; ++e) {
+        w[e] *= rstd;
+        b[e] = fmaf(-mean, w[e], b[e]);
+    }
+    with_activation(p.act, [&](auto act) {
+        each_row<T, W>(at, k, pitch, [&](int r, const DlVec<T, W>& v) {
+            float f[W];
+            dl_unpack(v, f);
+#pragma unroll
+            for (int e = 0; e < W; ++e) f[e] = activate<T, act.value>(fmaf(f[e], w[e], b[e]));
+            DlVec<T, W> out;
+            dl_pack(f, out);
+            *reinterpret_cast<DlVec<T, W>*>(y + first + r * pitch) = out;
+        }, x + first);
+    });
 }
 
-// partial (parts, 2, C): per team and row slice the sums of dz and dz * xh of every channel
-template <typename T, int W>
-__global__ void __launch_bounds__(MAX_LANES)
-norm_unit_bwd_kernel(const T* __restrict__ x, const T* __restrict__ gy, const float* __restrict__ mean_in,
-                     const float* __restrict__ rstd_in, T* __restrict__ gx, float* __restrict__ partial,
-                     const __grid_constant__ Norm p, const __grid_constant__ Cut k) {
-    extern __shared__ __align__(16) unsigned char shared_bytes[];
-    DlVec<T, W>* tile = reinterpret_cast<DlVec<T, W>*>(shared_bytes);
-    DlVec<T, W>* tile_g = tile + (size_t)k.cached * k.tx;
-    float* red = reinterpret_cast<float*>(shared_bytes + (size_t)2 * k.cached * k.tx * sizeof(DlVec<T, W>) / 16 * 16 + 16);
-    float* sums = red + (size_t)k.threads * (W > 2 ? W : 2);  // [2][groups]
-    float* shared_sums = sums + 2 * k.groups;                 // [2][2][groups], read by the other blocks
-    cg::cluster_group cluster = cg::this_cluster();
+// sums (N, G, parts, 2): the parts of s1 and s2.  partial (N * chunks, 2, C): the sums of dz and dz * xh of every channel
+template <typename T, int W, int DO>
+__global__ void __launch_bounds__(CHUNK_THREADS, 3)
+norm_chunk_bwd_kernel(const T* __restrict__ x, const T* __restrict__ gy, const float* __restrict__ mean_in,
+                      const float* __restrict__ rstd_in, T* __restrict__ gx, float* __restrict__ sums,
+                      float* __restrict__ partial, const __grid_constant__ Norm p, const __grid_constant__ Cut k) {
+    __shared__ float red[CHUNK_THREADS * (W > 2 ? W : 2)];
+    __shared__ float stats[2][MAX_LANES];  // s1 and s2 of the block's groups
     const Place at(p, k, W);
-    float w[W], b[W], sum_dz[W], sum_dzx[W];
-    if (at.live) load_params<W>(p, at.channel, w, b);
+    const int64_t pitch = p.C, first = (at.n * p.S + at.row0) * pitch + at.channel;
+    const int lane = threadIdx.x & 31, parts = k.chunks * k.split;
+    float w[W], b[W], rstd = 0.0f, off = 0.0f;  // xh = rstd * x + off
+    if (at.live) {
+        load_params<W>(p, at.channel, w, b);
+        rstd = rstd_in[at.n * p.G + at.group0 + at.group];
+        off = -mean_in[at.n * p.G + at.group0 + at.group] * rstd;
+    }
+    if (DO & SUMS) {
+        float dz_sum[W], dzx_sum[W], s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
-    for (int e = 0; e < W; ++e) sum_dz[e] = sum_dzx[e] = 0.0f;
-    const int cached = at.rows < k.cached ? at.rows : k.cached;
-    const int64_t team = blockIdx.x / k.cluster / k.blocks_c;
-    const int group0 = (int)(blockIdx.x / k.cluster % k.blocks_c) * k.groups;
-    const int64_t pitch = p.C;
-    const float over_m = 1.0f / ((float)p.S * (float)p.per_group);
-    int parity = 0;
-    for (int64_t n = team; n < p.N; n += k.teams, parity ^= 1) {
-        const int64_t from = (n * p.S + at.row0) * pitch + at.channel;
-        const T *src = x + from, *src_g = gy + from;
-        float part[2] = {0.0f, 0.0f}, rstd = 0.0f, off = 0.0f;  // xh = rstd * x + off
+        for (int e = 0; e < W; ++e) dz_sum[e] = dzx_sum[e] = 0.0f;
         if (at.live) {
-            for (int r = at.ty; r < cached; r += k.ty) {
-                copy_async<T, W>(&tile[r * k.tx + at.tx], reinterpret_cast<const DlVec<T, W>*>(src + r * pitch));
-                copy_async<T, W>(&tile_g[r * k.tx + at.tx], reinterpret_cast<const DlVec<T, W>*>(src_g + r * pitch));
-            }
-            rstd = rstd_in[n * p.G + group0 + at.group];
-            off = -mean_in[n * p.G + group0 + at.group] * rstd;
-            float unit_dz[W], unit_dzx[W];
-#pragma unroll
-            for (int e = 0; e < W; ++e) unit_dz[e] = unit_dzx[e] = 0.0f;
-            copy_wait_all();
             with_activation(p.act, [&](auto act) {
-                for (int r = at.ty; r < at.rows; r += k.ty) {
+                each_row<T, W>(at, k, pitch, [&](int, const DlVec<T, W>& v, const DlVec<T, W>& vg) {
                     float f[W], d[W];
-                    if (r < cached) {
-                        dl_unpack(tile[r * k.tx + at.tx], f);
-                        dl_unpack(tile_g[r * k.tx + at.tx], d);
-                    } else {
-                        dl_unpack(*reinterpret_cast<const DlVec<T, W>*>(src + r * pitch), f);
-                        dl_unpack(*reinterpret_cast<const DlVec<T, W>*>(src_g + r * pitch), d);
-                    }
+                    dl_unpack(v, f);
+                    dl_unpack(vg, d);
 #pragma unroll
                     for (int e = 0; e < W; ++e) {
                         const float xh = fmaf(f[e], rstd, off), dz = d[e] * slope<T, act.value>(fmaf(xh, w[e], b[e]));
-                        unit_dz[e] += dz;
-                        unit_dzx[e] = fmaf(dz, xh, unit_dzx[e]);
+                        dz_sum[e] += dz;
+                        dzx_sum[e] = fmaf(dz, xh, dzx_sum[e]);
                     }
-                }
+                }, x + first, gy + first);
             });
 #pragma unroll
             for (int e = 0; e < W; ++e) {
-                part[0] = fmaf(unit_dz[e], w[e], part[0]);
-                part[1] = fmaf(unit_dzx[e], w[e], part[1]);
-                sum_dz[e] += unit_dz[e];
-                sum_dzx[e] += unit_dzx[e];
+                s1 = fmaf(dz_sum[e], w[e], s1);
+                s2 = fmaf(dzx_sum[e], w[e], s2);
             }
         }
-        float* mine = k.cluster > 1 ? shared_sums + parity * 2 * k.groups : sums;
-        sum_groups<2>(part, at, k, red, mine);
-        float s1 = 0.0f, s2 = 0.0f;
-        if (k.cluster > 1) {
-            cluster.sync();
-            for (int r = 0; r < k.cluster; ++r) {
-                const float* other = cluster.map_shared_rank(mine, r);
-                s1 += other[at.group < k.groups ? at.group : 0];
-                s2 += other[k.groups + (at.group < k.groups ? at.group : 0)];
-            }
-        } else if (at.live) {
-            s1 = mine[at.group];
-            s2 = mine[k.groups + at.group];
-        }
-        if (at.live) {
-            // gx = rstd * w * dz - rstd * (s1 + xh * s2)
-            const float k1 = -rstd * s1 * over_m, k2 = -rstd * s2 * over_m;
-            float rw[W];
+        red[threadIdx.x] = s1;
+        red[CHUNK_THREADS + threadIdx.x] = s2;
+        __syncthreads();
+        warp_per_group(at, k, [&](int) { s1 = s2 = 0.0f; },
+            [&](int, int i) {
+                s1 += red[i];
+                s2 += red[CHUNK_THREADS + i];
+            },
+            [&](int g) {
 #pragma unroll
-            for (int e = 0; e < W; ++e) rw[e] = rstd * w[e];
-            T* dst = gx + from;
-            with_activation(p.act, [&](auto act) {
-                for (int r = at.ty; r < at.rows; r += k.ty) {
-                    float f[W], d[W];
-                    if (r < cached) {
-                        dl_unpack(tile[r * k.tx + at.tx], f);
-                        dl_unpack(tile_g[r * k.tx + at.tx], d);
-                    } else {
-                        dl_unpack(*reinterpret_cast<const DlVec<T, W>*>(src + r * pitch), f);
-                        dl_unpack(*reinterpret_cast<const DlVec<T, W>*>(src_g + r * pitch), d);
-                    }
-#pragma unroll
-                    for (int e = 0; e < W; ++e) {
-                        const float xh = fmaf(f[e], rstd, off), dz = d[e] * slope<T, act.value>(fmaf(xh, w[e], b[e]));
-                        f[e] = fmaf(dz, rw[e], fmaf(xh, k2, k1));
-                    }
-                    DlVec<T, W> out;
-                    dl_pack(f, out);
-                    *reinterpret_cast<DlVec<T, W>*>(dst + r * pitch) = out;
+                for (int s = 16; s > 0; s >>= 1) {
+                    s1 += __shfl_xor_sync(0xffffffffu, s1, s);
+                    s2 += __shfl_xor_sync(0xffffffffu, s2, s);
+                }
+                if (lane != 0) return;
+                if (DO & WRITE) {  // the only part
+                    stats[0][g] = s1;
+                    stats[1][g] = s2;
+                } else {
+                    float* out = sums + ((at.n * p.G + at.group0 + g) * parts + at.part(k)) * 2;
+                    out[0] = s1;
+                    out[1] = s2;
                 }
             });
+        if (partial != nullptr) {  // per channel over the rows of threads
+            const int channels = k.tx * W, valid = k.split > 1 ? at.group_lanes * W : at.groups * k.lanes * W;
+            float* out = partial + (at.n * k.chunks + at.chunk) * 2 * pitch + (at.channel - at.tx * W);
+#pragma unroll
+            for (int v = 0; v < 2; ++v) {
+                __syncthreads();
+                if (at.ty < k.ty) {
+#pragma unroll
+                    for (int e = 0; e < W; ++e) red[(at.ty * k.tx + at.tx) * W + e] = v == 0 ? dz_sum[e] : dzx_sum[e];
+                }
+                __syncthreads();
+                for (int c = threadIdx.x; c < valid; c += blockDim.x) {
+                    float sum = 0.0f;
+                    for (int r = 0; r < k.ty; ++r) sum += red[r * channels + c];
+                    out[v * pitch + c] = sum;
+                }
+            }
         }
     }
-    if (k.cluster > 1) cluster.sync();  // nobody leaves while others read its sums
-    if (partial == nullptr) return;
-    // per channel over the rows of threads
-    const int channels = k.tx * W;
-    const int64_t slice = k.by_channel ? team : team * k.cluster + at.rank;
+    if (!(DO & WRITE)) return;
+    if (!(DO & SUMS)) {
+        for (int g = threadIdx.x / 32; g < at.groups; g += blockDim.x / 32) {
+            const float2* in = reinterpret_cast<const float2*>(sums) + (at.n * p.G + at.group0 + g) * parts;
+            float s1 = 0.0f, s2 = 0.0f;
+            for (int i = lane; i < parts; i += 32) {
+                s1 += in[i].x;
+                s2 += in[i].y;
+            }
 #pragma unroll
-    for (int v = 0; v < 2; ++v) {
-        __syncthreads();
-        if (at.live) {
-#pragma unroll
-            for (int e = 0; e < W; ++e) red[(at.ty * k.tx + at.tx) * W + e] = v == 0 ? sum_dz[e] : sum_dzx[e];
-        }
-        __syncthreads();
-        const int first = (int)(blockIdx.x / k.cluster % k.blocks_c) * k.groups * k.lanes * W +
-                          (k.by_channel ? at.rank * channels : 0);
-        const int valid = k.by_channel ? at.group_lanes * W : channels;
-        for (int c = threadIdx.x; c < valid; c += k.threads) {
-            float sum = 0.0f;
-            for (int r = 0; r < k.ty; ++r) sum += red[r * channels + c];
-            partial[(slice * 2 + v) * p.C + first + c] = sum;
+            for (int s = 16; s > 0; s >>= 1) {
+                s1 += __shfl_xor_sync(0xffffffffu, s1, s);
+                s2 += __shfl_xor_sync(0xffffffffu, s2, s);
+            }
+            if (lane == 0) {
+                stats[0][g] = s1;
+                stats[1][g] = s2;
+            }
         }
     }
+    __syncthreads();
+    if (!at.live) return;
+    // gx = rstd * w * dz - rstd * (s1 + xh * s2) / m
+    const float over_m = 1.0f / ((float)p.S * (float)p.per_group);
+    const float k1 = -rstd * stats[0][at.group] * over_m, k2 = -rstd * stats[1][at.group] * over_m;
+    with_activation(p.act, [&](auto act) {
+        each_row<T, W>(at, k, pitch, [&](int r, const DlVec<T, W>& v, const DlVec<T, W>& vg) {
+            float f[W], d[W];
+            dl_unpack(v, f);
+            dl_unpack(vg, d);
+#pragma unroll
+            for (int e = 0; e < W; ++e) {
+                const float xh = fmaf(f[e], rstd, off), dz = d[e] * slope<T, act.value>(fmaf(xh, w[e], b[e]));
+                f[e] = fmaf(dz * w[e], rstd, fmaf(xh, k2, k1));
+            }
+            DlVec<T, W> out;
+            dl_pack(f, out);
+            *reinterpret_cast<DlVec<T, W>*>(gx + first + r * pitch) = out;
+        }, x + first, gy + first);
+    });
 }
 
 // ------------------------------------------------------------------------------------------ rows without positions
@@ -437,7 +459,7 @@ __device__ __forceinline__ float sum_lanes(float v, int lanes_log2) {
 constexpr int ROW_THREADS = 256;
 
 template <typename T, int W, int ITEMS>
-__global__ void __launch_bounds__(ROW_THREADS)
+__global__ void __launch_bounds__(ROW_THREADS, 4)
 norm_rows_kernel(const T* __restrict__ x, T* __restrict__ y, float* __restrict__ mean_out, float* __restrict__ rstd_out,
                  const __grid_constant__ Norm p, const __grid_constant__ RowCut k) {
     const int slot = blockIdx.y * k.tx + threadIdx.x % k.tx, ty = threadIdx.x / k.tx;
@@ -492,7 +514,7 @@ norm_rows_kernel(const T* __restrict__ x, T* __restrict__ y, float* __restrict__
 }
 
 template <typename T, int W, int ITEMS>
-__global__ void __launch_bounds__(ROW_THREADS)
+__global__ void __launch_bounds__(ROW_THREADS, 3)
 norm_rows_bwd_kernel(const T* __restrict__ x, const T* __restrict__ gy, const float* __restrict__ mean_in,
                      const float* __restrict__ rstd_in, T* __restrict__ gx, float* __restrict__ partial,
                      const __grid_constant__ Norm p, const __grid_constant__ RowCut k) {
@@ -598,65 +620,32 @@ norm_params_kernel(const float* __restrict__ partial, int64_t parts, int C, void
 }
 
 // ------------------------------------------------------------------------------------------ host
-constexpr size_t SHARED_MOST = 227 * 1024;    // of a block
-constexpr size_t SHARED_LIMIT = 190 * 1024;   // of these for tiles
-constexpr size_t SHARED_WANTED = 64 * 1024;   // so that about three blocks share an SM and overlap their phases
-
-// false: the groups are too wide.  `tensors` are held at once (1 forward, 2 backward).
-bool cut_units(const Norm& p, int W, int64_t esize, int tensors, bool accumulate, Cut& k) {
+// `resident` blocks of a launch fit an SM
+Cut cut_chunks(const Norm& p, int W, int resident) {
+    Cut k;
     k.lanes = p.per_group / W;
-    k.cluster = 1;
-    k.by_channel = k.lanes > MAX_LANES;
-    if (k.by_channel) {
-        while (k.cluster < MAX_CLUSTER && dl_ceil_div(k.lanes, k.cluster) > MAX_LANES) k.cluster *= 2;
-        if (dl_ceil_div(k.lanes, k.cluster) > MAX_LANES) return false;
-        k.groups = 1;
-        k.tx = (int)dl_ceil_div(k.lanes, k.cluster);
-    } else {
-        // the fewest groups that are 128 bytes wide together; 64 or 32 when the unit would not fit a cluster at the
-        // wanted size, or when there would be too few units for the SMs
-        for (int64_t width = 128; width >= 32; width /= 2) {
-            k.groups = 1;
-            while (k.groups < p.G && (p.G % k.groups != 0 || (int64_t)k.groups * p.per_group * esize < width)) ++k.groups;
-            const int64_t unit = p.S * k.groups * p.per_group * esize * tensors;
-            if (unit <= (int64_t)SHARED_WANTED * MAX_CLUSTER && p.N * (p.G / k.groups) * MAX_CLUSTER >= DL_NUM_SMS) break;
-        }
-        // all groups of a block need a lane each; wide groups of one-element vectors may not fit
-        while (k.groups * k.lanes > MAX_LANES) {
-            --k.groups;
-            while (p.G % k.groups != 0) --k.groups;
-        }
-        k.tx = k.groups * k.lanes;
-    }
-    k.blocks_c = p.G / k.groups;
-    const int64_t row_bytes = (int64_t)k.tx * W * esize * tensors;
-    const int most_threads = k.tx > 256 ? MAX_LANES : 256;
-    if (!k.by_channel) {
-        // a cluster when the unit is large, or when there are too few units for all SMs
-        const int64_t units = p.N * k.blocks_c;
-        while (k.cluster < MAX_CLUSTER && p.S >= 16 * k.cluster &&
-               (p.S * row_bytes > (int64_t)SHARED_WANTED * k.cluster ||
-                (units * k.cluster < 2 * DL_NUM_SMS && p.S * k.tx > 2 * (int64_t)most_threads * k.cluster)))
-            k.cluster *= 2;
-    }
-    const int64_t rows = k.by_channel ? p.S : dl_ceil_div(p.S, k.cluster);
-    if (rows > 0x7fffffff / 2) return false;
-    k.rows = (int)rows;
-    k.cached = (int)dl_min64(rows, dl_max64((int64_t)SHARED_LIMIT / row_bytes, 1));
-    k.ty = (int)dl_max64(dl_min64(rows, most_threads / k.tx), 1);
-    k.threads = (int)dl_ceil_div(k.tx * k.ty, 32) * 32;
-    // tiles (rounded up), sums of threads (of channels at the end of the backward pass), and a few floats per group
-    k.shared = (size_t)(k.cached * row_bytes + 32) + (size_t)k.threads * 4 * (accumulate && W > 2 ? W : 2) +
-               (size_t)k.groups * 4 * 10;
-    k.teams = p.N;
-    if (accumulate) {
-        // as many clusters as are resident at once, each with the same number of samples, give or take one
-        const int64_t resident = dl_max64(dl_min64((int64_t)(220 * 1024 / (k.shared + 1024)), 1024 / k.threads), 1);
-        const int64_t at_once = dl_max64(DL_NUM_SMS * resident / ((int64_t)k.blocks_c * k.cluster), 1);
-        k.teams = dl_ceil_div(p.N, dl_ceil_div(p.N, at_once));
-    }
-    return true;
+    k.split = (int)dl_ceil_div(k.lanes, MAX_LANES);
+    k.groups = k.split > 1 ? 1 : (int)dl_min64(MAX_LANES / k.lanes, p.G);
+    k.tx = k.split > 1 ? (int)dl_ceil_div(k.lanes, k.split) : k.groups * k.lanes;
+    k.ty = (int)dl_min64(CHUNK_THREADS / k.tx, p.S);
+    k.blocks_c = (int)(dl_ceil_div(p.G, k.groups) * k.split);
+    // as many chunks as are resident at once, but at least two rounds of loads in each; a sample whose groups are split
+    // over blocks of channels always takes two launches
+    const int64_t units = p.N * k.blocks_c, slots = (int64_t)DL_NUM_SMS * resident;
+    const int64_t most = dl_max64(p.S / ((int64_t)k.ty * IN_FLIGHT * 2), 1);
+    k.chunks = (int)dl_max64(dl_min64(slots / dl_max64(units, 1), most), 1);
+    k.rows = (int)dl_ceil_div(p.S, k.chunks);
+    k.chunks = (int)dl_ceil_div(p.S, k.rows);
+    return k;
 }
+constexpr int RESIDENT = 4, RESIDENT_BWD = 3;  // the kernels' launch bounds
+
+unsigned threads_of(const Cut& k) { return (unsigned)(dl_ceil_div(k.tx * k.ty, 32) * 32); }
+bool one_launch(const Cut& k) { return k.chunks == 1 && k.split == 1; }
+int64_t sums_floats(const Norm& p, const Cut& k) {
+    return one_launch(k) ? 0 : p.N * p.G * (int64_t)k.chunks * k.split * 2;
+}
+bool grid_fits(const Norm& p, const Cut& k) { return p.N * k.blocks_c * (int64_t)k.chunks <= 0x7fffffff; }
 
 bool cut_rows(const Norm& p, int W, int items, int64_t most_blocks, RowCut& k) {
     if (p.S != 1 || p.per_group / W > 32) return false;
@@ -673,23 +662,11 @@ bool cut_rows(const Norm& p, int W, int items, int64_t most_blocks, RowCut& k) {
     return true;
 }
 
-constexpr int ROW_ITEMS = 4, ROW_ITEMS_BWD = 2;
-constexpr int64_t ROW_BLOCKS = DL_NUM_SMS * 16, ROW_BLOCKS_BWD = DL_NUM_SMS * 4;
-
-void unit_config(const Cut& k, cudaLaunchConfig_t& cfg, cudaLaunchAttribute* attr, cudaStream_t s) {
-    cfg.gridDim = dim3((unsigned)(k.teams * k.blocks_c * k.cluster));
-    cfg.blockDim = dim3((unsigned)k.threads);
-    cfg.dynamicSmemBytes = k.shared;
-    cfg.stream = s;
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)k.cluster;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-}
+constexpr int ROW_ITEMS = 2, ROW_ITEMS_BWD = 1;
+constexpr int64_t ROW_BLOCKS = DL_NUM_SMS * 16, ROW_BLOCKS_BWD = DL_NUM_SMS * 3;
 
 template <typename T, int W>
-int launch_forward(const void* x, void* y, float* mean, float* rstd, const Norm& p, cudaStream_t s) {
+int launch_forward(const void* x, void* y, float* mean, float* rstd, float* sums, const Norm& p, cudaStream_t s) {
     const T* src = static_cast<const T*>(x);
     T* dst = static_cast<T*>(y);
     RowCut r;
@@ -698,66 +675,77 @@ int launch_forward(const void* x, void* y, float* mean, float* rstd, const Norm&
             src, dst, mean, rstd, p, r);
         return dl_launch_status();
     }
-    Cut k;
-    if (!cut_units(p, W, sizeof(T), 1, false, k)) return DL_ERR_TOO_LARGE;
-    if (k.teams * k.blocks_c * k.cluster > 0x7fffffff) return DL_ERR_TOO_LARGE;
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[1];
-    const auto kernel = norm_unit_kernel<T, W>;
-    static DlKernelLimits limits;
-    if (!dl_allow(reinterpret_cast<const void*>(kernel), limits, SHARED_MOST, false)) return DL_ERR_LAUNCH;
-    unit_config(k, cfg, attr, s);
-    return cudaLaunchKernelEx(&cfg, kernel, src, dst, mean, rstd, p, k) == cudaSuccess ? dl_launch_status()
-                                                                                      : DL_ERR_LAUNCH;
+    const Cut k = cut_chunks(p, W, RESIDENT);
+    if (!grid_fits(p, k)) return DL_ERR_TOO_LARGE;
+    const unsigned blocks = (unsigned)(p.N * k.blocks_c * k.chunks);
+    if (one_launch(k)) {
+        norm_chunk_kernel<T, W, SUMS | WRITE><<<blocks, threads_of(k), 0, s>>>(src, dst, mean, rstd, sums, p, k);
+        return dl_launch_status();
+    }
+    norm_chunk_kernel<T, W, SUMS><<<blocks, threads_of(k), 0, s>>>(src, dst, mean, rstd, sums, p, k);
+    if (cudaPeekAtLastError() != cudaSuccess) return DL_ERR_LAUNCH;
+    norm_chunk_kernel<T, W, WRITE><<<blocks, threads_of(k), 0, s>>>(src, dst, mean, rstd, sums, p, k);
+    return dl_launch_status();
 }
 
-// rows of `partial` that the backward pass with vectors of W writes; 0: not supported
-int64_t backward_parts(const Norm& p, int W, int64_t esize) {
+// floats of workspace: sums of the chunks, then the partial sums of the parameters' gradients
+int64_t forward_floats(const Norm& p, int W) {
     RowCut r;
-    if (cut_rows(p, W, ROW_ITEMS_BWD, ROW_BLOCKS_BWD, r)) return r.blocks_x;
-    Cut k;
-    if (!cut_units(p, W, esize, 2, true, k)) return 0;
-    return k.by_channel ? k.teams : k.teams * k.cluster;
+    if (cut_rows(p, W, ROW_ITEMS, ROW_BLOCKS, r)) return 0;
+    return sums_floats(p, cut_chunks(p, W, RESIDENT));
+}
+int64_t backward_floats(const Norm& p, int W, int64_t& parts) {
+    RowCut r;
+    if (cut_rows(p, W, ROW_ITEMS_BWD, ROW_BLOCKS_BWD, r)) {
+        parts = r.blocks_x;
+        return 0;
+    }
+    const Cut k = cut_chunks(p, W, RESIDENT_BWD);
+    parts = p.N * k.chunks;
+    return sums_floats(p, k);
 }
 
 template <typename T, int W>
 int launch_backward(const void* x, const void* g, const float* mean, const float* rstd, void* gx, void* gweight,
-                    void* gbias, float* partial, const Norm& p, cudaStream_t s) {
+                    void* gbias, float* scratch, const Norm& p, cudaStream_t s) {
     const T *src = static_cast<const T*>(x), *src_g = static_cast<const T*>(g);
     T* dst = static_cast<T*>(gx);
+    int64_t parts;
+    float* partial = scratch + backward_floats(p, W, parts);
     if (gweight == nullptr && gbias == nullptr) partial = nullptr;
     RowCut r;
     if (cut_rows(p, W, ROW_ITEMS_BWD, ROW_BLOCKS_BWD, r)) {
         norm_rows_bwd_kernel<T, W, ROW_ITEMS_BWD>
             <<<dim3((unsigned)r.blocks_x, (unsigned)r.blocks_c), ROW_THREADS, 0, s>>>(src, src_g, mean, rstd, dst, partial,
                                                                                      p, r);
-        if (cudaPeekAtLastError() != cudaSuccess) return DL_ERR_LAUNCH;
     } else {
-        Cut k;
-        if (!cut_units(p, W, sizeof(T), 2, true, k)) return DL_ERR_TOO_LARGE;
-        if (k.teams * k.blocks_c * k.cluster > 0x7fffffff) return DL_ERR_TOO_LARGE;
-        cudaLaunchConfig_t cfg = {};
-        cudaLaunchAttribute attr[1];
-        const auto kernel = norm_unit_bwd_kernel<T, W>;
-        static DlKernelLimits limits;
-        if (!dl_allow(reinterpret_cast<const void*>(kernel), limits, SHARED_MOST, false)) return DL_ERR_LAUNCH;
-        unit_config(k, cfg, attr, s);
-        if (cudaLaunchKernelEx(&cfg, kernel, src, src_g, mean, rstd, dst, partial, p, k) != cudaSuccess)
-            return DL_ERR_LAUNCH;
+        const Cut k = cut_chunks(p, W, RESIDENT_BWD);
+        if (!grid_fits(p, k)) return DL_ERR_TOO_LARGE;
+        const unsigned blocks = (unsigned)(p.N * k.blocks_c * k.chunks);
+        if (one_launch(k)) {
+            norm_chunk_bwd_kernel<T, W, SUMS | WRITE><<<blocks, threads_of(k), 0, s>>>(src, src_g, mean, rstd, dst, scratch,
+                                                                                      partial, p, k);
+        } else {
+            norm_chunk_bwd_kernel<T, W, SUMS><<<blocks, threads_of(k), 0, s>>>(src, src_g, mean, rstd, dst, scratch, partial,
+                                                                              p, k);
+            if (cudaPeekAtLastError() != cudaSuccess) return DL_ERR_LAUNCH;
+            norm_chunk_bwd_kernel<T, W, WRITE><<<blocks, threads_of(k), 0, s>>>(src, src_g, mean, rstd, dst, scratch,
+                                                                               partial, p, k);
+        }
     }
+    if (cudaPeekAtLastError() != cudaSuccess) return DL_ERR_LAUNCH;
     if (partial != nullptr)
-        norm_params_kernel<<<(unsigned)dl_ceil_div(p.C, 32), 1024, 0, s>>>(partial, backward_parts(p, W, sizeof(T)), p.C,
-                                                                         gweight, gbias, p.param_dtype);
+        norm_params_kernel<<<(unsigned)dl_ceil_div(p.C, 32), 1024, 0, s>>>(partial, parts, p.C, gweight, gbias, p.param_dtype);
     return dl_launch_status();
 }
 
 template <typename T>
-int forward_width(const void* x, void* y, float* mean, float* rstd, const Norm& p, cudaStream_t s) {
+int forward_width(const void* x, void* y, float* mean, float* rstd, float* sums, const Norm& p, cudaStream_t s) {
     const int w = dl_vector_width(sizeof(T), p.per_group, dl_address(x) | dl_address(y));
-    if (w == 16 / (int)sizeof(T)) return launch_forward<T, 16 / sizeof(T)>(x, y, mean, rstd, p, s);
-    if (w == 4) return launch_forward<T, 4>(x, y, mean, rstd, p, s);
-    if (w == 2) return launch_forward<T, 2>(x, y, mean, rstd, p, s);
-    return launch_forward<T, 1>(x, y, mean, rstd, p, s);
+    if (w == 16 / (int)sizeof(T)) return launch_forward<T, 16 / sizeof(T)>(x, y, mean, rstd, sums, p, s);
+    if (w == 4) return launch_forward<T, 4>(x, y, mean, rstd, sums, p, s);
+    if (w == 2) return launch_forward<T, 2>(x, y, mean, rstd, sums, p, s);
+    return launch_forward<T, 1>(x, y, mean, rstd, sums, p, s);
 }
 
 template <typename T>
@@ -788,25 +776,37 @@ bool describe(int64_t N, int64_t S, int64_t C, int64_t G, int64_t dtype, Norm& p
 
 }  // namespace
 
+// Addresses may rule out the wider vectors: the workspaces are large enough for every width that the sizes allow.
+DL_EXPORT int64_t dl_group_norm_scratch_bytes(int64_t N, int64_t S, int64_t C, int64_t G, int64_t dtype) {
+    Norm p;
+    if (!describe(N, S, C, G, dtype, p)) return -1;
+    int64_t floats = 0;
+    for (int w = dl_vector_width(dl_dtype_size(dtype), p.per_group, 0); w >= 1; w /= 2)
+        floats = dl_max64(floats, forward_floats(p, w));
+    return floats * 4;
+}
+
 DL_EXPORT int64_t dl_group_norm_bwd_scratch_bytes(int64_t N, int64_t S, int64_t C, int64_t G, int64_t dtype) {
     Norm p;
-    if (!describe(N, S, C, G, dtype, p)) return 0;
-    if (N == 0) return 256;
-    // the widest partial table of the vector widths that these sizes allow: addresses may rule out the wider ones
-    int64_t parts = 0;
-    for (int w = dl_vector_width(dl_dtype_size(dtype), p.per_group, 0); w >= 1; w /= 2)
-        parts = dl_max64(parts, backward_parts(p, w, dl_dtype_size(dtype)));
-    return parts * 2 * C * 4;
+    if (!describe(N, S, C, G, dtype, p)) return -1;
+    int64_t floats = 0, parts;
+    for (int w = dl_vector_width(dl_dtype_size(dtype), p.per_group, 0); w >= 1; w /= 2) {
+        const int64_t sums = backward_floats(p, w, parts);
+        floats = dl_max64(floats, sums + parts * 2 * C);
+    }
+    return floats * 4;
 }
 
 DL_EXPORT int dl_group_norm(const void* x, const void* weight, const void* bias, void* y, float* mean, float* rstd,
-                            int64_t N, int64_t S, int64_t C, int64_t G, int64_t dtype, int64_t param_dtype,
+                            void* scratch, int64_t N, int64_t S, int64_t C, int64_t G, int64_t dtype, int64_t param_dtype,
                             int64_t activation, float eps, dl_stream_t stream) {
     Norm p;
     DL_REQUIRE(describe(N, S, C, G, dtype, p) && dl_dtype_known(param_dtype));
     DL_REQUIRE(activation >= ACT_NONE && activation <= ACT_SIGMOID && eps >= 0.0f);
     if (N == 0) return DL_OK;
     DL_REQUIRE(x && y && (mean == nullptr) == (rstd == nullptr));
+    DL_REQUIRE(scratch || dl_group_norm_scratch_bytes(N, S, C, G, dtype) == 0);
+    DL_REQUIRE_ALIGNED(scratch, 16);
     DL_REQUIRE_ALIGNED(x, dl_dtype_size(dtype));
     DL_REQUIRE_ALIGNED(y, dl_dtype_size(dtype));
     p.weight = weight;
@@ -815,9 +815,10 @@ DL_EXPORT int dl_group_norm(const void* x, const void* weight, const void* bias,
     p.eps = eps;
     p.act = (int)activation;
     cudaStream_t s = dl_cast(stream);
-    if (dtype == DL_DTYPE_F32) return forward_width<float>(x, y, mean, rstd, p, s);
-    if (dtype == DL_DTYPE_BF16) return forward_width<__nv_bfloat16>(x, y, mean, rstd, p, s);
-    return forward_width<__half>(x, y, mean, rstd, p, s);
+    float* sums = static_cast<float*>(scratch);
+    if (dtype == DL_DTYPE_F32) return forward_width<float>(x, y, mean, rstd, sums, p, s);
+    if (dtype == DL_DTYPE_BF16) return forward_width<__nv_bfloat16>(x, y, mean, rstd, sums, p, s);
+    return forward_width<__half>(x, y, mean, rstd, sums, p, s);
 }
 
 DL_EXPORT int dl_group_norm_bwd(const void* x, const void* g, const void* weight, const void* bias, const float* mean,
@@ -834,7 +835,7 @@ DL_EXPORT int dl_group_norm_bwd(const void* x, const void* g, const void* weight
         if (gbias && cudaMemsetAsync(gbias, 0, bytes, s) != cudaSuccess) return DL_ERR_LAUNCH;
         return DL_OK;
     }
-    DL_REQUIRE(x && g && mean && rstd && gx && (scratch || (!gweight && !gbias)));
+    DL_REQUIRE(x && g && mean && rstd && gx && scratch);
     DL_REQUIRE_ALIGNED(x, dl_dtype_size(dtype));
     DL_REQUIRE_ALIGNED(g, dl_dtype_size(dtype));
     DL_REQUIRE_ALIGNED(gx, dl_dtype_size(dtype));

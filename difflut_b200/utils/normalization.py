@@ -25,7 +25,10 @@ def _check_activation(activation) -> int:
 
 @functools.lru_cache(maxsize=1024)
 def _scratch_bytes(N, S, C, G, code):
-    return int(_native.lib().dl_group_norm_bwd_scratch_bytes(N, S, C, G, code))
+    """Workspace of (the forward, the backward pass)."""
+    lib = _native.lib()
+    return (int(lib.dl_group_norm_scratch_bytes(N, S, C, G, code)),
+            int(lib.dl_group_norm_bwd_scratch_bytes(N, S, C, G, code)))
 
 
 def _address(t):
@@ -33,43 +36,44 @@ def _address(t):
 
 
 def _forward(x, weight, bias, dims, eps, act, keep):
+    """(result, mean and rstd behind the workspace, their address), the latter two for the backward pass only."""
     N, S, C, G, param_code = dims
+    code = _native.DTYPE_CODES[x.dtype]
     y = torch.empty_like(x)
-    stats = x.new_empty((2, N, G), dtype=torch.float32) if keep else None
-    mean = _address(stats)
+    size = _scratch_bytes(N, S, C, G, code)[0]
+    held = x.new_empty(size // 4 + (2 * N * G if keep else 0), dtype=torch.float32) if keep or size else None
+    scratch = _address(held)
+    mean = scratch + size if keep else None
     with _native.device_of(x):
         _native.entry("dl_group_norm")(x.data_ptr(), _address(weight), _address(bias), y.data_ptr(), mean,
-                                       mean + 4 * N * G if keep else None, N, S, C, G, _native.DTYPE_CODES[x.dtype],
-                                       param_code, act, eps)
-    return y, stats
+                                       mean + 4 * N * G if keep else None, scratch, N, S, C, G, code, param_code, act, eps)
+    return y, held, size
 
 
 class _GroupNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, dims, eps, act):
-        y, stats = _forward(x, weight, bias, dims, eps, act, True)
-        ctx.save_for_backward(x, weight, bias, stats)
-        ctx.spec = (dims, act)
+        y, held, mean_at = _forward(x, weight, bias, dims, eps, act, True)
+        ctx.save_for_backward(x, weight, bias, held)
+        ctx.spec = (dims, act, mean_at)
         return y
 
     @staticmethod
     @_native.once_differentiable_backward
     def backward(ctx, g):
-        x, weight, bias, stats = ctx.saved_tensors
-        (N, S, C, G, param_code), act = ctx.spec
+        x, weight, bias, held = ctx.saved_tensors
+        (N, S, C, G, param_code), act, mean_at = ctx.spec
         code = _native.DTYPE_CODES[x.dtype]
         g = g.contiguous()
         gx = torch.empty_like(x)
         gw = torch.empty_like(weight) if weight is not None and ctx.needs_input_grad[1] else None
         gb = torch.empty_like(bias) if bias is not None and ctx.needs_input_grad[2] else None
-        scratch = None
-        if gw is not None or gb is not None:
-            scratch = x.new_empty(_scratch_bytes(N, S, C, G, code), dtype=torch.uint8)
-        mean = stats.data_ptr()
+        scratch = x.new_empty(_scratch_bytes(N, S, C, G, code)[1], dtype=torch.uint8)
+        mean = held.data_ptr() + mean_at
         with _native.device_of(x):
             _native.entry("dl_group_norm_bwd")(x.data_ptr(), g.data_ptr(), _address(weight), _address(bias), mean,
                                                mean + 4 * N * G, gx.data_ptr(), _address(gw), _address(gb),
-                                               _address(scratch), N, S, C, G, code, param_code, act)
+                                               scratch.data_ptr(), N, S, C, G, code, param_code, act)
         return gx, gw, gb, None, None, None
 
 
@@ -113,8 +117,6 @@ def group_norm(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor] 
     weight = None if weight is None else weight.contiguous()
     bias = None if bias is None else bias.contiguous()
     dims = (N, S, C, num_groups, 0 if param_dtype is None else _native.DTYPE_CODES[param_dtype])
-    if _scratch_bytes(*dims[:4], _native.DTYPE_CODES[x.dtype]) == 0:
-        raise ValueError(f"groups of {C // num_groups} channels are wider than group_norm supports")
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
                                     or (bias is not None and bias.requires_grad)):
         return _GroupNormFn.apply(x, weight, bias, dims, float(eps), act)

@@ -571,13 +571,12 @@ int dl_embedding_bwd(const void* order, const void* g, void* gw, int64_t tokens,
  *   the S * C/G values of a sample's group; activation 0 none, 1 relu, 2 silu, 3 sigmoid.
  *   dl_group_norm       mean / rstd may be null (both).
  *   dl_group_norm_bwd   gx, and gweight / gbias where not null, from the mean / rstd of the forward call.
- *                       scratch: dl_group_norm_bwd_scratch_bytes bytes, 16-byte aligned (not needed when
- *                       both are null).  Fixed order of additions: run-to-run the same bits.
- * A group may be up to 4096 vectors wide (the widest power-of-two vector up to 16 bytes that C/G and the
- * addresses allow); wider ones return DL_ERR_TOO_LARGE (scratch size 0).                    */
-int dl_group_norm(const void* x, const void* weight, const void* bias, void* y, float* mean, float* rstd, int64_t N,
-                  int64_t S, int64_t C, int64_t G, int64_t dtype, int64_t param_dtype, int64_t activation, float eps,
-                  dl_stream_t stream);
+ * scratch: dl_group_norm_scratch_bytes / dl_group_norm_bwd_scratch_bytes bytes (0: none is needed, -1: the sizes are
+ * not valid), 16-byte aligned.  Fixed order of additions: run-to-run the same bits.           */
+int64_t dl_group_norm_scratch_bytes(int64_t N, int64_t S, int64_t C, int64_t G, int64_t dtype);
+int dl_group_norm(const void* x, const void* weight, const void* bias, void* y, float* mean, float* rstd, void* scratch,
+                  int64_t N, int64_t S, int64_t C, int64_t G, int64_t dtype, int64_t param_dtype, int64_t activation,
+                  float eps, dl_stream_t stream);
 int64_t dl_group_norm_bwd_scratch_bytes(int64_t N, int64_t S, int64_t C, int64_t G, int64_t dtype);
 int dl_group_norm_bwd(const void* x, const void* g, const void* weight, const void* bias, const float* mean,
                       const float* rstd, void* gx, void* gweight, void* gbias, void* scratch, int64_t N, int64_t S,
