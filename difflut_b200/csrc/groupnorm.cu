@@ -9,7 +9,7 @@
 // one adds up its sample's (a few hundred numbers) and writes.  Where samples alone fill the GPU a chunk is a sample and
 // one launch does both.  The second reading comes from L2 as far as the tensor fits there.  (Holding a sample in the shared
 // memory of a cluster, so that it is read once, was slower: all blocks load, then all compute, then all store, and each
-// sample costs a cluster barrier; 51 us instead of 38 us for 16 x 4096 x 512 bf16 forward.)
+// sample costs a cluster barrier: 51 us instead of 46 us forward, 90 instead of 80 us backward for 16 x 4096 x 512 bf16.)
 // A thread keeps to its own channels (a vector of W).  Rows without positions (S = 1) take kernels of their own, in which a
 // group is a few lanes of a warp and stays in registers.
 //
@@ -444,177 +444,224 @@ norm_chunk_bwd_kernel(const T* __restrict__ x, const T* __restrict__ gy, const f
 
 // ------------------------------------------------------------------------------------------ rows without positions
 // S = 1: a group is `lanes` lanes (padded to 2^lanes_log2 <= 32) of a warp, a block covers tx lanes of ty rows.
+// Vectors of four channels at most: parameters, sums and the rows in flight then fit the registers.
+constexpr int ROW_THREADS = 256;
+constexpr int ROW_WIDTH = 4;
+
 struct RowCut {
     int lanes, lanes_log2;
     int tx, ty;
+    int rows;          // per block
     int64_t blocks_x;  // down the rows
     int blocks_c;      // across the channels
 };
 
-__device__ __forceinline__ float sum_lanes(float v, int lanes_log2) {
-    for (int s = 1 << lanes_log2 >> 1; s > 0; s >>= 1) v += __shfl_xor_sync(0xffffffffu, v, s);
-    return v;
+template <int ITEMS>
+__device__ __forceinline__ void sum_lanes(float (&v)[ITEMS], int lanes_log2) {
+    for (int s = 1 << lanes_log2 >> 1; s > 0; s >>= 1) {
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], s);
+    }
 }
 
-constexpr int ROW_THREADS = 256;
+struct RowPlace {
+    int tx, ty, group, channel, first_lane;
+    int64_t row0;
+    int rows;  // of the block
+    bool live;
+    __device__ __forceinline__ RowPlace(const Norm& p, const RowCut& k, int W) {
+        tx = threadIdx.x % k.tx;
+        ty = threadIdx.x / k.tx;
+        const int slot = blockIdx.y * k.tx + tx, j = slot & ((1 << k.lanes_log2) - 1);
+        group = slot >> k.lanes_log2;
+        live = group < p.G && j < k.lanes && ty < k.ty;
+        channel = group * p.per_group + j * W;
+        first_lane = j == 0;
+        row0 = (int64_t)blockIdx.x * k.rows;
+        rows = (int)(p.N - row0 < k.rows ? p.N - row0 : k.rows);
+    }
+};
 
 template <typename T, int W, int ITEMS>
 __global__ void __launch_bounds__(ROW_THREADS, 4)
 norm_rows_kernel(const T* __restrict__ x, T* __restrict__ y, float* __restrict__ mean_out, float* __restrict__ rstd_out,
                  const __grid_constant__ Norm p, const __grid_constant__ RowCut k) {
-    const int slot = blockIdx.y * k.tx + threadIdx.x % k.tx, ty = threadIdx.x / k.tx;
-    const int group = slot >> k.lanes_log2, j = slot & ((1 << k.lanes_log2) - 1);
-    const bool live = group < p.G && j < k.lanes && ty < k.ty;
-    const int channel = group * p.per_group + j * W;
+    const RowPlace at(p, k, W);
+    const T* src = x + (at.row0 + at.ty) * p.C + at.channel;
+    T* dst = y + (at.row0 + at.ty) * p.C + at.channel;
+    const int64_t step = (int64_t)k.ty * p.C;
     float w[W], b[W];
-    bool first = true;
     const float over_m = 1.0f / (float)p.per_group;
     with_activation(p.act, [&](auto act) {
-    for (int64_t n0 = (int64_t)blockIdx.x * k.ty * ITEMS; n0 < p.N; n0 += (int64_t)gridDim.x * k.ty * ITEMS) {
-        DlVec<T, W> in[ITEMS];
+        for (int r0 = 0; r0 < at.rows; r0 += k.ty * ITEMS, src += ITEMS * step, dst += ITEMS * step) {
+            DlVec<T, W> in[ITEMS];
+            bool here[ITEMS];
+            float mean[ITEMS], square[ITEMS];
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i) {
-            const int64_t n = n0 + i * k.ty + ty;
-            if (live && n < p.N) in[i] = *reinterpret_cast<const DlVec<T, W>*>(x + n * p.C + channel);
-        }
-        if (first && live) load_params<W>(p, channel, w, b);  // behind the first rows' loads
-        first = false;
+            for (int i = 0; i < ITEMS; ++i) {
+                here[i] = at.live && r0 + i * k.ty + at.ty < at.rows;
+                if (here[i]) in[i] = *reinterpret_cast<const DlVec<T, W>*>(src + i * step);
+            }
+            if (r0 == 0 && at.live) load_params<W>(p, at.channel, w, b);  // behind the first rows' loads
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i) {
-            const int64_t n = n0 + i * k.ty + ty;
-            const bool here = live && n < p.N;
-            float f[W], sum = 0.0f, squares = 0.0f;
-            if (here) {
+            for (int i = 0; i < ITEMS; ++i) {
+                mean[i] = 0.0f;
+                if (!here[i]) continue;
+                float f[W];
                 dl_unpack(in[i], f);
 #pragma unroll
-                for (int e = 0; e < W; ++e) sum += f[e];
+                for (int e = 0; e < W; ++e) mean[i] += f[e];
             }
-            const float mean = sum_lanes(sum, k.lanes_log2) * over_m;
-            if (here) {
+            sum_lanes(mean, k.lanes_log2);
 #pragma unroll
-                for (int e = 0; e < W; ++e) {
-                    f[e] -= mean;
-                    squares = fmaf(f[e], f[e], squares);
+            for (int i = 0; i < ITEMS; ++i) {
+                mean[i] *= over_m;
+                square[i] = 0.0f;
+                if (!here[i]) continue;
+                float f[W];
+                dl_unpack(in[i], f);
+#pragma unroll
+                for (int e = 0; e < W; ++e) square[i] = fmaf(f[e] - mean[i], f[e] - mean[i], square[i]);
+            }
+            sum_lanes(square, k.lanes_log2);
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) {
+                if (!here[i]) continue;
+                const float rstd = rsqrtf(fmaf(square[i], over_m, p.eps));
+                if (at.first_lane && mean_out != nullptr) {
+                    const int64_t n = at.row0 + r0 + i * k.ty + at.ty;
+                    mean_out[n * p.G + at.group] = mean[i];
+                    rstd_out[n * p.G + at.group] = rstd;
                 }
-            }
-            const float rstd = rsqrtf(sum_lanes(squares, k.lanes_log2) * over_m + p.eps);
-            if (!here) continue;
-            if (j == 0 && mean_out != nullptr) {
-                mean_out[n * p.G + group] = mean;
-                rstd_out[n * p.G + group] = rstd;
-            }
+                float f[W];
+                dl_unpack(in[i], f);
 #pragma unroll
-            for (int e = 0; e < W; ++e) f[e] = activate<T, act.value>(fmaf(f[e] * rstd, w[e], b[e]));
-            DlVec<T, W> out;
-            dl_pack(f, out);
-            *reinterpret_cast<DlVec<T, W>*>(y + n * p.C + channel) = out;
+                for (int e = 0; e < W; ++e) f[e] = activate<T, act.value>(fmaf((f[e] - mean[i]) * rstd, w[e], b[e]));
+                DlVec<T, W> out;
+                dl_pack(f, out);
+                *reinterpret_cast<DlVec<T, W>*>(dst + i * step) = out;
+            }
         }
-    }
     });
 }
 
 template <typename T, int W, int ITEMS>
-__global__ void __launch_bounds__(ROW_THREADS, 3)
+__global__ void __launch_bounds__(ROW_THREADS, 4)
 norm_rows_bwd_kernel(const T* __restrict__ x, const T* __restrict__ gy, const float* __restrict__ mean_in,
                      const float* __restrict__ rstd_in, T* __restrict__ gx, float* __restrict__ partial,
                      const __grid_constant__ Norm p, const __grid_constant__ RowCut k) {
     __shared__ float red[ROW_THREADS * W];
-    const int tx = threadIdx.x % k.tx, slot = blockIdx.y * k.tx + tx, ty = threadIdx.x / k.tx;
-    const int group = slot >> k.lanes_log2, j = slot & ((1 << k.lanes_log2) - 1);
-    const bool live = group < p.G && j < k.lanes && ty < k.ty;
-    const int channel = group * p.per_group + j * W;
+    const RowPlace at(p, k, W);
+    const int64_t first = (at.row0 + at.ty) * p.C + at.channel, step = (int64_t)k.ty * p.C;
+    const T *src = x + first, *src_g = gy + first;
+    T* dst = gx + first;
+    const float *mean = mean_in + (at.row0 + at.ty) * p.G + at.group, *rstd = rstd_in + (at.row0 + at.ty) * p.G + at.group;
+    const int64_t group_step = (int64_t)k.ty * p.G;
     float w[W], b[W], sum_dz[W], sum_dzx[W];
-    bool first = true;
 #pragma unroll
     for (int e = 0; e < W; ++e) sum_dz[e] = sum_dzx[e] = 0.0f;
     const float over_m = 1.0f / (float)p.per_group;
     with_activation(p.act, [&](auto act) {
-    for (int64_t n0 = (int64_t)blockIdx.x * k.ty * ITEMS; n0 < p.N; n0 += (int64_t)gridDim.x * k.ty * ITEMS) {
-        DlVec<T, W> in[ITEMS], in_g[ITEMS];
-        float mean[ITEMS], rstd[ITEMS];
+        for (int r0 = 0; r0 < at.rows; r0 += k.ty * ITEMS) {
+            DlVec<T, W> in[ITEMS], in_g[ITEMS];
+            bool here[ITEMS];
+            float mu[ITEMS], rs[ITEMS], s1[ITEMS], s2[ITEMS], xh[ITEMS][W], dzw[ITEMS][W];
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i) {
-            const int64_t n = n0 + i * k.ty + ty;
-            if (live && n < p.N) {
-                in[i] = *reinterpret_cast<const DlVec<T, W>*>(x + n * p.C + channel);
-                in_g[i] = *reinterpret_cast<const DlVec<T, W>*>(gy + n * p.C + channel);
-                mean[i] = mean_in[n * p.G + group];
-                rstd[i] = rstd_in[n * p.G + group];
-            }
-        }
-        if (first && live) load_params<W>(p, channel, w, b);  // behind the first rows' loads
-        first = false;
-#pragma unroll
-        for (int i = 0; i < ITEMS; ++i) {
-            const int64_t n = n0 + i * k.ty + ty;
-            const bool here = live && n < p.N;
-            float xh[W], dzw[W], s1 = 0.0f, s2 = 0.0f;
-            if (here) {
-                const float off = -mean[i] * rstd[i];
-                dl_unpack(in[i], xh);
-                dl_unpack(in_g[i], dzw);
-#pragma unroll
-                for (int e = 0; e < W; ++e) {
-                    xh[e] = fmaf(xh[e], rstd[i], off);
-                    const float dz = dzw[e] * slope<T, act.value>(fmaf(xh[e], w[e], b[e]));
-                    sum_dz[e] += dz;
-                    sum_dzx[e] = fmaf(dz, xh[e], sum_dzx[e]);
-                    dzw[e] = dz * w[e];
-                    s1 += dzw[e];
-                    s2 = fmaf(dzw[e], xh[e], s2);
+            for (int i = 0; i < ITEMS; ++i) {
+                here[i] = at.live && r0 + i * k.ty + at.ty < at.rows;
+                if (here[i]) {
+                    in[i] = *reinterpret_cast<const DlVec<T, W>*>(src + i * step);
+                    in_g[i] = *reinterpret_cast<const DlVec<T, W>*>(src_g + i * step);
+                    mu[i] = mean[i * group_step];
+                    rs[i] = rstd[i * group_step];
                 }
             }
-            s1 = sum_lanes(s1, k.lanes_log2) * over_m;
-            s2 = sum_lanes(s2, k.lanes_log2) * over_m;
-            if (!here) continue;
+            if (r0 == 0 && at.live) load_params<W>(p, at.channel, w, b);  // behind the first rows' loads
 #pragma unroll
-            for (int e = 0; e < W; ++e) xh[e] = rstd[i] * (dzw[e] - fmaf(xh[e], s2, s1));
-            DlVec<T, W> out;
-            dl_pack(xh, out);
-            *reinterpret_cast<DlVec<T, W>*>(gx + n * p.C + channel) = out;
+            for (int i = 0; i < ITEMS; ++i) {
+                s1[i] = s2[i] = 0.0f;
+                if (!here[i]) continue;
+                const float off = -mu[i] * rs[i];
+                dl_unpack(in[i], xh[i]);
+                dl_unpack(in_g[i], dzw[i]);
+#pragma unroll
+                for (int e = 0; e < W; ++e) {
+                    xh[i][e] = fmaf(xh[i][e], rs[i], off);
+                    const float dz = dzw[i][e] * slope<T, act.value>(fmaf(xh[i][e], w[e], b[e]));
+                    sum_dz[e] += dz;
+                    sum_dzx[e] = fmaf(dz, xh[i][e], sum_dzx[e]);
+                    dzw[i][e] = dz * w[e];
+                    s1[i] += dzw[i][e];
+                    s2[i] = fmaf(dzw[i][e], xh[i][e], s2[i]);
+                }
+            }
+            sum_lanes(s1, k.lanes_log2);
+            sum_lanes(s2, k.lanes_log2);
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) {
+                if (!here[i]) continue;
+                const float a = s1[i] * over_m, c = s2[i] * over_m;
+#pragma unroll
+                for (int e = 0; e < W; ++e) xh[i][e] = rs[i] * (dzw[i][e] - fmaf(xh[i][e], c, a));
+                DlVec<T, W> out;
+                dl_pack(xh[i], out);
+                *reinterpret_cast<DlVec<T, W>*>(dst + i * step) = out;
+            }
+            src += ITEMS * step;
+            src_g += ITEMS * step;
+            dst += ITEMS * step;
+            mean += ITEMS * group_step;
+            rstd += ITEMS * group_step;
         }
-    }
     });
     if (partial == nullptr) return;
 #pragma unroll
     for (int v = 0; v < 2; ++v) {
         __syncthreads();
-        if (ty < k.ty) {
+        if (at.ty < k.ty) {
 #pragma unroll
-            for (int e = 0; e < W; ++e) red[(ty * k.tx + tx) * W + e] = v == 0 ? sum_dz[e] : sum_dzx[e];
+            for (int e = 0; e < W; ++e) red[(at.ty * k.tx + at.tx) * W + e] = v == 0 ? sum_dz[e] : sum_dzx[e];
         }
         __syncthreads();
-        if (live && ty == 0) {
+        if (at.live && at.ty == 0) {
 #pragma unroll
             for (int e = 0; e < W; ++e) {
                 float sum = 0.0f;
-                for (int r = 0; r < k.ty; ++r) sum += red[(r * k.tx + tx) * W + e];
-                partial[((int64_t)blockIdx.x * 2 + v) * p.C + channel + e] = sum;
+                for (int r = 0; r < k.ty; ++r) sum += red[(r * k.tx + at.tx) * W + e];
+                partial[((int64_t)blockIdx.x * 2 + v) * p.C + at.channel + e] = sum;
             }
         }
     }
 }
 
-// gbias / gweight[c] = sum over parts of partial[part][0 / 1][c]; 32 channels x 32 threads down the parts per block
-__global__ void __launch_bounds__(1024)
+// gbias / gweight[c] = sum over parts of partial[part][0 / 1][c]; 8 channels (a sector) x 128 threads down the parts
+constexpr int PARAM_CHANNELS = 8, PARAM_ROWS = 128;
+
+__global__ void __launch_bounds__(PARAM_CHANNELS * PARAM_ROWS)
 norm_params_kernel(const float* __restrict__ partial, int64_t parts, int C, void* gweight, void* gbias, int param_dtype) {
-    __shared__ float red[2][32][33];
-    const int c = blockIdx.x * 32 + (threadIdx.x & 31), y = threadIdx.x >> 5;
+    __shared__ float red[2][PARAM_ROWS / 4][PARAM_CHANNELS];
+    const int x = threadIdx.x % PARAM_CHANNELS, y = threadIdx.x / PARAM_CHANNELS, c = blockIdx.x * PARAM_CHANNELS + x;
     float sum[2] = {0.0f, 0.0f};
     if (c < C) {
 #pragma unroll 4
-        for (int64_t i = y; i < parts; i += 32) {
+        for (int64_t i = y; i < parts; i += PARAM_ROWS) {
             sum[0] += partial[(i * 2) * C + c];
             sum[1] += partial[(i * 2 + 1) * C + c];
         }
     }
 #pragma unroll
-    for (int v = 0; v < 2; ++v) red[v][y][threadIdx.x & 31] = sum[v];
+    for (int v = 0; v < 2; ++v) {
+        sum[v] += __shfl_xor_sync(0xffffffffu, sum[v], 8);
+        sum[v] += __shfl_xor_sync(0xffffffffu, sum[v], 16);
+        if (y % 4 == 0) red[v][y / 4][x] = sum[v];  // a warp holds four rows
+    }
     __syncthreads();
-    if (y < 2) {  // warp 0: bias, warp 1: weight
+    if (threadIdx.x < 2 * PARAM_CHANNELS) {
+        const int v = threadIdx.x / PARAM_CHANNELS;
         float total = 0.0f;
-        for (int r = 0; r < 32; ++r) total += red[y][r][threadIdx.x & 31];
-        void* out = y == 0 ? gbias : gweight;
+#pragma unroll
+        for (int r = 0; r < PARAM_ROWS / 4; ++r) total += red[v][r][x];
+        void* out = v == 0 ? gbias : gweight;
         if (c < C && out != nullptr) dl_store_from_float(out, param_dtype, c, total);
     }
 }
@@ -647,6 +694,7 @@ int64_t sums_floats(const Norm& p, const Cut& k) {
 }
 bool grid_fits(const Norm& p, const Cut& k) { return p.N * k.blocks_c * (int64_t)k.chunks <= 0x7fffffff; }
 
+// W as the kernel takes it, at most ROW_WIDTH
 bool cut_rows(const Norm& p, int W, int items, int64_t most_blocks, RowCut& k) {
     if (p.S != 1 || p.per_group / W > 32) return false;
     k.lanes = p.per_group / W;
@@ -658,20 +706,26 @@ bool cut_rows(const Norm& p, int W, int items, int64_t most_blocks, RowCut& k) {
     const int64_t across = dl_ceil_div(slots, k.tx);
     if (across > 65535) return false;
     k.blocks_c = (int)across;
-    k.blocks_x = dl_min64(dl_ceil_div(p.N, (int64_t)k.ty * items), dl_max64(most_blocks / across, 1));
+    // one round of resident blocks, each with as many rows as the others
+    const int64_t rows =
+        dl_ceil_div(p.N, dl_min64(dl_ceil_div(p.N, (int64_t)k.ty * items), dl_max64(most_blocks / across, 1)));
+    if (rows > 0x3fffffff) return false;
+    k.rows = (int)rows;
+    k.blocks_x = dl_ceil_div(p.N, rows);
     return true;
 }
 
-constexpr int ROW_ITEMS = 2, ROW_ITEMS_BWD = 1;
-constexpr int64_t ROW_BLOCKS = DL_NUM_SMS * 16, ROW_BLOCKS_BWD = DL_NUM_SMS * 3;
+constexpr int row_width(int W) { return W < ROW_WIDTH ? W : ROW_WIDTH; }
+constexpr int ROW_ITEMS = 4, ROW_ITEMS_BWD = 2;   // rows a thread loads before it uses the first
+constexpr int64_t ROW_BLOCKS = DL_NUM_SMS * 4;    // resident: the kernels' launch bounds
 
 template <typename T, int W>
 int launch_forward(const void* x, void* y, float* mean, float* rstd, float* sums, const Norm& p, cudaStream_t s) {
     const T* src = static_cast<const T*>(x);
     T* dst = static_cast<T*>(y);
     RowCut r;
-    if (cut_rows(p, W, ROW_ITEMS, ROW_BLOCKS, r)) {
-        norm_rows_kernel<T, W, ROW_ITEMS><<<dim3((unsigned)r.blocks_x, (unsigned)r.blocks_c), ROW_THREADS, 0, s>>>(
+    if (cut_rows(p, row_width(W), ROW_ITEMS, ROW_BLOCKS, r)) {
+        norm_rows_kernel<T, row_width(W), ROW_ITEMS><<<dim3((unsigned)r.blocks_x, (unsigned)r.blocks_c), ROW_THREADS, 0, s>>>(
             src, dst, mean, rstd, p, r);
         return dl_launch_status();
     }
@@ -691,12 +745,12 @@ int launch_forward(const void* x, void* y, float* mean, float* rstd, float* sums
 // floats of workspace: sums of the chunks, then the partial sums of the parameters' gradients
 int64_t forward_floats(const Norm& p, int W) {
     RowCut r;
-    if (cut_rows(p, W, ROW_ITEMS, ROW_BLOCKS, r)) return 0;
+    if (cut_rows(p, row_width(W), ROW_ITEMS, ROW_BLOCKS, r)) return 0;
     return sums_floats(p, cut_chunks(p, W, RESIDENT));
 }
 int64_t backward_floats(const Norm& p, int W, int64_t& parts) {
     RowCut r;
-    if (cut_rows(p, W, ROW_ITEMS_BWD, ROW_BLOCKS_BWD, r)) {
+    if (cut_rows(p, row_width(W), ROW_ITEMS_BWD, ROW_BLOCKS, r)) {
         parts = r.blocks_x;
         return 0;
     }
@@ -714,8 +768,8 @@ int launch_backward(const void* x, const void* g, const float* mean, const float
     float* partial = scratch + backward_floats(p, W, parts);
     if (gweight == nullptr && gbias == nullptr) partial = nullptr;
     RowCut r;
-    if (cut_rows(p, W, ROW_ITEMS_BWD, ROW_BLOCKS_BWD, r)) {
-        norm_rows_bwd_kernel<T, W, ROW_ITEMS_BWD>
+    if (cut_rows(p, row_width(W), ROW_ITEMS_BWD, ROW_BLOCKS, r)) {
+        norm_rows_bwd_kernel<T, row_width(W), ROW_ITEMS_BWD>
             <<<dim3((unsigned)r.blocks_x, (unsigned)r.blocks_c), ROW_THREADS, 0, s>>>(src, src_g, mean, rstd, dst, partial,
                                                                                      p, r);
     } else {
@@ -735,7 +789,7 @@ int launch_backward(const void* x, const void* g, const float* mean, const float
     }
     if (cudaPeekAtLastError() != cudaSuccess) return DL_ERR_LAUNCH;
     if (partial != nullptr)
-        norm_params_kernel<<<(unsigned)dl_ceil_div(p.C, 32), 1024, 0, s>>>(partial, parts, p.C, gweight, gbias, p.param_dtype);
+        norm_params_kernel<<<(unsigned)dl_ceil_div(p.C, PARAM_CHANNELS), PARAM_CHANNELS * PARAM_ROWS, 0, s>>>(partial, parts, p.C, gweight, gbias, p.param_dtype);
     return dl_launch_status();
 }
 
