@@ -6,12 +6,16 @@
 //
 // Both cuts are one question: down to which (logit, index) does a running sum, of ones or of weights, stay below a
 // target?  It is answered without sorting: a histogram over (max - l) / T in 2048 steps of 1/32 finds the step in which
-// the target falls, and the few logits of that step are ranked among themselves by counting (or, when very many share the
-// step, by histograms over the bits of their keys and, for equal ones, over their index).
+// the target falls.  Usually at most a thousand logits lie in that step and above it (min-p only lowers their number):
+// they are collected and sorted in shared memory, where cuts and draw are prefix sums.  Otherwise the logits of that one
+// step are sorted (or, when very many share it, told apart by histograms over the bits of their keys and, for equal ones,
+// over their index), and the draw goes over the row once more.
 //
 // A class next to a border must not depend on the order of additions, so weights are whole numbers: exp in double
 // precision, as fixed point with up to 50 fractional bits, chosen so that the sum of a row fits 62 bits.  Integer sums are
-// exact in any order, so shared-memory atomics are harmless here.
+// exact in any order, so shared-memory atomics are harmless here.  The atomics of the weights are what a pass would spend
+// its time on; V classes that weigh less than (1 - p) / V of the largest each cannot hold the border of top-p, and go to a
+// register instead.
 //
 // Rows of up to 512 classes take one warp and registers; longer ones a block of 512 threads, or a cluster of up to
 // eight when there are few rows.  Each pass reads the logits again: after the first they come from L2.
@@ -28,7 +32,7 @@ typedef unsigned long long u64;
 constexpr int THREADS = 512;
 constexpr int WARPS = THREADS / 32;
 constexpr int BINS = 2048;
-constexpr int LIST = 512;  // most logits ranked by counting
+constexpr int LIST = 1024;  // most logits that are collected and sorted
 constexpr int MAX_CLUSTER = 8;
 constexpr int SMALL_V = 512;
 constexpr int TABLE = 128;
@@ -85,34 +89,36 @@ __device__ __forceinline__ float logit_of(uint32_t key) {
 
 // exp(-(top - l) / T) as fixed point.  With j = round(128 z / ln 2) and r = z - j ln 2 / 128, |r| < 0.0028,
 // e^-z = 2^(-j / 128) e^-r: a table for the fraction of the power, four terms of the series for e^-r (the fifth is below
-// 2^-49), the whole part of the power as an exponent.
+// 2^-49), the whole part of the power as an exponent.  Without branches: the steps of several logits then overlap.
 struct Weigher {
     const double* table;  // 2^(shift - i / 128)
     double top, inverse_T, most_z;
-    bool infinite;        // the largest logit is +inf
+    bool infinite;        // the largest logit is +inf: only such logits weigh something
     u64 one;
     __device__ __forceinline__ Weigher(const double* table, uint32_t top_key, double inverse_T, int shift)
         : table(table), inverse_T(inverse_T) {
         const float t = logit_of(top_key);
         infinite = t == INFINITY;
         top = infinite ? 0.0 : (double)t;
-        most_z = 0.6931471805599453 * (shift + 2);  // less than a quarter of the last bit from here on
+        most_z = 0.6931471805599453 * (shift + 2);  // a quarter of the last bit: rounds to 0
         one = 1ull << shift;
     }
-    __device__ __forceinline__ u64 operator()(uint32_t key) const {
-        const float l = logit_of(key);
-        if (infinite) return l == INFINITY ? one : 0ull;
-        const double z = (top - (double)l) * inverse_T;
-        if (!(z < most_z)) return 0ull;
+    // 0 for NaN and -inf
+    __device__ __forceinline__ u64 of(float l) const {
+        double z = (top - (double)l) * inverse_T;
+        z = z < most_z ? z : most_z;
         const double magic = 6755399441055744.0;  // 1.5 * 2^52: the sum's low word is the rounded integer
         const double shifted = fma(z, 184.6649652337873, magic);
         const int j = __double2loint(shifted);
         const double r = fma(shifted - magic, -0.0054152123481245725, z);
-        const double e = fma(fma(fma(fma(r, 1.0 / 24, -1.0 / 6), r, 0.5), r, -1.0), r, 1.0);
+        // the series in two halves, so that the steps wait less for one another
+        const double rr = r * r, e = fma(fma(fma(r, 1.0 / 24, -1.0 / 6), r, 0.5), rr, 1.0 - r);
         double w = table[j & (TABLE - 1)] * e;
         w = __hiloint2double(__double2hiint(w) - ((j >> 7) << 20), __double2loint(w));
-        return (u64)__double_as_longlong(w + 4503599627370496.0) - 0x4330000000000000ull;  // w < 2^52, rounded
+        const u64 fixed = (u64)__double_as_longlong(w + 4503599627370496.0) - 0x4330000000000000ull;  // w < 2^52, rounded
+        return infinite ? (l == INFINITY ? one : 0ull) : fixed;
     }
+    __device__ __forceinline__ u64 operator()(uint32_t key) const { return of(logit_of(key)); }
 };
 
 __device__ __forceinline__ void fill_table(double* table, int shift, int tid, int threads) {
@@ -197,7 +203,9 @@ sample_small_kernel(const T* __restrict__ logits, const __grid_constant__ Job jo
                 int n = 0;
 #pragma unroll
                 for (int j = 0; j < PER; ++j) n += key[j] >= at;
-                if (__reduce_add_sync(FULL, n) >= rule.top_k) t = at;
+                n = __reduce_add_sync(FULL, n);
+                if (n >= rule.top_k) t = at;
+                if (n == rule.top_k) break;  // exactly these
             }
             int above = 0;
 #pragma unroll
@@ -279,16 +287,18 @@ sample_small_kernel(const T* __restrict__ logits, const __grid_constant__ Job jo
 }
 
 // ------------------------------------------------------------------------------------------ a block or cluster per row
-struct Shared {
+struct __align__(16) Shared {
     double table[TABLE];
     uint32_t low[BINS], high[BINS];  // the two words of every step's sum
-    u64 list_weight[LIST], all_weight[LIST];
-    uint32_t list_key[LIST], list_index[LIST], all_key[LIST], all_index[LIST];
+    uint32_t count[BINS];
+    u64 list[LIST];    // collected by this block: key, then the index inverted
+    u64 sorted[LIST];  // of the whole row, in the first block
     u64 warp_value[WARPS];
+    uint32_t warp_counted[WARPS];
+    u64 tail;
     u64 found[4];
     u64 published[2][4];  // for the other blocks, two turns
     uint32_t list_count;
-    u64 result;
 };
 
 // down to where a running sum stays below its target: keys above, and equal keys up to an index
@@ -305,22 +315,57 @@ struct Row {
     Shared& sh;
     cg::cluster_group cluster;
     int rank, ranks, tid, lane, warp, turn;
+    bool vectors;
 
     __device__ __forceinline__ void barrier() {
         if (ranks > 1) cluster.sync();
         else __syncthreads();
     }
+    // f(index, stride, four logits) over the slice, element e at index + e * stride; NaN where there is none.  By vectors
+    // when every row starts on 16 bytes (slices do then).
     template <typename F>
-    __device__ __forceinline__ void each(F f) const {  // f(index, key) over the slice, four loads in flight
-        uint32_t i = from + tid;
-        for (; i + 3 * THREADS < to; i += 4 * THREADS) {
+    __device__ __forceinline__ void each4(F f) const {
+        constexpr int N = 16 / sizeof(T), AHEAD = 16 / N;
+        uint32_t i = from;
+        if (vectors) {
+            constexpr uint32_t STEP = THREADS * N;
+            const uint32_t whole = from + (to - from) / STEP * STEP;
+            for (i = from + tid * N; i < whole; i += AHEAD * STEP) {
+                DlVec<T, N> v[AHEAD];
+#pragma unroll
+                for (int k = 0; k < AHEAD; ++k)
+                    if (i + k * STEP < whole) v[k] = *reinterpret_cast<const DlVec<T, N>*>(logits + i + k * STEP);
+#pragma unroll
+                for (int k = 0; k < AHEAD; ++k) {
+                    if (i + k * STEP >= whole) break;
+                    float l[N];
+                    dl_unpack(v[k], l);
+#pragma unroll
+                    for (int q = 0; q < N; q += 4) {
+                        const float four[4] = {l[q], l[q + 1], l[q + 2], l[q + 3]};
+                        f(i + k * STEP + q, 1u, four);
+                    }
+                }
+            }
+            i = whole;
+        }
+        for (i += tid; i < to; i += 4 * THREADS) {
             float l[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) l[k] = dl_to_float(logits[i + k * THREADS]);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) f(i + k * THREADS, key_of(l[k]));
+            for (int k = 0; k < 4; ++k) l[k] = i + k * THREADS < to ? dl_to_float(logits[i + k * THREADS]) : NAN;
+            f(i, (uint32_t)THREADS, l);
         }
-        for (; i < to; i += THREADS) f(i, key_of(dl_to_float(logits[i])));
+    }
+    template <typename F>
+    __device__ __forceinline__ void each(F f) const {
+        each4([&](uint32_t i, uint32_t stride, const float (&l)[4]) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) f(i + e * stride, l[e]);
+        });
+    }
+    template <typename F>
+    __device__ __forceinline__ void each_key(F f) const {
+        each([&](uint32_t i, float l) { f(i, key_of(l)); });
     }
     // over the whole row: `combine` of every thread's value
     template <typename F>
@@ -330,8 +375,9 @@ struct Row {
         __syncthreads();
         if (lane == 0) sh.warp_value[warp] = v;
         __syncthreads();
-        v = sh.warp_value[0];
-        for (int k = 1; k < WARPS; ++k) v = combine(v, sh.warp_value[k]);
+        v = sh.warp_value[lane % WARPS];
+#pragma unroll
+        for (int s = WARPS / 2; s > 0; s >>= 1) v = combine(v, __shfl_xor_sync(FULL, v, s));
         if (ranks == 1) return v;
         if (tid == 0) sh.published[turn][0] = v;
         cluster.sync();
@@ -340,130 +386,247 @@ struct Row {
         turn ^= 1;
         return v;
     }
-    // clears the histogram, adds value(i, key) at step(i, key) wherever that is not negative, and finds the step at which
-    // the row's sum reaches target(total).  False: it never does.
-    template <typename S, typename G>
-    __device__ __forceinline__ bool crossing(S step, G target, int& at, u64& before, u64& total, u64& goal) {
+    void __device__ __forceinline__ clear_histogram() {
         __syncthreads();
-        for (int b = tid; b < BINS; b += THREADS) sh.low[b] = sh.high[b] = 0;
-        if (tid == 0) sh.found[0] = BINS;
+        for (int b = tid; b < BINS; b += THREADS) sh.low[b] = sh.high[b] = sh.count[b] = 0;
+        if (tid == 0) {
+            sh.found[0] = BINS;
+            sh.tail = 0;
+        }
         __syncthreads();
-        each([&](uint32_t i, uint32_t key) {
-            u64 value;
-            const int b = step(i, key, value);
-            if (b < 0) return;
-            const uint32_t lo = (uint32_t)value, old = atomicAdd(&sh.low[b], lo);
-            const uint32_t hi = (uint32_t)(value >> 32) + (old + lo < old ? 1u : 0u);
-            if (hi) atomicAdd(&sh.high[b], hi);
-        });
+    }
+    __device__ __forceinline__ void add_weight(int b, u64 value) {
+        const uint32_t lo = (uint32_t)value, old = atomicAdd(&sh.low[b], lo);
+        const uint32_t hi = (uint32_t)(value >> 32) + (old + lo < old ? 1u : 0u);
+        if (hi) atomicAdd(&sh.high[b], hi);
+    }
+    // The step at which the row's sum over the histogram reaches target(total); total includes the tails.  False: it never
+    // does.  upto: how many logits were counted up to and including that step.
+    template <typename G>
+    __device__ __forceinline__ bool find_step(G target, int& at, u64& before, u64& total, u64& goal, uint32_t& upto) {
         barrier();
         constexpr int PER = BINS / THREADS;
         u64 v[PER], sum = 0;
+        uint32_t n[PER], counted = 0;
+        total = 0;
+        if (ranks > 1)
+            for (int r = 0; r < ranks; ++r) total += *cluster.map_shared_rank(&sh.tail, r);
+        else
+            total = sh.tail;
 #pragma unroll
         for (int k = 0; k < PER; ++k) {
             v[k] = 0;
-            for (int r = 0; r < ranks; ++r) {
-                const uint32_t* low = ranks > 1 ? cluster.map_shared_rank(sh.low, r) : sh.low;
-                const uint32_t* high = ranks > 1 ? cluster.map_shared_rank(sh.high, r) : sh.high;
-                v[k] += (u64)low[tid * PER + k] | (u64)high[tid * PER + k] << 32;
-            }
+            n[k] = 0;
+        }
+        for (int r = 0; r < ranks; ++r) {
+            const Shared* other = ranks > 1 ? cluster.map_shared_rank(&sh, r) : &sh;
+            static_assert(PER == 4, "one access per array");
+            const uint4 lo = *reinterpret_cast<const uint4*>(&other->low[tid * PER]);
+            const uint4 hi = *reinterpret_cast<const uint4*>(&other->high[tid * PER]);
+            const uint4 c = *reinterpret_cast<const uint4*>(&other->count[tid * PER]);
+            v[0] += (u64)lo.x | (u64)hi.x << 32;
+            v[1] += (u64)lo.y | (u64)hi.y << 32;
+            v[2] += (u64)lo.z | (u64)hi.z << 32;
+            v[3] += (u64)lo.w | (u64)hi.w << 32;
+            n[0] += c.x;
+            n[1] += c.y;
+            n[2] += c.z;
+            n[3] += c.w;
+        }
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
             sum += v[k];
+            counted += n[k];
         }
         const u64 inclusive = warp_inclusive(sum, lane);
-        if (lane == 31) sh.warp_value[warp] = inclusive;
+        uint32_t counted_inclusive = counted;
+#pragma unroll
+        for (int s = 1; s < 32; s <<= 1) {
+            const uint32_t o = __shfl_up_sync(FULL, counted_inclusive, s);
+            if (lane >= s) counted_inclusive += o;
+        }
+        if (lane == 31) {
+            sh.warp_value[warp] = inclusive;
+            sh.warp_counted[warp] = counted_inclusive;
+        }
         __syncthreads();
         u64 run = inclusive - sum;
-        total = 0;
+        uint32_t run_counted = counted_inclusive - counted;
+#pragma unroll
         for (int k = 0; k < WARPS; ++k) {
-            if (k < warp) run += sh.warp_value[k];
-            total += sh.warp_value[k];
+            const u64 w = sh.warp_value[k];
+            if (k < warp) {
+                run += w;
+                run_counted += sh.warp_counted[k];
+            }
+            total += w;
         }
         goal = target(total);
 #pragma unroll
         for (int k = 0; k < PER; ++k) {
+            run_counted += n[k];
             if (run < goal && run + v[k] >= goal) {
                 sh.found[0] = tid * PER + k;
                 sh.found[1] = run;
+                sh.found[2] = run_counted;
             }
             run += v[k];
         }
         barrier();  // also: nobody clears a histogram that others still read
         at = (int)sh.found[0];
         before = sh.found[1];
+        upto = (uint32_t)sh.found[2];
         return at < BINS;
     }
-    // The cut at which the sum of value over the members stays below the target, members in descending order.
-    // weight(key) is a member's value, goal_of the target from the members' total.
-    template <typename M, typename W, typename S, typename G>
-    __device__ __forceinline__ bool cut(M member, W weight, S coarse, G goal_of, Cut& out) {
-        int at;
-        u64 before, total, goal;
-        const bool crosses = crossing(
-            [&](uint32_t i, uint32_t key, u64& value) {
-                if (!member(i, key)) return -1;
-                value = weight(key);
-                return coarse(key);
-            },
-            goal_of, at, before, total, goal);
-        if (!crosses) return false;
-        // the members of that step
+    // adds value(i, key) at step(i, key) wherever that is not negative, and finds the step of target(total)
+    template <typename S, typename G>
+    __device__ __forceinline__ bool crossing(S step, G target, int& at, u64& before, u64& total, u64& goal) {
+        clear_histogram();
+        each_key([&](uint32_t i, uint32_t key) {
+            u64 value;
+            const int b = step(i, key, value);
+            if (b >= 0) add_weight(b, value);
+        });
+        uint32_t unused;
+        return find_step(target, at, before, total, goal, unused);
+    }
+    // Collects the logits that wanted(index, logit) accepts.  Returns how many the row has; up to LIST of them are then
+    // `sorted` in the cluster's first block, largest first, equal ones by index.
+    template <typename F>
+    __device__ __forceinline__ uint32_t collect(F wanted) {
+        __syncthreads();
         if (tid == 0) sh.list_count = 0;
         __syncthreads();
-        each([&](uint32_t i, uint32_t key) {
-            if (!member(i, key) || coarse(key) != at) return;
-            const uint32_t n = atomicAdd(&sh.list_count, 1u);
-            if (n < LIST) {
-                sh.list_key[n] = key;
-                sh.list_index[n] = i;
-                sh.list_weight[n] = weight(key);
+        each4([&](uint32_t i, uint32_t stride, const float (&l)[4]) {
+            bool want[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) want[e] = wanted(i + e * stride, l[e]);
+            if (!(want[0] | want[1] | want[2] | want[3])) return;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (!want[e]) continue;
+                const uint32_t n = atomicAdd(&sh.list_count, 1u);
+                if (n < LIST) sh.list[n] = (u64)key_of(l[e]) << 32 | (uint32_t)~(i + e * stride);
             }
         });
         barrier();
-        uint32_t n = 0, here = 0;
-        for (int r = 0; r < ranks; ++r) {
-            const uint32_t c = ranks > 1 ? *cluster.map_shared_rank(&sh.list_count, r) : sh.list_count;
-            n += c;
-        }
-        if (n <= LIST) {
+        uint32_t n = 0;
+        for (int r = 0; r < ranks; ++r) n += ranks > 1 ? *cluster.map_shared_rank(&sh.list_count, r) : sh.list_count;
+        if (rank == 0 && n <= LIST) {
             uint32_t start = 0;
             for (int r = 0; r < ranks; ++r) {
                 const Shared* other = ranks > 1 ? cluster.map_shared_rank(&sh, r) : &sh;
-                here = other->list_count;
-                if (tid < (int)here) {
-                    sh.all_key[start + tid] = other->list_key[tid];
-                    sh.all_index[start + tid] = other->list_index[tid];
-                    sh.all_weight[start + tid] = other->list_weight[tid];
-                }
+                const uint32_t here = other->list_count;
+                for (uint32_t i = tid; i < here; i += THREADS) sh.sorted[start + i] = other->list[i];
                 start += here;
             }
-            barrier();
-            u64 worst = ~0ull;
-            if (tid < (int)n) {
-                const uint32_t key = sh.all_key[tid], index = sh.all_index[tid];
-                u64 ahead = before;
-                for (uint32_t k = 0; k < n; ++k) {
-                    const uint32_t other = sh.all_key[k];
-                    if (other > key || (other == key && sh.all_index[k] < index)) ahead += sh.all_weight[k];
+            sort(n);
+        }
+        barrier();  // the lists are free again
+        return n;
+    }
+    // sorts `sorted` descending by a bitonic network; entries from n up to the next power of two become 0
+    __device__ __noinline__ void sort(uint32_t n) {
+        uint32_t size = 2;
+        while (size < n) size *= 2;
+        __syncthreads();
+        for (uint32_t i = n + tid; i < size; i += THREADS) sh.sorted[i] = 0;
+        for (uint32_t run = 2; run <= size; run *= 2) {
+            for (uint32_t s = run / 2; s > 0; s /= 2) {
+                __syncthreads();
+                for (uint32_t q = tid; q < size / 2; q += THREADS) {
+                    const uint32_t i = 2 * q - (q & (s - 1)), j = i + s;  // q with a 0 put in at bit s
+                    const u64 a = sh.sorted[i], b = sh.sorted[j];
+                    if ((a < b) == ((i & run) == 0)) {
+                        sh.sorted[i] = b;
+                        sh.sorted[j] = a;
+                    }
                 }
-                if (ahead < goal) worst = (u64)key << 32 | (uint32_t)~index;
             }
-            __syncthreads();
+        }
+        __syncthreads();
+    }
+    // Running sums of two values per thread in list order: a, b become the sums up to and including them.  Returns the
+    // total.
+    __device__ __noinline__ u64 scan_pairs(u64& a, u64& b) {
+        const u64 sum = a + b, inclusive = warp_inclusive(sum, lane);
+        __syncthreads();
+        if (lane == 31) sh.warp_value[warp] = inclusive;
+        __syncthreads();
+        u64 run = inclusive - sum, total = 0;
 #pragma unroll
-            for (int s = 16; s > 0; s >>= 1) {
-                const u64 o = __shfl_xor_sync(FULL, worst, s);
-                worst = o < worst ? o : worst;
+        for (int k = 0; k < WARPS; ++k) {
+            const u64 v = sh.warp_value[k];
+            if (k < warp) run += v;
+            total += v;
+        }
+        a += run;
+        b = run + sum;
+        return total;
+    }
+    // Cuts and draw among the n sorted logits, by the first block.  What is kept is a prefix of them.  k: 0, or how many
+    // top-k keeps; total: the weight of all that top-k keeps when k is 0 (the n logits are the row's largest then, down to
+    // where top-p or min-p ends).
+    template <typename W>
+    __device__ __noinline__ int64_t finish(uint32_t n, uint32_t k, u64 total, const Rule& rule, const W& weigh) {
+        static_assert(LIST == 2 * THREADS, "two entries per thread");
+        const uint32_t i = 2 * tid;
+        if (k > 0 && k < n) n = k;
+        const u64 e0 = i < n ? sh.sorted[i] : 0ull, e1 = i + 1 < n ? sh.sorted[i + 1] : 0ull;
+        const u64 w0 = i < n ? weigh((uint32_t)(e0 >> 32)) : 0ull, w1 = i + 1 < n ? weigh((uint32_t)(e1 >> 32)) : 0ull;
+        u64 upto0 = w0, upto1 = w1;
+        const u64 all = scan_pairs(upto0, upto1);
+        const u64 goal = rule.top_p < 1.0 ? share_of(rule.top_p, k > 0 ? all : total) : ~0ull;
+        const bool keep0 = i < n && upto0 - w0 < goal && w0 >= rule.least;
+        const bool keep1 = i + 1 < n && upto1 - w1 < goal && w1 >= rule.least;
+        // by index now: the largest inverted index first
+        const auto by_index = [](u64 e) { return e << 32 | e >> 32; };
+        const uint32_t kept = __syncthreads_count(keep0) + __syncthreads_count(keep1);
+        if (keep0) sh.sorted[i] = by_index(e0);
+        if (keep1) sh.sorted[i + 1] = by_index(e1);
+        if (kept > 1) sort(kept);
+        else __syncthreads();
+        const u64 a = i < kept ? sh.sorted[i] : 0ull, b = i + 1 < kept ? sh.sorted[i + 1] : 0ull;
+        upto0 = i < kept ? weigh((uint32_t)a) : 0ull;
+        upto1 = i + 1 < kept ? weigh((uint32_t)b) : 0ull;
+        const u64 a_weight = upto0, b_weight = upto1;
+        const u64 sum = scan_pairs(upto0, upto1), point = point_of(rule.u, sum);
+        // one entry's weight spans the point
+        if (a_weight > 0 && upto0 > point && upto0 - a_weight <= point) sh.found[3] = (uint32_t)~(uint32_t)(a >> 32);
+        if (b_weight > 0 && upto1 > point && upto1 - b_weight <= point) sh.found[3] = (uint32_t)~(uint32_t)(b >> 32);
+        __syncthreads();
+        return (int64_t)sh.found[3];
+    }
+    // The cut in step `at`, before which the members weigh `before`, at which the sum of weight(key) over the members, in
+    // descending order, stays below `goal`.
+    template <typename M, typename W, typename S>
+    __device__ __noinline__ Cut cut_in(int at, u64 before, u64 goal, M member, W weight, S coarse) {
+        Cut out;
+        const uint32_t n = collect([&](uint32_t i, float l) {
+            const uint32_t key = key_of(l);
+            return member(i, key) && coarse(key) == at;
+        });
+        if (n <= LIST) {
+            if (rank == 0) {
+                const uint32_t i = 2 * tid;
+                const u64 w0 = i < n ? weight((uint32_t)(sh.sorted[i] >> 32)) : 0ull;
+                const u64 w1 = i + 1 < n ? weight((uint32_t)(sh.sorted[i + 1] >> 32)) : 0ull;
+                u64 upto0 = w0, upto1 = w1;
+                scan_pairs(upto0, upto1);
+                const uint32_t kept = __syncthreads_count(i < n && before + upto0 - w0 < goal) +
+                                      __syncthreads_count(i + 1 < n && before + upto1 - w1 < goal);
+                if (tid == 0) sh.found[3] = sh.sorted[kept - 1];  // the step holds the border: at least one is kept
             }
-            if (lane == 0) sh.warp_value[warp] = worst;
-            __syncthreads();
-            worst = sh.warp_value[0];
-            for (int k = 1; k < WARPS; ++k) worst = sh.warp_value[k] < worst ? sh.warp_value[k] : worst;
-            out.key = (uint32_t)(worst >> 32);
-            out.last = ~(uint32_t)worst;
-            return true;
+            barrier();
+            const u64 last = ranks > 1 ? *cluster.map_shared_rank(&sh.found[3], 0) : sh.found[3];
+            out.key = (uint32_t)(last >> 32);
+            out.last = ~(uint32_t)last;
+            barrier();
+            return out;
         }
         // very many in one step: narrow their keys down to one
         u64 least = ~0ull, most = 0;
-        each([&](uint32_t i, uint32_t key) {
+        each_key([&](uint32_t i, uint32_t key) {
             if (!member(i, key) || coarse(key) != at) return;
             least = key < least ? key : least;
             most = key > most ? key : most;
@@ -497,7 +660,7 @@ struct Row {
         uint32_t ilo = 0, ihi = 0xffffffffu;
         {
             u64 first = ~0ull, last = 0;
-            each([&](uint32_t i, uint32_t key) {
+            each_key([&](uint32_t i, uint32_t key) {
                 if (key != klo || !member(i, key)) return;
                 first = i < first ? i : first;
                 last = i > last ? i : last;
@@ -524,44 +687,140 @@ struct Row {
         }
         out.key = klo;
         out.last = ilo;
+        return out;
+    }
+    // the same with the step still to be found; goal_of: the target from the members' total.  False: no cut.
+    template <typename M, typename W, typename S, typename G>
+    __device__ __forceinline__ bool cut(M member, W weight, S coarse, G goal_of, Cut& out) {
+        int at;
+        u64 before, total, goal;
+        if (!crossing(
+                [&](uint32_t i, uint32_t key, u64& value) {
+                    if (!member(i, key)) return -1;
+                    value = weight(key);
+                    return coarse(key);
+                },
+                goal_of, at, before, total, goal))
+            return false;
+        out = cut_in(at, before, goal, member, weight, coarse);
         return true;
     }
 };
 
 template <typename T>
-__global__ void __launch_bounds__(THREADS)
-sample_kernel(const T* __restrict__ logits, const __grid_constant__ Job job, int ranks) {
+__global__ void __launch_bounds__(THREADS, 2)
+sample_kernel(const T* __restrict__ logits, const __grid_constant__ Job job, int ranks, uint32_t slice, int vectors) {
     extern __shared__ __align__(16) unsigned char dynamic_shared[];
     Shared& sh = *reinterpret_cast<Shared*>(dynamic_shared);
     const int64_t row = blockIdx.x / ranks;
     const int rank = (int)(blockIdx.x % ranks), tid = threadIdx.x;
-    const uint32_t V = (uint32_t)job.V, slice = (V + ranks - 1) / ranks;
+    const uint32_t V = (uint32_t)job.V;
     const uint32_t from = rank * slice < V ? rank * slice : V, to = from + slice < V ? from + slice : V;
-    Row<T> r{logits + row * job.pitch, from, to, sh, cg::this_cluster(), rank, ranks, tid, tid & 31, tid >> 5, 0};
+    Row<T> r{logits + row * job.pitch, from, to, sh, cg::this_cluster(), rank, ranks, tid, tid & 31, tid >> 5, 0,
+             vectors != 0};
     const Rule rule(job, row);
     fill_table(sh.table, job.shift, tid, THREADS);
 
-    // the largest key, and the lowest index that has it
-    u64 best = 0;
-    r.each([&](uint32_t i, uint32_t key) {
-        const u64 c = (u64)key << 32 | (uint32_t)~i;
-        best = key != 0u && c > best ? c : best;
-    });
-    best = r.reduce(best, [](u64 a, u64 b) { return a > b ? a : b; });
-    const uint32_t most = (uint32_t)(best >> 32);
-    if (most == 0u || rule.greedy) {
-        if (rank == 0 && tid == 0) job.out[row] = most == 0u ? -1 : (int64_t)(uint32_t)~(uint32_t)best;
+    uint32_t most;
+    if (rule.greedy) {  // the largest key, and the lowest index that has it
+        u64 best = 0;
+        r.each_key([&](uint32_t i, uint32_t key) {
+            const u64 c = (u64)key << 32 | (uint32_t)~i;
+            best = key != 0u && c > best ? c : best;
+        });
+        best = r.reduce(best, [](u64 a, u64 b) { return a > b ? a : b; });
+        if (rank == 0 && tid == 0) job.out[row] = best == 0 ? -1 : (int64_t)(uint32_t)~(uint32_t)best;
         r.barrier();  // nobody leaves while others read its numbers
         return;
     }
+    float largest = -INFINITY;
+    r.each([&](uint32_t, float l) { largest = fmaxf(largest, l); });  // NaN loses
+    most = (uint32_t)r.reduce(key_of(largest), [](u64 a, u64 b) { return a > b ? a : b; });
+    if (most == 0u) {
+        if (rank == 0 && tid == 0) job.out[row] = -1;
+        r.barrier();
+        return;
+    }
     const Weigher weigh(sh.table, most, rule.inverse_T, job.shift);
-    const float top = logit_of(most), steps_per_unit = 32.0f * (float)rule.inverse_T;
-    // 2048 steps of 1/32 down from the largest logit, in fp32: monotone, and weights below 2^-50 are in the last one
-    const auto coarse = [&](uint32_t key) {
-        const float d = (top - logit_of(key)) * steps_per_unit;  // NaN for inf - inf: the first step
-        return d < (float)(BINS - 1) ? (int)d : (d >= 0.0f ? BINS - 1 : 0);
+    // halves, so that no difference of finite logits overflows
+    const float half_top = 0.5f * logit_of(most), steps_per_half = (float)fmin(64.0 * rule.inverse_T, 3e38);
+    // 2048 steps of 1/32 down from the largest logit, in fp32: monotone, and weights below 2^-50 are in the last one.
+    // It is not below any `behind` for NaN and -inf, nor for logits so far away that they weigh nothing; +inf, whose
+    // distance is not a number either, is told apart.
+    const auto distance = [&](float l) { return fmaf(l, -0.5f, half_top) * steps_per_half; };
+    const auto step_of = [&](float l) { return l == INFINITY ? 0 : (int)fminf(distance(l), (float)(BINS - 1)); };
+    const auto coarse = [&](uint32_t key) { return step_of(logit_of(key)); };
+    const auto within = [&](float l, float behind) { return distance(l) < behind || l == INFINITY; };
+    const auto done = [&](uint32_t n, uint32_t k, u64 total) {
+        if (rank == 0) {
+            const int64_t id = r.finish(n, k, total, rule, weigh);
+            if (tid == 0) job.out[row] = id;
+        }
+        r.barrier();  // nobody leaves while others read its numbers
     };
+    // min-p keeps nothing behind this step; one step more for the rounding of the distance
+    const double ratio = (double)rule.least / (double)(1ull << job.shift);
+    const int last_step = rule.least > 0 && !weigh.infinite ? (int)fmin(-log(ratio) * 32.0 + 2.0, BINS - 1.0) : BINS - 1;
     Cut cut{1u, FULL};  // everything but key 0
+    bool cut_found = false;
+    if (rule.top_k > 0 && rule.top_k <= LIST) {
+        int at;
+        u64 before, total, goal;
+        uint32_t upto;
+        r.clear_histogram();
+        r.each([&](uint32_t, float l) {
+            if (l > -INFINITY) atomicAdd(&sh.low[step_of(l)], 1u);
+        });
+        const u64 k = (u64)rule.top_k;
+        const bool cuts = r.find_step([k](u64) { return k; }, at, before, total, goal, upto);
+        const float behind = cuts && at < BINS - 1 ? (float)(at + 1) : INFINITY;
+        const uint32_t n = r.collect([&](uint32_t, float l) { return within(l, behind); });
+        if (n <= LIST) return done(n, (uint32_t)rule.top_k, 0);
+    } else if (rule.top_k == 0 && rule.top_p < 1.0) {
+        int at;
+        u64 before, total, goal;
+        uint32_t upto;
+        r.clear_histogram();
+        // lighter than (1 - p) / V of the largest: together no more than 1 - p of the total, so the border lies above them
+        const float light = (float)fmin(log((double)job.V / (1.0 - rule.top_p)) * 32.0 + 2.0, (double)(BINS - 1));
+        u64 tail = 0;
+        r.each4([&](uint32_t, uint32_t, const float (&l)[4]) {
+            u64 w[4];
+            bool heavy[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                w[e] = weigh.of(l[e]);
+                heavy[e] = within(l[e], light);
+                tail += heavy[e] ? 0ull : w[e];
+            }
+            if (!(heavy[0] | heavy[1] | heavy[2] | heavy[3])) return;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (!heavy[e]) continue;
+                const int b = step_of(l[e]);
+                r.add_weight(b, w[e]);
+                atomicAdd(&sh.count[b], 1u);
+            }
+        });
+        tail = warp_sum(tail);
+        if (r.lane == 0 && tail > 0) atomicAdd(&sh.tail, tail);
+        const double share = rule.top_p;
+        if (r.find_step([share](u64 all) { return share_of(share, all); }, at, before, total, goal, upto)) {
+            const int end = at < last_step ? at + 1 : last_step + 1;
+            const float behind = end < BINS ? (float)end : INFINITY;
+            if (upto <= LIST || at > last_step) {
+                const uint32_t n = r.collect([&](uint32_t, float l) { return within(l, behind); });
+                if (n <= LIST) return done(n, 0, total);
+            }
+            cut = r.cut_in(at, before, goal, [](uint32_t, uint32_t key) { return key != 0u; }, weigh, coarse);
+            cut_found = true;
+        }
+    } else if (rule.top_k == 0 && rule.least > 0) {
+        const float behind = last_step + 1 < BINS ? (float)(last_step + 1) : INFINITY;
+        const uint32_t n = r.collect([&](uint32_t, float l) { return within(l, behind); });
+        if (n <= LIST) return done(n, 0, 0);
+    }
+    // many candidates: the cuts one after the other, then the draw over the row
     if (rule.top_k > 0) {
         const u64 k = (u64)rule.top_k;
         Cut c;
@@ -569,7 +828,7 @@ sample_kernel(const T* __restrict__ logits, const __grid_constant__ Job job, int
                   [k](u64) { return k; }, c))
             cut = c;
     }
-    if (rule.top_p < 1.0) {
+    if (rule.top_p < 1.0 && !cut_found) {
         const Cut held = cut;
         const double p = rule.top_p;
         Cut c;
@@ -579,8 +838,11 @@ sample_kernel(const T* __restrict__ logits, const __grid_constant__ Job job, int
     }
     // the draw: every warp sums a run of the slice, the run that holds the point is cut up again
     const u64 least = rule.least;
+    const float border = cut.last == FULL ? -INFINITY : logit_of(cut.key);  // most logits are told by one comparison
     const auto kept = [&](uint32_t i) {
-        const uint32_t key = key_of(dl_to_float(r.logits[i]));
+        const float l = dl_to_float(r.logits[i]);
+        if (!(l >= border)) return (u64)0;
+        const uint32_t key = key_of(l);
         if (!cut.holds(key, i)) return (u64)0;
         const u64 w = weigh(key);
         return w < least ? (u64)0 : w;
@@ -646,10 +908,13 @@ int launch_sample(const void* logits, const Job& job, cudaStream_t s) {
         else sample_small_kernel<T, 16><<<(unsigned)blocks, 128, 0, s>>>(src, job);
         return dl_launch_status();
     }
-    // more blocks per row while they have 4096 classes each and the rows alone do not fill the SMs four times
+    // more blocks per row while they have 8192 classes each and all are resident together: every block has its own
+    // histograms, lists and barriers to go through
     int ranks = 1;
-    while (ranks < MAX_CLUSTER && job.V >= (int64_t)8192 * ranks && job.R * ranks < (int64_t)DL_NUM_SMS * 4) ranks *= 2;
+    while (ranks < MAX_CLUSTER && job.V >= (int64_t)16384 * ranks && job.R * ranks <= DL_NUM_SMS) ranks *= 2;
     if (job.R * ranks > 0x7fffffff) return DL_ERR_TOO_LARGE;
+    const int vectors = dl_address(logits) % 16 == 0 && (job.R == 1 || job.pitch * (int64_t)sizeof(T) % 16 == 0);
+    const uint32_t slice = (uint32_t)(dl_ceil_div(dl_ceil_div(job.V, ranks), 8) * 8);  // whole vectors
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(job.R * ranks));
     cfg.blockDim = dim3(THREADS);
@@ -664,7 +929,7 @@ int launch_sample(const void* logits, const Job& job, cudaStream_t s) {
     const auto kernel = sample_kernel<T>;
     static DlKernelLimits limits;
     if (!dl_allow(reinterpret_cast<const void*>(kernel), limits, sizeof(Shared), false)) return DL_ERR_LAUNCH;
-    return cudaLaunchKernelEx(&cfg, kernel, src, job, ranks) == cudaSuccess ? dl_launch_status() : DL_ERR_LAUNCH;
+    return cudaLaunchKernelEx(&cfg, kernel, src, job, ranks, slice, vectors) == cudaSuccess ? dl_launch_status() : DL_ERR_LAUNCH;
 }
 
 }  // namespace

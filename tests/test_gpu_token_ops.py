@@ -614,6 +614,15 @@ def test_sampling_extreme_temperatures(V, T):
         _check_samples(x, u, T, k, p)
 
 
+@pytest.mark.parametrize("V", [300, 3000, 40000])
+def test_sampling_logits_of_any_size(V):
+    """Differences beyond the type's range, weighed by a temperature as large."""
+    x = (_normal(8, V) * 1e38).clamp(-3.4e38, 3.4e38)
+    for T in (1.0, 1e37, 1e38, 3e38):
+        for k, p in ((0, 1.0), (20, 1.0), (2000, 0.9), (0, 0.9), (20, 0.5)):
+            _check_samples(x, _u(8), T, k, p)
+
+
 @pytest.mark.parametrize("V", [300, 3000])
 def test_sampling_ends_of_the_random_numbers(V):
     """u = 0 takes the first kept class, the largest u below 1 the last; numbers outside [0, 1) and NaN are pulled in."""
