@@ -87,36 +87,41 @@ __device__ __forceinline__ float logit_of(uint32_t key) {
     return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 
-// exp(-(top - l) / T) as fixed point.  With j = round(128 z / ln 2) and r = z - j ln 2 / 128, |r| < 0.0028,
-// e^-z = 2^(-j / 128) e^-r: a table for the fraction of the power, four terms of the series for e^-r (the fifth is below
-// 2^-49), the whole part of the power as an exponent.  Without branches: the steps of several logits then overlap.
+// exp(-(top - l) / T) as fixed point.  With t = 128 (top - l) / (T ln 2), j = round(t) and f = t - j, it is
+// 2^(-j / 128) 2^(-f / 128): a table for the fraction of the first power, its whole part as an exponent, and four terms of
+// the series of e^(-f ln 2 / 128) (|f| <= 1/2: the fifth is below 2^-49).  Ten double-precision operations, which are
+// what a pass of exponentials costs (about three cycles each for a warp); no branches, so that the steps of several logits
+// overlap.
 struct Weigher {
     const double* table;  // 2^(shift - i / 128)
-    double top, inverse_T, most_z;
+    double top, scale;    // scale: 128 / (T ln 2)
+    float least;          // logits below weigh less than half the last bit
     bool infinite;        // the largest logit is +inf: only such logits weigh something
     u64 one;
     __device__ __forceinline__ Weigher(const double* table, uint32_t top_key, double inverse_T, int shift)
-        : table(table), inverse_T(inverse_T) {
+        : table(table) {
         const float t = logit_of(top_key);
         infinite = t == INFINITY;
         top = infinite ? 0.0 : (double)t;
-        most_z = 0.6931471805599453 * (shift + 2);  // a quarter of the last bit: rounds to 0
+        scale = fmin(inverse_T * 184.6649652337873, 1e300);
+        // no more than 2^-(shift + 2), so far away that fp32 rounding does not bring it back
+        least = (float)fmax(top - (shift + 3) * 128.0 / scale, -3.4028234663852886e38);  // the lowest finite value
         one = 1ull << shift;
     }
     // 0 for NaN and -inf
     __device__ __forceinline__ u64 of(float l) const {
-        double z = (top - (double)l) * inverse_T;
-        z = z < most_z ? z : most_z;
+        const double d = top - (double)fmaxf(l, least);
         const double magic = 6755399441055744.0;  // 1.5 * 2^52: the sum's low word is the rounded integer
-        const double shifted = fma(z, 184.6649652337873, magic);
+        const double shifted = fma(d, scale, magic);
         const int j = __double2loint(shifted);
-        const double r = fma(shifted - magic, -0.0054152123481245725, z);
-        // the series in two halves, so that the steps wait less for one another
-        const double rr = r * r, e = fma(fma(fma(r, 1.0 / 24, -1.0 / 6), r, 0.5), rr, 1.0 - r);
+        const double f = fma(d, scale, magic - shifted);
+        // (ln 2 / 128)^n / n!
+        const double e = fma(f, fma(f, fma(f, fma(f, 3.583032305400251e-11, -2.6466421444330967e-08),
+                                           1.4662262387640423e-05), -0.0054152123481245725), 1.0);
         double w = table[j & (TABLE - 1)] * e;
         w = __hiloint2double(__double2hiint(w) - ((j >> 7) << 20), __double2loint(w));
         const u64 fixed = (u64)__double_as_longlong(w + 4503599627370496.0) - 0x4330000000000000ull;  // w < 2^52, rounded
-        return infinite ? (l == INFINITY ? one : 0ull) : fixed;
+        return infinite ? (l == INFINITY ? one : 0ull) : (l >= least ? fixed : 0ull);
     }
     __device__ __forceinline__ u64 operator()(uint32_t key) const { return of(logit_of(key)); }
 };
@@ -520,13 +525,15 @@ struct Row {
                 for (uint32_t i = tid; i < here; i += THREADS) sh.sorted[start + i] = other->list[i];
                 start += here;
             }
-            sort(n);
+            sort(sh, n, tid);
         }
         barrier();  // the lists are free again
         return n;
     }
     // sorts `sorted` descending by a bitonic network; entries from n up to the next power of two become 0
-    __device__ __noinline__ void sort(uint32_t n) {
+    // (Out of line, like the two functions below: they run once. Whatever they take by reference would live in memory for
+    // the whole kernel, so they take copies.)
+    __device__ __noinline__ static void sort(Shared& sh, uint32_t n, int tid) {
         uint32_t size = 2;
         while (size < n) size *= 2;
         __syncthreads();
@@ -548,7 +555,7 @@ struct Row {
     }
     // Running sums of two values per thread in list order: a, b become the sums up to and including them.  Returns the
     // total.
-    __device__ __noinline__ u64 scan_pairs(u64& a, u64& b) {
+    __device__ __forceinline__ u64 scan_pairs(u64& a, u64& b) const {
         const u64 sum = a + b, inclusive = warp_inclusive(sum, lane);
         __syncthreads();
         if (lane == 31) sh.warp_value[warp] = inclusive;
@@ -568,14 +575,16 @@ struct Row {
     // top-k keeps; total: the weight of all that top-k keeps when k is 0 (the n logits are the row's largest then, down to
     // where top-p or min-p ends).
     template <typename W>
-    __device__ __noinline__ int64_t finish(uint32_t n, uint32_t k, u64 total, const Rule& rule, const W& weigh) {
+    __device__ __noinline__ static int64_t finish(Row r, uint32_t n, uint32_t k, u64 total, Rule rule, W weigh) {
+        Shared& sh = r.sh;
+        const int tid = r.tid;
         static_assert(LIST == 2 * THREADS, "two entries per thread");
         const uint32_t i = 2 * tid;
         if (k > 0 && k < n) n = k;
         const u64 e0 = i < n ? sh.sorted[i] : 0ull, e1 = i + 1 < n ? sh.sorted[i + 1] : 0ull;
         const u64 w0 = i < n ? weigh((uint32_t)(e0 >> 32)) : 0ull, w1 = i + 1 < n ? weigh((uint32_t)(e1 >> 32)) : 0ull;
         u64 upto0 = w0, upto1 = w1;
-        const u64 all = scan_pairs(upto0, upto1);
+        const u64 all = r.scan_pairs(upto0, upto1);
         const u64 goal = rule.top_p < 1.0 ? share_of(rule.top_p, k > 0 ? all : total) : ~0ull;
         const bool keep0 = i < n && upto0 - w0 < goal && w0 >= rule.least;
         const bool keep1 = i + 1 < n && upto1 - w1 < goal && w1 >= rule.least;
@@ -584,13 +593,13 @@ struct Row {
         const uint32_t kept = __syncthreads_count(keep0) + __syncthreads_count(keep1);
         if (keep0) sh.sorted[i] = by_index(e0);
         if (keep1) sh.sorted[i + 1] = by_index(e1);
-        if (kept > 1) sort(kept);
+        if (kept > 1) sort(sh, kept, tid);
         else __syncthreads();
         const u64 a = i < kept ? sh.sorted[i] : 0ull, b = i + 1 < kept ? sh.sorted[i + 1] : 0ull;
         upto0 = i < kept ? weigh((uint32_t)a) : 0ull;
         upto1 = i + 1 < kept ? weigh((uint32_t)b) : 0ull;
         const u64 a_weight = upto0, b_weight = upto1;
-        const u64 sum = scan_pairs(upto0, upto1), point = point_of(rule.u, sum);
+        const u64 sum = r.scan_pairs(upto0, upto1), point = point_of(rule.u, sum);
         // one entry's weight spans the point
         if (a_weight > 0 && upto0 > point && upto0 - a_weight <= point) sh.found[3] = (uint32_t)~(uint32_t)(a >> 32);
         if (b_weight > 0 && upto1 > point && upto1 - b_weight <= point) sh.found[3] = (uint32_t)~(uint32_t)(b >> 32);
@@ -600,9 +609,13 @@ struct Row {
     // The cut in step `at`, before which the members weigh `before`, at which the sum of weight(key) over the members, in
     // descending order, stays below `goal`.
     template <typename M, typename W, typename S>
-    __device__ __noinline__ Cut cut_in(int at, u64 before, u64 goal, M member, W weight, S coarse) {
+    __device__ __noinline__ static Cut cut_in(Row r, int at, u64 before, u64 goal, M member, W weight, S coarse) {
+        return r.cut_here(at, before, goal, member, weight, coarse);
+    }
+    template <typename M, typename W, typename S>
+    __device__ __forceinline__ Cut cut_here(int at, u64 before, u64 goal, M member, W weight, S coarse) {
         Cut out;
-        const uint32_t n = collect([&](uint32_t i, float l) {
+        const uint32_t n = collect([=](uint32_t i, float l) {
             const uint32_t key = key_of(l);
             return member(i, key) && coarse(key) == at;
         });
@@ -702,7 +715,7 @@ struct Row {
                 },
                 goal_of, at, before, total, goal))
             return false;
-        out = cut_in(at, before, goal, member, weight, coarse);
+        out = cut_in(*this, at, before, goal, member, weight, coarse);
         return true;
     }
 };
@@ -747,13 +760,13 @@ sample_kernel(const T* __restrict__ logits, const __grid_constant__ Job job, int
     // 2048 steps of 1/32 down from the largest logit, in fp32: monotone, and weights below 2^-50 are in the last one.
     // It is not below any `behind` for NaN and -inf, nor for logits so far away that they weigh nothing; +inf, whose
     // distance is not a number either, is told apart.
-    const auto distance = [&](float l) { return fmaf(l, -0.5f, half_top) * steps_per_half; };
-    const auto step_of = [&](float l) { return l == INFINITY ? 0 : (int)fminf(distance(l), (float)(BINS - 1)); };
-    const auto coarse = [&](uint32_t key) { return step_of(logit_of(key)); };
-    const auto within = [&](float l, float behind) { return distance(l) < behind || l == INFINITY; };
+    const auto distance = [half_top, steps_per_half](float l) { return fmaf(l, -0.5f, half_top) * steps_per_half; };
+    const auto step_of = [distance](float l) { return l == INFINITY ? 0 : (int)fminf(distance(l), (float)(BINS - 1)); };
+    const auto coarse = [step_of](uint32_t key) { return step_of(logit_of(key)); };
+    const auto within = [distance](float l, float behind) { return distance(l) < behind || l == INFINITY; };
     const auto done = [&](uint32_t n, uint32_t k, u64 total) {
         if (rank == 0) {
-            const int64_t id = r.finish(n, k, total, rule, weigh);
+            const int64_t id = Row<T>::finish(r, n, k, total, rule, weigh);
             if (tid == 0) job.out[row] = id;
         }
         r.barrier();  // nobody leaves while others read its numbers
@@ -774,7 +787,7 @@ sample_kernel(const T* __restrict__ logits, const __grid_constant__ Job job, int
         const u64 k = (u64)rule.top_k;
         const bool cuts = r.find_step([k](u64) { return k; }, at, before, total, goal, upto);
         const float behind = cuts && at < BINS - 1 ? (float)(at + 1) : INFINITY;
-        const uint32_t n = r.collect([&](uint32_t, float l) { return within(l, behind); });
+        const uint32_t n = r.collect([within, behind](uint32_t, float l) { return within(l, behind); });
         if (n <= LIST) return done(n, (uint32_t)rule.top_k, 0);
     } else if (rule.top_k == 0 && rule.top_p < 1.0) {
         int at;
@@ -809,15 +822,15 @@ sample_kernel(const T* __restrict__ logits, const __grid_constant__ Job job, int
             const int end = at < last_step ? at + 1 : last_step + 1;
             const float behind = end < BINS ? (float)end : INFINITY;
             if (upto <= LIST || at > last_step) {
-                const uint32_t n = r.collect([&](uint32_t, float l) { return within(l, behind); });
+                const uint32_t n = r.collect([within, behind](uint32_t, float l) { return within(l, behind); });
                 if (n <= LIST) return done(n, 0, total);
             }
-            cut = r.cut_in(at, before, goal, [](uint32_t, uint32_t key) { return key != 0u; }, weigh, coarse);
+            cut = Row<T>::cut_in(r, at, before, goal, [](uint32_t, uint32_t key) { return key != 0u; }, weigh, coarse);
             cut_found = true;
         }
     } else if (rule.top_k == 0 && rule.least > 0) {
         const float behind = last_step + 1 < BINS ? (float)(last_step + 1) : INFINITY;
-        const uint32_t n = r.collect([&](uint32_t, float l) { return within(l, behind); });
+        const uint32_t n = r.collect([within, behind](uint32_t, float l) { return within(l, behind); });
         if (n <= LIST) return done(n, 0, 0);
     }
     // many candidates: the cuts one after the other, then the draw over the row
@@ -839,13 +852,9 @@ sample_kernel(const T* __restrict__ logits, const __grid_constant__ Job job, int
     // the draw: every warp sums a run of the slice, the run that holds the point is cut up again
     const u64 least = rule.least;
     const float border = cut.last == FULL ? -INFINITY : logit_of(cut.key);  // most logits are told by one comparison
-    const auto kept = [&](uint32_t i) {
-        const float l = dl_to_float(r.logits[i]);
-        if (!(l >= border)) return (u64)0;
-        const uint32_t key = key_of(l);
-        if (!cut.holds(key, i)) return (u64)0;
-        const u64 w = weigh(key);
-        return w < least ? (u64)0 : w;
+    const auto kept = [&](uint32_t i, float l) {
+        const u64 w = weigh.of(l);
+        return cut.holds(key_of(l), i) && w >= least ? w : 0ull;
     };
     uint32_t lo = from, hi = to;
     u64 point = 0;
@@ -854,8 +863,18 @@ sample_kernel(const T* __restrict__ logits, const __grid_constant__ Job job, int
         const uint32_t run = (hi - lo + WARPS - 1) / WARPS;
         const uint32_t begin = lo + r.warp * run < hi ? lo + r.warp * run : hi, end = begin + run < hi ? begin + run : hi;
         u64 sum = 0;
-#pragma unroll 4
-        for (uint32_t i = begin + r.lane; i < end; i += 32) sum += kept(i);
+        for (uint32_t i = begin + r.lane; i < end; i += 128) {
+            float l[4];
+            bool any = false;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                l[k] = i + 32 * k < end ? dl_to_float(r.logits[i + 32 * k]) : NAN;
+                any |= l[k] >= border;
+            }
+            if (!any) continue;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) sum += kept(i + 32 * k, l[k]);
+        }
         sum = warp_sum(sum);
         if (r.lane == 0) sh.warp_value[r.warp] = sum;
         __syncthreads();
@@ -886,7 +905,8 @@ sample_kernel(const T* __restrict__ logits, const __grid_constant__ Job job, int
         __syncthreads();
         if (hi - lo <= 32) {
             if (r.warp == 0) {
-                const u64 upto = warp_inclusive(lo + r.lane < hi ? kept(lo + r.lane) : 0ull, r.lane);
+                const u64 mine = lo + r.lane < hi ? kept(lo + r.lane, dl_to_float(r.logits[lo + r.lane])) : 0ull;
+                const u64 upto = warp_inclusive(mine, r.lane);
                 const uint32_t hit = __ballot_sync(FULL, upto > point);
                 if (r.lane == 0) job.out[row] = (int64_t)lo + __ffs(hit) - 1;
             }
