@@ -32,7 +32,7 @@ typedef unsigned long long u64;
 constexpr int THREADS = 512;
 constexpr int WARPS = THREADS / 32;
 constexpr int BINS = 2048;
-constexpr int LIST = 1024;  // most logits that are collected and sorted
+constexpr int LIST = 2048;  // most logits that are collected and sorted
 constexpr int MAX_CLUSTER = 8;
 constexpr int SMALL_V = 512;
 constexpr int TABLE = 128;
@@ -538,9 +538,12 @@ struct Row {
         while (size < n) size *= 2;
         __syncthreads();
         for (uint32_t i = n + tid; i < size; i += THREADS) sh.sorted[i] = 0;
+        // pairs up to 32 apart stay within the 64 entries that a warp holds in every step
+        __syncthreads();
         for (uint32_t run = 2; run <= size; run *= 2) {
             for (uint32_t s = run / 2; s > 0; s /= 2) {
-                __syncthreads();
+                if (s > 32 || s == 32 && run > 64) __syncthreads();
+                else __syncwarp();
                 for (uint32_t q = tid; q < size / 2; q += THREADS) {
                     const uint32_t i = 2 * q - (q & (s - 1)), j = i + s;  // q with a 0 put in at bit s
                     const u64 a = sh.sorted[i], b = sh.sorted[j];
@@ -578,31 +581,58 @@ struct Row {
     __device__ __noinline__ static int64_t finish(Row r, uint32_t n, uint32_t k, u64 total, Rule rule, W weigh) {
         Shared& sh = r.sh;
         const int tid = r.tid;
-        static_assert(LIST == 2 * THREADS, "two entries per thread");
-        const uint32_t i = 2 * tid;
+        constexpr uint32_t ROUND = 2 * THREADS;  // two entries per thread at a time
         if (k > 0 && k < n) n = k;
-        const u64 e0 = i < n ? sh.sorted[i] : 0ull, e1 = i + 1 < n ? sh.sorted[i + 1] : 0ull;
-        const u64 w0 = i < n ? weigh((uint32_t)(e0 >> 32)) : 0ull, w1 = i + 1 < n ? weigh((uint32_t)(e1 >> 32)) : 0ull;
-        u64 upto0 = w0, upto1 = w1;
-        const u64 all = r.scan_pairs(upto0, upto1);
-        const u64 goal = rule.top_p < 1.0 ? share_of(rule.top_p, k > 0 ? all : total) : ~0ull;
-        const bool keep0 = i < n && upto0 - w0 < goal && w0 >= rule.least;
-        const bool keep1 = i + 1 < n && upto1 - w1 < goal && w1 >= rule.least;
-        // by index now: the largest inverted index first
+        const auto weight = [&](uint32_t i, int word) {  // word: where the key is
+            return i < n ? weigh((uint32_t)(sh.sorted[i] >> (32 * word))) : 0ull;
+        };
+        if (k > 0 && rule.top_p < 1.0) {
+            total = 0;
+            for (uint32_t base = 0; base < n; base += ROUND) {
+                u64 a = weight(base + 2 * tid, 1), b = weight(base + 2 * tid + 1, 1);
+                total += r.scan_pairs(a, b);
+            }
+        }
+        const u64 goal = rule.top_p < 1.0 ? share_of(rule.top_p, total) : ~0ull;
+        // by index from here on: the largest inverted index first
         const auto by_index = [](u64 e) { return e << 32 | e >> 32; };
-        const uint32_t kept = __syncthreads_count(keep0) + __syncthreads_count(keep1);
-        if (keep0) sh.sorted[i] = by_index(e0);
-        if (keep1) sh.sorted[i + 1] = by_index(e1);
-        if (kept > 1) sort(sh, kept, tid);
-        else __syncthreads();
-        const u64 a = i < kept ? sh.sorted[i] : 0ull, b = i + 1 < kept ? sh.sorted[i + 1] : 0ull;
-        upto0 = i < kept ? weigh((uint32_t)a) : 0ull;
-        upto1 = i + 1 < kept ? weigh((uint32_t)b) : 0ull;
-        const u64 a_weight = upto0, b_weight = upto1;
-        const u64 sum = r.scan_pairs(upto0, upto1), point = point_of(rule.u, sum);
-        // one entry's weight spans the point
-        if (a_weight > 0 && upto0 > point && upto0 - a_weight <= point) sh.found[3] = (uint32_t)~(uint32_t)(a >> 32);
-        if (b_weight > 0 && upto1 > point && upto1 - b_weight <= point) sh.found[3] = (uint32_t)~(uint32_t)(b >> 32);
+        uint32_t kept = 0;
+        u64 before = 0;
+        for (uint32_t base = 0; base < n; base += ROUND) {
+            const uint32_t i = base + 2 * tid;
+            const u64 w0 = weight(i, 1), w1 = weight(i + 1, 1);
+            u64 upto0 = w0, upto1 = w1;
+            const u64 round = r.scan_pairs(upto0, upto1);
+            const bool keep0 = i < n && before + upto0 - w0 < goal && w0 >= rule.least;
+            const bool keep1 = i + 1 < n && before + upto1 - w1 < goal && w1 >= rule.least;
+            if (keep0) {
+                sh.sorted[i] = by_index(sh.sorted[i]);
+                if (!keep1) sh.found[2] = before + upto0;  // the last one, unless a later thread has another
+            }
+            if (keep1) sh.sorted[i + 1] = by_index(sh.sorted[i + 1]);
+            const uint32_t here = __syncthreads_count(keep0) + __syncthreads_count(keep1);
+            if (keep1 && here == (uint32_t)(2 * tid + 2)) sh.found[2] = before + upto1;
+            kept += here;
+            before += round;
+            __syncthreads();
+            if (here < ROUND) break;
+        }
+        const u64 sum = sh.found[2], point = point_of(rule.u, sum);
+        sort(sh, kept, tid);
+        n = kept;
+        before = 0;
+        for (uint32_t base = 0; base < n; base += ROUND) {
+            const uint32_t i = base + 2 * tid;
+            const u64 w0 = weight(i, 0), w1 = weight(i + 1, 0);
+            u64 upto0 = w0, upto1 = w1;
+            const u64 round = r.scan_pairs(upto0, upto1);
+            // one entry's weight spans the point
+            if (w0 > 0 && before + upto0 > point && before + upto0 - w0 <= point)
+                sh.found[3] = (uint32_t)~(uint32_t)(sh.sorted[i] >> 32);
+            if (w1 > 0 && before + upto1 > point && before + upto1 - w1 <= point)
+                sh.found[3] = (uint32_t)~(uint32_t)(sh.sorted[i + 1] >> 32);
+            before += round;
+        }
         __syncthreads();
         return (int64_t)sh.found[3];
     }
@@ -621,13 +651,17 @@ struct Row {
         });
         if (n <= LIST) {
             if (rank == 0) {
-                const uint32_t i = 2 * tid;
-                const u64 w0 = i < n ? weight((uint32_t)(sh.sorted[i] >> 32)) : 0ull;
-                const u64 w1 = i + 1 < n ? weight((uint32_t)(sh.sorted[i + 1] >> 32)) : 0ull;
-                u64 upto0 = w0, upto1 = w1;
-                scan_pairs(upto0, upto1);
-                const uint32_t kept = __syncthreads_count(i < n && before + upto0 - w0 < goal) +
-                                      __syncthreads_count(i + 1 < n && before + upto1 - w1 < goal);
+                uint32_t kept = 0;
+                for (uint32_t base = 0; base < n; base += 2 * THREADS) {
+                    const uint32_t i = base + 2 * tid;
+                    const u64 w0 = i < n ? weight((uint32_t)(sh.sorted[i] >> 32)) : 0ull;
+                    const u64 w1 = i + 1 < n ? weight((uint32_t)(sh.sorted[i + 1] >> 32)) : 0ull;
+                    u64 upto0 = w0, upto1 = w1;
+                    const u64 round = scan_pairs(upto0, upto1);
+                    kept += __syncthreads_count(i < n && before + upto0 - w0 < goal) +
+                            __syncthreads_count(i + 1 < n && before + upto1 - w1 < goal);
+                    before += round;
+                }
                 if (tid == 0) sh.found[3] = sh.sorted[kept - 1];  // the step holds the border: at least one is kept
             }
             barrier();
@@ -873,7 +907,8 @@ sample_kernel(const T* __restrict__ logits, const __grid_constant__ Job job, int
             }
             if (!any) continue;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) sum += kept(i + 32 * k, l[k]);
+            for (int k = 0; k < 4; ++k)
+                if (l[k] >= border) sum += kept(i + 32 * k, l[k]);
         }
         sum = warp_sum(sum);
         if (r.lane == 0) sh.warp_value[r.warp] = sum;
