@@ -34,18 +34,16 @@ static inline int64_t dl_max64(int64_t a, int64_t b) { return a > b ? a : b; }
 // Number of streaming multiprocessors the grids are sized for (B200: 148).
 constexpr int DL_NUM_SMS = 148;
 
-// Lets a kernel use `bytes` of dynamic shared memory (and clusters of more than eight blocks), once per device: the two
-// calls cost as much as a launch.  `done` is a static of the caller, one per kernel, always with the same size.
+// Lets a kernel use `bytes` of dynamic shared memory, asked for once per device: the call costs a good part of a launch.
+// `done` is a static of the caller, one per kernel, always with the same size.
 struct DlKernelLimits {
     std::atomic<bool> set[64];
 };
-static inline bool dl_allow(const void* kernel, DlKernelLimits& done, size_t bytes, bool large_clusters) {
+static inline bool dl_allow(const void* kernel, DlKernelLimits& done, size_t bytes) {
     int device = 0;
     if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) return false;
     if (done.set[device].load(std::memory_order_acquire)) return true;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess) return false;
-    if (large_clusters && cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
-        return false;
     done.set[device].store(true, std::memory_order_release);
     return true;
 }

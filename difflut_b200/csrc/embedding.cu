@@ -26,7 +26,7 @@ constexpr int SORT_KEYS = 8;  // per thread and tile
 constexpr int SORT_TILE = SORT_KEYS * SORT_THREADS;
 constexpr int SORT_DIGIT_BITS = 9;  // two passes sort tables of up to 2^18 - 1 rows
 constexpr int SORT_BINS = 1 << SORT_DIGIT_BITS;
-constexpr int MAX_CLUSTER = 16;  // beyond the portable 8: a B200 GPC holds 16 blocks of one SM each
+constexpr int MAX_CLUSTER = 8;  // 16 (not portable) sort in 32 us instead of 36, but beside a lookup both take 51 us
 // id as stored, or -1 when it is outside [0, V)
 template <typename I>
 __device__ __forceinline__ int64_t checked_id(const I* ids, int64_t t, int64_t V) {
@@ -83,7 +83,7 @@ __global__ void __launch_bounds__(256) embedding_kernel(Lookup<T, I> p) {
 // Stable least-significant-digit radix sort of (key, position); ids that take no gradient get the key V and end up
 // last.  Block r of the sorting cluster (the grid's first) owns the r-th run of tokens.  Per pass a warp ranks its
 // tokens among its own by matching digits, a column scan over the warps ranks them in the block, and the blocks'
-// digit counts are added up through distributed shared memory.  A run of one tile (all there is up to 131072 tokens)
+// digit counts are added up through distributed shared memory.  A run of one tile (all there is up to 65536 tokens)
 // stays on the chip: between the passes the tokens go straight to the shared memory of the block that ranks them next.
 // Longer runs are counted first and go through the workspace.
 struct SortShared {
@@ -322,9 +322,9 @@ embedding_sum_kernel(const uint2* __restrict__ sorted, const T* __restrict__ g, 
         }
         return;
     }
-    const int64_t block = (int64_t)blockIdx.x - zero_before;
-    const int slab = (int)(block % slabs);
-    const int64_t range = block / slabs * SUM_WARPS + warp;
+    // the slabs of a range are neighbouring warps: they read the same rows at the same time
+    const int64_t item = ((int64_t)blockIdx.x - zero_before) * SUM_WARPS + warp, range = item / slabs;
+    const int slab = (int)(item - range * slabs);
     if (range >= ranges) return;
     const int64_t col = ((int64_t)slab * 32 + lane) * W;
     const bool live = col < D;
@@ -516,8 +516,9 @@ BackwardPlan backward_plan(int64_t tokens, int64_t D, int64_t dtype) {
     BackwardPlan p;
     const int64_t width = 16 / dl_dtype_size(dtype);
     const int64_t slabs = dl_ceil_div(D, 32 * width);
-    // 24 warps for each SM, all of them resident at once; ranges of fewer than 8 tokens would mostly be joining
-    p.range_len = dl_min64(dl_max64(dl_ceil_div(tokens * slabs, (int64_t)DL_NUM_SMS * 24), 8), 1024);
+    // 48 warps for each SM, two rounds of what is resident: ranges differ in what they add to or leave out of their ends
+    // (65536 tokens of 2 KB: 56 us, with half as many 63 us).  Ranges of fewer than 8 tokens would mostly be joining.
+    p.range_len = dl_min64(dl_max64(dl_ceil_div(tokens * slabs, (int64_t)DL_NUM_SMS * 48), 8), 1024);
     p.ranges = dl_ceil_div(tokens, p.range_len);
     const int64_t row_len = slabs * 32 * width;  // floats per partial row: enough for every vector width
     p.off_tail = aligned256(p.ranges * row_len * 4);
@@ -549,7 +550,7 @@ int launch_forward(const void* ids, const void* weight, void* out, int64_t token
         return dl_launch_status();
     }
     const OrderPlan p = order_plan(tokens, V);
-    // runs of 1024 tokens (a key per thread) while the cluster is not full, longer ones from 16384 tokens on
+    // runs of 1024 tokens (a key per thread) while the cluster is not full, longer ones from 8192 tokens on
     int per_log2 = 10;
     while (((int64_t)MAX_CLUSTER << per_log2) < tokens) ++per_log2;
     int ranks = 1;
@@ -574,7 +575,7 @@ int launch_forward(const void* ids, const void* weight, void* out, int64_t token
     cfg.numAttrs = 1;
     const auto kernel = embedding_sorting_kernel<T, W, I>;
     static DlKernelLimits limits;
-    if (!dl_allow(reinterpret_cast<const void*>(kernel), limits, sizeof(SortShared), true)) return DL_ERR_LAUNCH;
+    if (!dl_allow(reinterpret_cast<const void*>(kernel), limits, sizeof(SortShared))) return DL_ERR_LAUNCH;
     const cudaError_t e = cudaLaunchKernelEx(
         &cfg, kernel, look, padding, reinterpret_cast<uint2*>(order), reinterpret_cast<uint2*>(order + p.off_b),
         reinterpret_cast<uint8_t*>(order + p.off_present), p.passes, p.digit_bits, per, per_log2);
@@ -613,7 +614,7 @@ int launch_sums(const char* order, const void* g, void* gw, char* scratch, int64
     float* tail = reinterpret_cast<float*>(scratch + p.off_tail);
     const int slabs = (int)dl_ceil_div(D, 32 * W);
     const int64_t zero_blocks = dl_ceil_div(V, ZERO_ROWS);
-    const int64_t blocks = dl_ceil_div(p.ranges, SUM_WARPS) * slabs + zero_blocks;
+    const int64_t blocks = dl_ceil_div(p.ranges * slabs, SUM_WARPS) + zero_blocks;
     const int64_t join_blocks = dl_ceil_div(p.ranges, JOIN_RANGES) * slabs;
     if (blocks > 0x7fffffff || join_blocks > 0x7fffffff) return DL_ERR_TOO_LARGE;
     embedding_sum_kernel<T, W><<<(unsigned)blocks, 32 * SUM_WARPS, 0, s>>>(

@@ -983,7 +983,7 @@ int launch_sample(const void* logits, const Job& job, cudaStream_t s) {
     cfg.numAttrs = 1;
     const auto kernel = sample_kernel<T>;
     static DlKernelLimits limits;
-    if (!dl_allow(reinterpret_cast<const void*>(kernel), limits, sizeof(Shared), false)) return DL_ERR_LAUNCH;
+    if (!dl_allow(reinterpret_cast<const void*>(kernel), limits, sizeof(Shared))) return DL_ERR_LAUNCH;
     return cudaLaunchKernelEx(&cfg, kernel, src, job, ranks, slice, vectors) == cudaSuccess ? dl_launch_status() : DL_ERR_LAUNCH;
 }
 

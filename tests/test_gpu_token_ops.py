@@ -211,6 +211,16 @@ def test_embedding_distributions(kind, T):
     _check_embedding(T, 700, 16, torch.float32, kind)
 
 
+@pytest.mark.parametrize("T", [65536, 65537, 140000])
+def test_embedding_more_tokens_than_the_chip_sorts_in_place(T):
+    """Up to 65536 tokens stay in distributed shared memory between the passes, more go through the workspace."""
+    ids = _ids(T, 300000, 5, "uniform").to(DEV)
+    W = torch.zeros(300000, 1, device=DEV, requires_grad=True)
+    g = torch.ones(T, 1, device=DEV)
+    (gW,) = torch.autograd.grad(embedding_lookup(ids, W), W, g)
+    assert torch.equal(gW[:, 0], torch.bincount(ids, minlength=300000).float())
+
+
 def test_embedding_long_ranges_of_one_id():
     """So many tokens that a range holds more than 32 of them."""
     _check_embedding(60000, 3, 520, torch.bfloat16, "uniform")
