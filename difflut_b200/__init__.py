@@ -3,7 +3,7 @@
 Import layout mirrors the reference package (`difflut`): `REGISTRY`, the `register_*`
 decorators, `BaseNode`, `BaseLUTLayer`, `BaseEncoder`, and the sub-packages `nodes`, `layers`,
 `encoder`, `utils`.  Importing the package registers "dwn", "probabilistic", "random",
-"learnable" and "thermometer".  All arithmetic runs in the CUDA library built from `csrc/`
+"learnable", "thermometer" and "embedding".  All arithmetic runs in the CUDA library built from `csrc/`
 (`python -m difflut_b200.build`); there is no CPU path.
 """
 

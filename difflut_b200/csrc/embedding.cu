@@ -263,8 +263,8 @@ constexpr int ROWS_IN_FLIGHT = 16;  // per warp, as copies to shared memory: 24 
 // A segment that goes on behind its range for fewer tokens than this is finished by the warp that began it; the next
 // range leaves them out.  Both sides read the same entry of the sorted list to decide.
 constexpr int REACH = 32;
-constexpr int JOIN_WARPS = 4;
-constexpr int JOIN_RANGES = 2;  // looked at per block; few have something to join
+constexpr int JOIN_WARPS = 16;
+constexpr int JOIN_RANGES = 4;  // looked at per block; few have something to join
 
 // does the segment of `key` reach REACH tokens behind position `at`?
 __device__ __forceinline__ bool reaches_far(const uint2* sorted, int64_t at, int64_t tokens, uint32_t key) {
@@ -461,7 +461,7 @@ embedding_join_kernel(const uint2* __restrict__ sorted, T* __restrict__ gw, cons
         for (int e = 0; e < W; ++e) acc[e] = 0.0f;
         const float* p = head + (range + 1 + from) * row_len + col;
         if (col < D) {
-#pragma unroll 4
+#pragma unroll 8
             for (int64_t i = from; i < to; ++i, p += row_len) {
                 const DlVec<float, W> row = *reinterpret_cast<const DlVec<float, W>*>(p);
 #pragma unroll

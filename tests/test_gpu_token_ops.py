@@ -11,10 +11,12 @@ import numpy as np
 import pytest
 import torch
 
-from difflut_b200.encoder import EmbeddingEncoder, embedding_lookup
+from difflut_b200.encoder import EmbeddingEncoder, ThermometerEncoder, embedding_lookup
 from difflut_b200.layers import ConvolutionalLayer, ConvolutionConfig, RandomLayer
-from difflut_b200.nodes import NodeConfig, ProbabilisticNode
-from difflut_b200.utils import Dropout, GroupNorm, dropout, group_norm, sample_logits
+from difflut_b200.network import DWNNetwork
+from difflut_b200.nodes import DWNNode, NodeConfig, ProbabilisticNode
+from difflut_b200.utils import Dropout, GroupNorm, GroupSum, dropout, group_norm, sample_logits
+from parity_util import close_normwise
 from token_util import (TYPES, check, dropped, embedding_grad, half_step, kept_weights, norm_reference, sample_row,
                         smallest)
 
@@ -712,3 +714,112 @@ def test_sampling_captured_and_on_streams():
             outs.append(sample_logits(x, u, temperature=0.9, top_k=100, top_p=0.9))
     torch.cuda.synchronize()
     assert all(torch.equal(o, got) for o in outs)
+
+
+# ---------------------------------------------------------------------------------------------- all of them together
+class _TokenModel(torch.nn.Module):
+    """ids (B, T) -> embedding -> group norm + sigmoid -> dropout -> LUT layer -> GroupSum logits (B, k)."""
+
+    def __init__(self, vocabulary, tokens, width, nodes, classes, p):
+        super().__init__()
+        self.encoder = EmbeddingEncoder(vocabulary, num_bits=width, scale=2.0, padding_idx=0, flatten=False)
+        self.norm = GroupNorm(4, width, activation="sigmoid")
+        self.dropout = Dropout(p)
+        self.layer = RandomLayer(tokens * width, nodes, ProbabilisticNode, NodeConfig(input_dim=4, output_dim=1), seed=3)
+        self.head = GroupSum(k=classes, tau=2.0, use_randperm=False)
+
+    def features(self, ids):
+        return self.norm(self.encoder(ids)).reshape(ids.shape[0], -1)
+
+    def forward(self, ids, mask=None):
+        x = self.features(ids)
+        x = self.dropout(x) if mask is None else dropout(x, self.dropout.p, **mask)
+        return self.head(self.layer(x))
+
+
+def _token_model(p=0.25):
+    torch.manual_seed(0)
+    model = _TokenModel(50, 6, 16, 60, 10, p).to(DEV).train()
+    g = torch.Generator().manual_seed(1)
+    ids = torch.randint(0, 50, (33, 6), generator=g).to(DEV)
+    labels = torch.randint(0, 10, (33,), generator=g).to(DEV)
+    return model, ids, labels
+
+
+def test_token_model_equals_its_plain_form():
+    """Logits, loss and every gradient against the same LUT layer behind 64-bit plain forms of the operators."""
+    model, ids, labels = _token_model()
+    logits = model(ids, dict(seed=11, offset=4))
+    loss = torch.nn.functional.cross_entropy(logits, labels)
+    loss.backward()
+    table = model.encoder.weight.detach().double().requires_grad_(True)
+    w, b = (t.detach().double().requires_grad_(True) for t in (model.norm.weight, model.norm.bias))
+    x = table[ids] * 2.0
+    x = torch.sigmoid(torch.nn.functional.group_norm(x.transpose(1, 2), 4, w, b)).transpose(1, 2).reshape(33, -1)
+    gone = dropped(x.numel(), 0.25, 11, 4).view(x.shape).to(DEV)
+    x = torch.where(gone, 0.0, x / 0.75).float()
+    names = [n for n, _ in model.layer.named_parameters()]
+    before = {n: p.grad.clone() for n, p in model.layer.named_parameters()}
+    model.layer.zero_grad()
+    want = model.head(model.layer(x))
+    want_loss = torch.nn.functional.cross_entropy(want, labels)
+    want_loss.backward()
+    # inputs differ in the last bits of fp32; the layer's outputs are sums of 16 products of four such inputs
+    assert float((logits - want).abs().max()) <= 1e-5 * float(want.abs().max())
+    assert abs(float(loss - want_loss)) <= 1e-5
+    close_normwise(before[names[0]], dict(model.layer.named_parameters())[names[0]].grad, "layer")
+    table.grad[0] = 0.0  # padding
+    close_normwise(model.encoder.weight.grad, table.grad, "embedding table")
+    close_normwise(model.norm.weight.grad, w.grad, "norm weight")
+    close_normwise(model.norm.bias.grad, b.grad, "norm bias")
+
+
+def test_token_model_trains_captured_and_samples():
+    """A captured step draws a new mask per replay and moves the parameters; ids are then sampled from the logits."""
+    model, ids, labels = _token_model(p=0.5)
+    optimizer = torch.optim.SGD(model.parameters(), lr=0.5)
+
+    def step():
+        optimizer.zero_grad(set_to_none=True)
+        loss = torch.nn.functional.cross_entropy(model(ids), labels)
+        loss.backward()
+        optimizer.step()
+        return loss.detach()
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss = step()
+    start = [p.detach().clone() for p in model.parameters()]
+    losses = []
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        losses.append(float(loss))
+    assert len(set(losses)) == 3 and all(math.isfinite(v) for v in losses)
+    assert all(not torch.equal(a, p) for a, p in zip(start, model.parameters()))
+    model.eval()
+    with torch.no_grad():
+        assert model.dropout(ids) is ids
+        logits = model.head(model.layer(model.features(ids)))
+    _check_samples(logits, _u(33), 0.5, 4, 0.9)
+
+
+def test_network_samples_from_its_logits():
+    x = torch.rand(300, 12, generator=torch.Generator().manual_seed(0))
+    enc = ThermometerEncoder(num_bits=4).fit(x)
+    layers = [RandomLayer(48, 40, DWNNode, NodeConfig(input_dim=6, output_dim=1), seed=0).to(DEV),
+              RandomLayer(40, 30, DWNNode, NodeConfig(input_dim=6, output_dim=1), seed=1).to(DEV)]
+    net = DWNNetwork(enc, layers, GroupSum(k=10, tau=1.0, use_randperm=False))
+    x, u = x.to(DEV), _u(300)
+    logits = net.logits(x)
+    assert torch.equal(net.sample(x, u, temperature=0.7, top_k=3), sample_logits(logits, u, temperature=0.7, top_k=3))
+    assert torch.equal(net.sample(x, temperature=0.0), logits.argmax(dim=1))
+    ids = net.sample(x)
+    assert ids.shape == (300,) and int(ids.min()) >= 0 and int(ids.max()) < 10
