@@ -96,7 +96,6 @@ __device__ __forceinline__ void load_params(const Norm& p, int c, float (&w)[W],
 
 // ------------------------------------------------------------------------------------------ chunks of rows
 constexpr int CHUNK_THREADS = 256;
-constexpr int IN_FLIGHT = 4;  // rows a thread loads before it uses the first
 
 // How the tensor is cut; a function of sizes, type and alignment.
 struct Cut {
@@ -151,26 +150,59 @@ struct Place {
     __device__ __forceinline__ int part(const Cut& k) const { return chunk * k.split + piece; }
 };
 
-// f(row, vectors...) for every row of the thread, IN_FLIGHT loads of every tensor ahead of their use
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
+
+// rows of every tensor that a thread has on their way to its slots of shared memory, at 16 bytes each
+template <int TENSORS>
+struct Ring {
+    static constexpr int AHEAD = TENSORS == 1 ? 8 : 4;  // 32 KB per block
+    template <typename V>
+    static constexpr size_t bytes() {
+        return sizeof(V) < 4 ? 0 : (size_t)AHEAD * TENSORS * CHUNK_THREADS * sizeof(V);
+    }
+};
+
+// f(row, vectors...) for every row of the thread.  The rows come through a ring in shared memory, of which every thread
+// fills and reads its own slots: loads go on while it computes, without holding registers (batches of four loads in
+// registers instead: 17 and 38 us instead of 13 and 30 us for the sums of 33.5 M bf16 elements forward and backward).
 template <typename T, int W, typename F, typename... Src>
 __device__ __forceinline__ void each_row(const Place& at, const Cut& k, int64_t pitch, F f, const Src*... src) {
-    int r = at.ty;
-    for (; r + (IN_FLIGHT - 1) * k.ty < at.rows; r += IN_FLIGHT * k.ty) {
-        DlVec<T, W> v[sizeof...(Src)][IN_FLIGHT];
+    if constexpr (sizeof(DlVec<T, W>) < 4) {  // there is no such copy of two bytes
+        for (int r = at.ty; r < at.rows; r += k.ty) f(r, *reinterpret_cast<const DlVec<T, W>*>(src + r * pitch)...);
+    } else {
+        constexpr int TENSORS = (int)sizeof...(Src), AHEAD = Ring<TENSORS>::AHEAD, BYTES = (int)sizeof(DlVec<T, W>);
+        extern __shared__ __align__(16) unsigned char ring_bytes_of_block[];
+        DlVec<T, W>* ring = reinterpret_cast<DlVec<T, W>*>(ring_bytes_of_block) + threadIdx.x;
         const T* const from[] = {src...};
+        auto request = [&](int r, int slot) {
+            if (r < at.rows) {
 #pragma unroll
-        for (int u = 0; u < IN_FLIGHT; ++u) {
+                for (int s = 0; s < TENSORS; ++s) {
+                    const uint32_t to = (uint32_t)__cvta_generic_to_shared(ring + (slot * TENSORS + s) * CHUNK_THREADS);
+                    if constexpr (BYTES == 16)
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from[s] + r * pitch) : "memory");
+                    else
+                        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(from[s] + r * pitch), "n"(BYTES)
+                                     : "memory");
+                }
+            }
+            copy_commit();
+        };
 #pragma unroll
-            for (int s = 0; s < (int)sizeof...(Src); ++s)
-                v[s][u] = *reinterpret_cast<const DlVec<T, W>*>(from[s] + (r + u * k.ty) * pitch);
+        for (int d = 0; d < AHEAD; ++d) request(at.ty + d * k.ty, d);
+        int slot = 0;
+        for (int r = at.ty; r < at.rows; r += k.ty) {
+            copy_wait<AHEAD - 1>();
+            const DlVec<T, W>* here = ring + slot * TENSORS * CHUNK_THREADS;
+            if constexpr (TENSORS == 1) f(r, here[0]);
+            else f(r, here[0], here[CHUNK_THREADS]);
+            request(r + AHEAD * k.ty, slot);
+            slot = slot + 1 < AHEAD ? slot + 1 : 0;
         }
-#pragma unroll
-        for (int u = 0; u < IN_FLIGHT; ++u) {
-            if constexpr (sizeof...(Src) == 1) f(r + u * k.ty, v[0][u]);
-            else f(r + u * k.ty, v[0][u], v[1][u]);
-        }
+        copy_wait<0>();  // nothing is under way into slots that are used again
     }
-    for (; r < at.rows; r += k.ty) f(r, *reinterpret_cast<const DlVec<T, W>*>(src + r * pitch)...);
 }
 
 // Joins sets of values given by count, mean and squares around their means, one per call and lane, about the mean of one
@@ -676,10 +708,10 @@ Cut cut_chunks(const Norm& p, int W, int resident) {
     k.tx = k.split > 1 ? (int)dl_ceil_div(k.lanes, k.split) : k.groups * k.lanes;
     k.ty = (int)dl_min64(CHUNK_THREADS / k.tx, p.S);
     k.blocks_c = (int)(dl_ceil_div(p.G, k.groups) * k.split);
-    // as many chunks as are resident at once, but at least two rounds of loads in each; a sample whose groups are split
+    // as many chunks as are resident at once, but rows enough in each to keep the loads going; a sample whose groups are split
     // over blocks of channels always takes two launches
     const int64_t units = p.N * k.blocks_c, slots = (int64_t)DL_NUM_SMS * resident;
-    const int64_t most = dl_max64(p.S / ((int64_t)k.ty * IN_FLIGHT * 2), 1);
+    const int64_t most = dl_max64(p.S / ((int64_t)k.ty * 8), 1);
     k.chunks = (int)dl_max64(dl_min64(slots / dl_max64(units, 1), most), 1);
     k.rows = (int)dl_ceil_div(p.S, k.chunks);
     k.chunks = (int)dl_ceil_div(p.S, k.rows);
@@ -732,13 +764,14 @@ int launch_forward(const void* x, void* y, float* mean, float* rstd, float* sums
     const Cut k = cut_chunks(p, W, RESIDENT);
     if (!grid_fits(p, k)) return DL_ERR_TOO_LARGE;
     const unsigned blocks = (unsigned)(p.N * k.blocks_c * k.chunks);
+    constexpr size_t ring = Ring<1>::template bytes<DlVec<T, W>>();
     if (one_launch(k)) {
-        norm_chunk_kernel<T, W, SUMS | WRITE><<<blocks, threads_of(k), 0, s>>>(src, dst, mean, rstd, sums, p, k);
+        norm_chunk_kernel<T, W, SUMS | WRITE><<<blocks, threads_of(k), ring, s>>>(src, dst, mean, rstd, sums, p, k);
         return dl_launch_status();
     }
-    norm_chunk_kernel<T, W, SUMS><<<blocks, threads_of(k), 0, s>>>(src, dst, mean, rstd, sums, p, k);
+    norm_chunk_kernel<T, W, SUMS><<<blocks, threads_of(k), ring, s>>>(src, dst, mean, rstd, sums, p, k);
     if (cudaPeekAtLastError() != cudaSuccess) return DL_ERR_LAUNCH;
-    norm_chunk_kernel<T, W, WRITE><<<blocks, threads_of(k), 0, s>>>(src, dst, mean, rstd, sums, p, k);
+    norm_chunk_kernel<T, W, WRITE><<<blocks, threads_of(k), ring, s>>>(src, dst, mean, rstd, sums, p, k);
     return dl_launch_status();
 }
 
@@ -776,14 +809,15 @@ int launch_backward(const void* x, const void* g, const float* mean, const float
         const Cut k = cut_chunks(p, W, RESIDENT_BWD);
         if (!grid_fits(p, k)) return DL_ERR_TOO_LARGE;
         const unsigned blocks = (unsigned)(p.N * k.blocks_c * k.chunks);
+        constexpr size_t ring = Ring<2>::template bytes<DlVec<T, W>>();
         if (one_launch(k)) {
-            norm_chunk_bwd_kernel<T, W, SUMS | WRITE><<<blocks, threads_of(k), 0, s>>>(src, src_g, mean, rstd, dst, scratch,
+            norm_chunk_bwd_kernel<T, W, SUMS | WRITE><<<blocks, threads_of(k), ring, s>>>(src, src_g, mean, rstd, dst, scratch,
                                                                                       partial, p, k);
         } else {
-            norm_chunk_bwd_kernel<T, W, SUMS><<<blocks, threads_of(k), 0, s>>>(src, src_g, mean, rstd, dst, scratch, partial,
+            norm_chunk_bwd_kernel<T, W, SUMS><<<blocks, threads_of(k), ring, s>>>(src, src_g, mean, rstd, dst, scratch, partial,
                                                                               p, k);
             if (cudaPeekAtLastError() != cudaSuccess) return DL_ERR_LAUNCH;
-            norm_chunk_bwd_kernel<T, W, WRITE><<<blocks, threads_of(k), 0, s>>>(src, src_g, mean, rstd, dst, scratch,
+            norm_chunk_bwd_kernel<T, W, WRITE><<<blocks, threads_of(k), ring, s>>>(src, src_g, mean, rstd, dst, scratch,
                                                                                partial, p, k);
         }
     }
