@@ -326,8 +326,8 @@ struct Row {
         if (ranks > 1) cluster.sync();
         else __syncthreads();
     }
-    // f(index, stride, four logits) over the slice, element e at index + e * stride; NaN where there is none.  By vectors
-    // when every row starts on 16 bytes (slices do then).
+    // f(index, stride, four logits) over the slice, element e at index + e * stride; NaN where there is none.  The lanes of a
+    // warp call f together.  By vectors when every row starts on 16 bytes (slices do then).
     template <typename F>
     __device__ __forceinline__ void each4(F f) const {
         constexpr int N = 16 / sizeof(T), AHEAD = 16 / N;
@@ -354,11 +354,14 @@ struct Row {
             }
             i = whole;
         }
-        for (i += tid; i < to; i += 4 * THREADS) {
+        for (; i < to; i += 4 * THREADS) {  // all lanes together
             float l[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) l[k] = i + k * THREADS < to ? dl_to_float(logits[i + k * THREADS]) : NAN;
-            f(i, (uint32_t)THREADS, l);
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t at = i + tid + k * THREADS;
+                l[k] = at < to ? dl_to_float(logits[at]) : NAN;
+            }
+            f(i + tid, (uint32_t)THREADS, l);
         }
     }
     template <typename F>
@@ -506,12 +509,21 @@ struct Row {
             bool want[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) want[e] = wanted(i + e * stride, l[e]);
-            if (!(want[0] | want[1] | want[2] | want[3])) return;
+            // one atomic per warp: on one address they follow one another
+            uint32_t mask[4], all = 0;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                if (!want[e]) continue;
-                const uint32_t n = atomicAdd(&sh.list_count, 1u);
-                if (n < LIST) sh.list[n] = (u64)key_of(l[e]) << 32 | (uint32_t)~(i + e * stride);
+                mask[e] = __ballot_sync(FULL, want[e]);
+                all += __popc(mask[e]);
+            }
+            if (all == 0) return;
+            uint32_t at = lane == 0 ? atomicAdd(&sh.list_count, all) : 0u;
+            at = __shfl_sync(FULL, at, 0);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t n = at + __popc(mask[e] & ((1u << lane) - 1));
+                if (want[e] && n < LIST) sh.list[n] = (u64)key_of(l[e]) << 32 | (uint32_t)~(i + e * stride);
+                at += __popc(mask[e]);
             }
         });
         barrier();
@@ -530,29 +542,58 @@ struct Row {
         barrier();  // the lists are free again
         return n;
     }
-    // sorts `sorted` descending by a bitonic network; entries from n up to the next power of two become 0
-    // (Out of line, like the two functions below: they run once. Whatever they take by reference would live in memory for
-    // the whole kernel, so they take copies.)
+    // Sorts `sorted` descending by a bitonic network; what is behind n becomes 0.  A thread holds four neighbours: partners
+    // one and two apart are its own, up to 64 apart other lanes', farther ones come through shared memory (10 of 66 steps
+    // for 2048; with every step there it took 17 us).  (Out of line, like the two functions below: they run once. Whatever
+    // they take by reference would live in memory for the whole kernel, so they take copies.)
     __device__ __noinline__ static void sort(Shared& sh, uint32_t n, int tid) {
-        uint32_t size = 2;
+        static_assert(LIST == 4 * THREADS, "four entries per thread");
+        uint32_t size = 128;  // whole warps
         while (size < n) size *= 2;
+        const uint32_t first = 4 * tid;
+        const bool active = first < size;
+        u64 v[4];
         __syncthreads();
-        for (uint32_t i = n + tid; i < size; i += THREADS) sh.sorted[i] = 0;
-        // pairs up to 32 apart stay within the 64 entries that a warp holds in every step
-        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = first + e < n ? sh.sorted[first + e] : 0ull;
+        const auto order = [](u64& a, u64& b, bool descending) {
+            if ((a < b) == descending) {
+                const u64 c = a;
+                a = b;
+                b = c;
+            }
+        };
         for (uint32_t run = 2; run <= size; run *= 2) {
             for (uint32_t s = run / 2; s > 0; s /= 2) {
-                if (s > 32 || s == 32 && run > 64) __syncthreads();
-                else __syncwarp();
-                for (uint32_t q = tid; q < size / 2; q += THREADS) {
-                    const uint32_t i = 2 * q - (q & (s - 1)), j = i + s;  // q with a 0 put in at bit s
-                    const u64 a = sh.sorted[i], b = sh.sorted[j];
-                    if ((a < b) == ((i & run) == 0)) {
-                        sh.sorted[i] = b;
-                        sh.sorted[j] = a;
+                if (s >= 128) {
+                    __syncthreads();
+                    if (active) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) sh.sorted[first + e] = v[e];
+                    }
+                    __syncthreads();
+                }
+                if (!active) continue;
+                if (s == 1) {
+                    order(v[0], v[1], (first & run) == 0);
+                    order(v[2], v[3], ((first + 2) & run) == 0);
+                } else if (s == 2) {
+                    order(v[0], v[2], (first & run) == 0);
+                    order(v[1], v[3], (first & run) == 0);
+                } else {
+                    const bool larger = ((first & s) == 0) == ((first & run) == 0);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const u64 o = s >= 128 ? sh.sorted[(first + e) ^ s] : __shfl_xor_sync(FULL, v[e], s / 4);
+                        if ((v[e] < o) == larger) v[e] = o;
                     }
                 }
             }
+        }
+        __syncthreads();
+        if (active) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sh.sorted[first + e] = v[e];
         }
         __syncthreads();
     }
