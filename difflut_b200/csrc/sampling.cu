@@ -5,11 +5,13 @@
 //   the class is the first i, in ascending order, whose running sum of kept weights exceeds u * (total kept weight).
 //
 // Both cuts are one question: down to which (logit, index) does a running sum, of ones or of weights, stay below a
-// target?  It is answered without sorting: a histogram over (max - l) / T in 2048 steps of 1/32 finds the step in which
-// the target falls.  Usually at most a thousand logits lie in that step and above it (min-p only lowers their number):
-// they are collected and sorted in shared memory, where cuts and draw are prefix sums.  Otherwise the logits of that one
-// step are sorted (or, when very many share it, told apart by histograms over the bits of their keys and, for equal ones,
-// over their index), and the draw goes over the row once more.
+// target?  It is answered without sorting the row: a histogram over (max - l) / T in 2048 steps of 1/32 finds the step in
+// which the target falls.  The logits in that step and above it are collected in lists in shared memory, and only those of
+// that one step are sorted.  The draw is a histogram as well, of the listed weights over the index, and the 1/2048 of the row
+// in which the point falls is read once more.  (Sorting the whole list by key and then by index took 34 of 48 us for 1900
+// logits.)  For top-k the list is short: it is sorted, and cuts and draw are prefix sums.  Should the lists not hold them,
+// the logits of the step are told apart by histograms over the bits of their keys and, for equal ones, over their index, and
+// the draw goes over the row.
 //
 // A class next to a border must not depend on the order of additions, so weights are whole numbers: exp in double
 // precision, as fixed point with up to 50 fractional bits, chosen so that the sum of a row fits 62 bits.  Integer sums are
@@ -19,6 +21,12 @@
 //
 // Rows of up to 512 classes take one warp and registers; longer ones a block of 512 threads, or a cluster of up to
 // eight when there are few rows.  Each pass reads the logits again: after the first they come from L2.
+//
+// Measured: 64 rows of 32000 bf16 logits, T .8: 5.8 us for the largest, 19 us to draw from all, 20 us with top-k 50 and top-p
+// .95, 35 us with top-p .95 alone.  Of the latter the histogram of the weights takes 11 us, the two searches in histograms
+// 3 us each, collecting 6 us: latency of passes with one or two rounds of loads per thread, not bandwidth (the 4 MB are read
+// in a microsecond).  256 rows of 65536 fp32 logits with top-p .9 and min-p .01: 88 us, 43 of them the histogram, bound by
+// double precision and shared-memory atomics (the 67 MB take 10).
 #include <cooperative_groups.h>
 
 #include "elements.cuh"
@@ -295,15 +303,14 @@ sample_small_kernel(const T* __restrict__ logits, const __grid_constant__ Job jo
 struct __align__(16) Shared {
     double table[TABLE];
     uint32_t low[BINS], high[BINS];  // the two words of every step's sum
-    uint32_t count[BINS];
     u64 list[LIST];    // collected by this block: key, then the index inverted
+    u64 part[LIST];    // those of the list that share a step
     u64 sorted[LIST];  // of the whole row, in the first block
     u64 warp_value[WARPS];
-    uint32_t warp_counted[WARPS];
     u64 tail;
     u64 found[4];
     u64 published[2][4];  // for the other blocks, two turns
-    uint32_t list_count;
+    uint32_t list_count, part_count;
 };
 
 // down to where a running sum stays below its target: keys above, and equal keys up to an index
@@ -396,7 +403,7 @@ struct Row {
     }
     void __device__ __forceinline__ clear_histogram() {
         __syncthreads();
-        for (int b = tid; b < BINS; b += THREADS) sh.low[b] = sh.high[b] = sh.count[b] = 0;
+        for (int b = tid; b < BINS; b += THREADS) sh.low[b] = sh.high[b] = 0;
         if (tid == 0) {
             sh.found[0] = BINS;
             sh.tail = 0;
@@ -408,82 +415,67 @@ struct Row {
         const uint32_t hi = (uint32_t)(value >> 32) + (old + lo < old ? 1u : 0u);
         if (hi) atomicAdd(&sh.high[b], hi);
     }
+    // four at once, so that their round trips overlap
+    __device__ __forceinline__ void add_weights(const int (&b)[4], const u64 (&value)[4]) {
+        uint32_t old[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (value[e]) old[e] = atomicAdd(&sh.low[b[e]], (uint32_t)value[e]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (!value[e]) continue;
+            const uint32_t lo = (uint32_t)value[e], hi = (uint32_t)(value[e] >> 32) + (old[e] + lo < old[e] ? 1u : 0u);
+            if (hi) atomicAdd(&sh.high[b[e]], hi);
+        }
+    }
     // The step at which the row's sum over the histogram reaches target(total); total includes the tails.  False: it never
-    // does.  upto: how many logits were counted up to and including that step.
+    // does.
     template <typename G>
-    __device__ __forceinline__ bool find_step(G target, int& at, u64& before, u64& total, u64& goal, uint32_t& upto) {
+    __device__ __forceinline__ bool find_step(G target, int& at, u64& before, u64& total, u64& goal) {
         barrier();
         constexpr int PER = BINS / THREADS;
         u64 v[PER], sum = 0;
-        uint32_t n[PER], counted = 0;
         total = 0;
         if (ranks > 1)
             for (int r = 0; r < ranks; ++r) total += *cluster.map_shared_rank(&sh.tail, r);
         else
             total = sh.tail;
 #pragma unroll
-        for (int k = 0; k < PER; ++k) {
-            v[k] = 0;
-            n[k] = 0;
-        }
+        for (int k = 0; k < PER; ++k) v[k] = 0;
         for (int r = 0; r < ranks; ++r) {
             const Shared* other = ranks > 1 ? cluster.map_shared_rank(&sh, r) : &sh;
             static_assert(PER == 4, "one access per array");
             const uint4 lo = *reinterpret_cast<const uint4*>(&other->low[tid * PER]);
             const uint4 hi = *reinterpret_cast<const uint4*>(&other->high[tid * PER]);
-            const uint4 c = *reinterpret_cast<const uint4*>(&other->count[tid * PER]);
             v[0] += (u64)lo.x | (u64)hi.x << 32;
             v[1] += (u64)lo.y | (u64)hi.y << 32;
             v[2] += (u64)lo.z | (u64)hi.z << 32;
             v[3] += (u64)lo.w | (u64)hi.w << 32;
-            n[0] += c.x;
-            n[1] += c.y;
-            n[2] += c.z;
-            n[3] += c.w;
         }
 #pragma unroll
-        for (int k = 0; k < PER; ++k) {
-            sum += v[k];
-            counted += n[k];
-        }
+        for (int k = 0; k < PER; ++k) sum += v[k];
         const u64 inclusive = warp_inclusive(sum, lane);
-        uint32_t counted_inclusive = counted;
-#pragma unroll
-        for (int s = 1; s < 32; s <<= 1) {
-            const uint32_t o = __shfl_up_sync(FULL, counted_inclusive, s);
-            if (lane >= s) counted_inclusive += o;
-        }
-        if (lane == 31) {
-            sh.warp_value[warp] = inclusive;
-            sh.warp_counted[warp] = counted_inclusive;
-        }
+        if (lane == 31) sh.warp_value[warp] = inclusive;
         __syncthreads();
         u64 run = inclusive - sum;
-        uint32_t run_counted = counted_inclusive - counted;
 #pragma unroll
         for (int k = 0; k < WARPS; ++k) {
             const u64 w = sh.warp_value[k];
-            if (k < warp) {
-                run += w;
-                run_counted += sh.warp_counted[k];
-            }
+            if (k < warp) run += w;
             total += w;
         }
         goal = target(total);
 #pragma unroll
         for (int k = 0; k < PER; ++k) {
-            run_counted += n[k];
             if (run < goal && run + v[k] >= goal) {
                 sh.found[0] = tid * PER + k;
                 sh.found[1] = run;
-                sh.found[2] = run_counted;
             }
             run += v[k];
         }
         barrier();  // also: nobody clears a histogram that others still read
         at = (int)sh.found[0];
         before = sh.found[1];
-        upto = (uint32_t)sh.found[2];
         return at < BINS;
     }
     // adds value(i, key) at step(i, key) wherever that is not negative, and finds the step of target(total)
@@ -495,14 +487,12 @@ struct Row {
             const int b = step(i, key, value);
             if (b >= 0) add_weight(b, value);
         });
-        uint32_t unused;
-        return find_step(target, at, before, total, goal, unused);
+        return find_step(target, at, before, total, goal);
     }
-    // Collects the logits that wanted(index, logit) accepts.  Returns how many the row has; up to LIST of them are then
-    // `sorted` in the cluster's first block, largest first, equal ones by index.
+    // Collects the logits that wanted(index, logit) accepts in the blocks' lists.  False: a list was too short for them.
     template <typename F>
-    __device__ __forceinline__ uint32_t collect(F wanted) {
-        __syncthreads();
+    __device__ __forceinline__ bool collect(F wanted) {
+        barrier();  // nobody reads the last list any more
         if (tid == 0) sh.list_count = 0;
         __syncthreads();
         each4([&](uint32_t i, uint32_t stride, const float (&l)[4]) {
@@ -527,33 +517,58 @@ struct Row {
             }
         });
         barrier();
+        bool fits = true;
+        for (int r = 0; r < ranks; ++r)
+            fits &= (ranks > 1 ? *cluster.map_shared_rank(&sh.list_count, r) : sh.list_count) <= LIST;
+        return fits;
+    }
+    // Brings the entries of the blocks' lists (`part`: of their parts) to the first block and sorts them there, if there
+    // are no more than LIST, largest first, equal ones by index.  Returns how many there are.  After a barrier.
+    __device__ __forceinline__ uint32_t gather(bool part) {
         uint32_t n = 0;
-        for (int r = 0; r < ranks; ++r) n += ranks > 1 ? *cluster.map_shared_rank(&sh.list_count, r) : sh.list_count;
+        for (int r = 0; r < ranks; ++r) {
+            const Shared* other = ranks > 1 ? cluster.map_shared_rank(&sh, r) : &sh;
+            n += part ? other->part_count : other->list_count;
+        }
         if (rank == 0 && n <= LIST) {
             uint32_t start = 0;
             for (int r = 0; r < ranks; ++r) {
                 const Shared* other = ranks > 1 ? cluster.map_shared_rank(&sh, r) : &sh;
-                const uint32_t here = other->list_count;
-                for (uint32_t i = tid; i < here; i += THREADS) sh.sorted[start + i] = other->list[i];
+                const uint32_t here = part ? other->part_count : other->list_count;
+                for (uint32_t i = tid; i < here; i += THREADS) sh.sorted[start + i] = (part ? other->part : other->list)[i];
                 start += here;
             }
             sort(sh, n, tid);
         }
-        barrier();  // the lists are free again
         return n;
     }
-    // Sorts `sorted` descending by a bitonic network; what is behind n becomes 0.  A thread holds four neighbours: partners
+    // Sorts `sorted` descending: by counting, or by a bitonic network.  There a thread holds four neighbours: partners
     // one and two apart are its own, up to 64 apart other lanes', farther ones come through shared memory (10 of 66 steps
-    // for 2048; with every step there it took 17 us).  (Out of line, like the two functions below: they run once. Whatever
+    // for 2048).  (Out of line, like the two functions below: they run once. Whatever
     // they take by reference would live in memory for the whole kernel, so they take copies.)
     __device__ __noinline__ static void sort(Shared& sh, uint32_t n, int tid) {
         static_assert(LIST == 4 * THREADS, "four entries per thread");
-        uint32_t size = 128;  // whole warps
+        __syncthreads();
+        if (n <= THREADS) {
+            // few: the place of an entry is the number of larger ones; all are different.  Several lanes share the counting.
+            uint32_t lanes = 32;
+            while (lanes * n > THREADS) lanes /= 2;
+            const uint32_t i = tid / lanes;
+            const u64 mine = i < n ? sh.sorted[i] : 0ull;
+            uint32_t place = 0;
+            if (i < n)
+                for (uint32_t j = tid % lanes; j < n; j += lanes) place += sh.sorted[j] > mine;
+            for (uint32_t s = lanes / 2; s > 0; s /= 2) place += __shfl_xor_sync(FULL, place, s);
+            __syncthreads();
+            if (i < n && tid % lanes == 0) sh.sorted[place] = mine;
+            __syncthreads();
+            return;
+        }
+        uint32_t size = 2 * THREADS;
         while (size < n) size *= 2;
         const uint32_t first = 4 * tid;
         const bool active = first < size;
         u64 v[4];
-        __syncthreads();
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = first + e < n ? sh.sorted[first + e] : 0ull;
         const auto order = [](u64& a, u64& b, bool descending) {
@@ -615,25 +630,23 @@ struct Row {
         b = run + sum;
         return total;
     }
-    // Cuts and draw among the n sorted logits, by the first block.  What is kept is a prefix of them.  k: 0, or how many
-    // top-k keeps; total: the weight of all that top-k keeps when k is 0 (the n logits are the row's largest then, down to
-    // where top-p or min-p ends).
+    // Cuts and draw among the n sorted logits, the row's largest, of which top-k keeps k; by the first block.  What is kept
+    // is a prefix of them.
     template <typename W>
-    __device__ __noinline__ static int64_t finish(Row r, uint32_t n, uint32_t k, u64 total, Rule rule, W weigh) {
+    __device__ __noinline__ static int64_t finish(Row r, uint32_t n, uint32_t k, Rule rule, W weigh) {
         Shared& sh = r.sh;
         const int tid = r.tid;
         constexpr uint32_t ROUND = 2 * THREADS;  // two entries per thread at a time
-        if (k > 0 && k < n) n = k;
+        if (k < n) n = k;
         const auto weight = [&](uint32_t i, int word) {  // word: where the key is
             return i < n ? weigh((uint32_t)(sh.sorted[i] >> (32 * word))) : 0ull;
         };
-        if (k > 0 && rule.top_p < 1.0) {
-            total = 0;
+        u64 total = 0;
+        if (rule.top_p < 1.0)
             for (uint32_t base = 0; base < n; base += ROUND) {
                 u64 a = weight(base + 2 * tid, 1), b = weight(base + 2 * tid + 1, 1);
                 total += r.scan_pairs(a, b);
             }
-        }
         const u64 goal = rule.top_p < 1.0 ? share_of(rule.top_p, total) : ~0ull;
         // by index from here on: the largest inverted index first
         const auto by_index = [](u64 e) { return e << 32 | e >> 32; };
@@ -677,6 +690,68 @@ struct Row {
         __syncthreads();
         return (int64_t)sh.found[3];
     }
+    // The cut among the n sorted logits: down to where their running sum, which starts with `before`, stays below `goal`.
+    // At least one does, unless the logits change meanwhile.
+    template <typename W>
+    __device__ __forceinline__ Cut cut_sorted(uint32_t n, u64 before, u64 goal, W weight) {
+        if (rank == 0) {
+            uint32_t kept = 0;
+            for (uint32_t base = 0; base < n; base += 2 * THREADS) {
+                const uint32_t i = base + 2 * tid;
+                const u64 w0 = i < n ? weight((uint32_t)(sh.sorted[i] >> 32)) : 0ull;
+                const u64 w1 = i + 1 < n ? weight((uint32_t)(sh.sorted[i + 1] >> 32)) : 0ull;
+                u64 upto0 = w0, upto1 = w1;
+                const u64 round = scan_pairs(upto0, upto1);
+                kept += __syncthreads_count(i < n && before + upto0 - w0 < goal) +
+                        __syncthreads_count(i + 1 < n && before + upto1 - w1 < goal);
+                before += round;
+            }
+            if (tid == 0) sh.found[3] = sh.sorted[kept > 0 ? kept - 1 : 0];
+        }
+        barrier();
+        const u64 last = ranks > 1 ? *cluster.map_shared_rank(&sh.found[3], 0) : sh.found[3];
+        barrier();
+        return Cut{(uint32_t)(last >> 32), ~(uint32_t)last};
+    }
+    // cut_in among the logits in the blocks' lists, which hold step `at` and all above.  Key 0 when too many share the step.
+    template <typename W, typename S>
+    __device__ __noinline__ static Cut cut_in_list(Row r, int at, u64 before, u64 goal, W weight, S coarse) {
+        Shared& sh = r.sh;
+        if (r.tid == 0) sh.part_count = 0;
+        __syncthreads();
+        for (uint32_t i = r.tid; i < sh.list_count; i += THREADS) {
+            const u64 entry = sh.list[i];
+            if (coarse((uint32_t)(entry >> 32)) == at) sh.part[atomicAdd(&sh.part_count, 1u)] = entry;
+        }
+        r.barrier();
+        const uint32_t n = r.gather(true);
+        return n <= LIST ? r.cut_sorted(n, before, goal, weight) : Cut{0u, 0u};
+    }
+    // The draw among the logits in the blocks' lists that `cut` holds and that weigh no less than `least`: the run of
+    // indexes, one of 2048 at most, in which the running sum first exceeds the point for u.
+    struct Drawn {
+        uint32_t from, to;
+        u64 point;  // what is left of it there
+    };
+    template <typename W>
+    __device__ __noinline__ static Drawn draw_in_list(Row r, uint32_t V, Cut cut, u64 least, double u, W weigh) {
+        Shared& sh = r.sh;
+        int width = 0;
+        while (((V - 1) >> width) >= BINS) ++width;
+        r.clear_histogram();
+        for (uint32_t i = r.tid; i < sh.list_count; i += THREADS) {
+            const u64 entry = sh.list[i];
+            const uint32_t key = (uint32_t)(entry >> 32), index = ~(uint32_t)entry;
+            const u64 w = weigh(key);
+            if (cut.holds(key, index) && w >= least) r.add_weight((int)(index >> width), w);
+        }
+        int at;
+        u64 before, total, goal;
+        r.find_step([u](u64 all) { return point_of(u, all) + 1; }, at, before, total, goal);
+        const uint32_t most = (V - 1) >> width;
+        const uint32_t from = ((uint32_t)at < most ? (uint32_t)at : most) << width, last = from + ((1u << width) - 1);
+        return Drawn{from, last < V ? last + 1 : V, goal - 1 - before};
+    }
     // The cut in step `at`, before which the members weigh `before`, at which the sum of weight(key) over the members, in
     // descending order, stays below `goal`.
     template <typename M, typename W, typename S>
@@ -685,33 +760,15 @@ struct Row {
     }
     template <typename M, typename W, typename S>
     __device__ __forceinline__ Cut cut_here(int at, u64 before, u64 goal, M member, W weight, S coarse) {
-        Cut out;
-        const uint32_t n = collect([=](uint32_t i, float l) {
+        const bool fits = collect([=](uint32_t i, float l) {
             const uint32_t key = key_of(l);
             return member(i, key) && coarse(key) == at;
         });
-        if (n <= LIST) {
-            if (rank == 0) {
-                uint32_t kept = 0;
-                for (uint32_t base = 0; base < n; base += 2 * THREADS) {
-                    const uint32_t i = base + 2 * tid;
-                    const u64 w0 = i < n ? weight((uint32_t)(sh.sorted[i] >> 32)) : 0ull;
-                    const u64 w1 = i + 1 < n ? weight((uint32_t)(sh.sorted[i + 1] >> 32)) : 0ull;
-                    u64 upto0 = w0, upto1 = w1;
-                    const u64 round = scan_pairs(upto0, upto1);
-                    kept += __syncthreads_count(i < n && before + upto0 - w0 < goal) +
-                            __syncthreads_count(i + 1 < n && before + upto1 - w1 < goal);
-                    before += round;
-                }
-                if (tid == 0) sh.found[3] = sh.sorted[kept - 1];  // the step holds the border: at least one is kept
-            }
-            barrier();
-            const u64 last = ranks > 1 ? *cluster.map_shared_rank(&sh.found[3], 0) : sh.found[3];
-            out.key = (uint32_t)(last >> 32);
-            out.last = ~(uint32_t)last;
-            barrier();
-            return out;
+        if (fits) {
+            const uint32_t n = gather(false);
+            if (n <= LIST) return cut_sorted(n, before, goal, weight);
         }
+        Cut out;
         // very many in one step: narrow their keys down to one
         u64 least = ~0ull, most = 0;
         each_key([&](uint32_t i, uint32_t key) {
@@ -839,74 +896,73 @@ sample_kernel(const T* __restrict__ logits, const __grid_constant__ Job job, int
     const auto step_of = [distance](float l) { return l == INFINITY ? 0 : (int)fminf(distance(l), (float)(BINS - 1)); };
     const auto coarse = [step_of](uint32_t key) { return step_of(logit_of(key)); };
     const auto within = [distance](float l, float behind) { return distance(l) < behind || l == INFINITY; };
-    const auto done = [&](uint32_t n, uint32_t k, u64 total) {
-        if (rank == 0) {
-            const int64_t id = Row<T>::finish(r, n, k, total, rule, weigh);
-            if (tid == 0) job.out[row] = id;
-        }
-        r.barrier();  // nobody leaves while others read its numbers
-    };
     // min-p keeps nothing behind this step; one step more for the rounding of the distance
     const double ratio = (double)rule.least / (double)(1ull << job.shift);
     const int last_step = rule.least > 0 && !weigh.infinite ? (int)fmin(-log(ratio) * 32.0 + 2.0, BINS - 1.0) : BINS - 1;
     Cut cut{1u, FULL};  // everything but key 0
     bool cut_found = false;
+    bool listed = false;  // the blocks' lists hold all that can be drawn
     if (rule.top_k > 0 && rule.top_k <= LIST) {
         int at;
         u64 before, total, goal;
-        uint32_t upto;
         r.clear_histogram();
         r.each([&](uint32_t, float l) {
             if (l > -INFINITY) atomicAdd(&sh.low[step_of(l)], 1u);
         });
         const u64 k = (u64)rule.top_k;
-        const bool cuts = r.find_step([k](u64) { return k; }, at, before, total, goal, upto);
+        const bool cuts = r.find_step([k](u64) { return k; }, at, before, total, goal);
         const float behind = cuts && at < BINS - 1 ? (float)(at + 1) : INFINITY;
-        const uint32_t n = r.collect([within, behind](uint32_t, float l) { return within(l, behind); });
-        if (n <= LIST) return done(n, (uint32_t)rule.top_k, 0);
+        if (r.collect([within, behind](uint32_t, float l) { return within(l, behind); })) {
+            const uint32_t n = r.gather(false);
+            if (n <= LIST) {
+                if (rank == 0) {
+                    const int64_t id = Row<T>::finish(r, n, (uint32_t)rule.top_k, rule, weigh);
+                    if (tid == 0) job.out[row] = id;
+                }
+                r.barrier();  // nobody leaves while others read its numbers
+                return;
+            }
+        }
     } else if (rule.top_k == 0 && rule.top_p < 1.0) {
         int at;
         u64 before, total, goal;
-        uint32_t upto;
         r.clear_histogram();
         // lighter than (1 - p) / V of the largest: together no more than 1 - p of the total, so the border lies above them
         const float light = (float)fmin(log((double)job.V / (1.0 - rule.top_p)) * 32.0 + 2.0, (double)(BINS - 1));
         u64 tail = 0;
         r.each4([&](uint32_t, uint32_t, const float (&l)[4]) {
             u64 w[4];
-            bool heavy[4];
+            int b[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 w[e] = weigh.of(l[e]);
-                heavy[e] = within(l[e], light);
-                tail += heavy[e] ? 0ull : w[e];
+                b[e] = 0;
+                if (within(l[e], light)) b[e] = step_of(l[e]);
+                else {
+                    tail += w[e];
+                    w[e] = 0;
+                }
             }
-            if (!(heavy[0] | heavy[1] | heavy[2] | heavy[3])) return;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if (!heavy[e]) continue;
-                const int b = step_of(l[e]);
-                r.add_weight(b, w[e]);
-                atomicAdd(&sh.count[b], 1u);
-            }
+            r.add_weights(b, w);
         });
         tail = warp_sum(tail);
         if (r.lane == 0 && tail > 0) atomicAdd(&sh.tail, tail);
         const double share = rule.top_p;
-        if (r.find_step([share](u64 all) { return share_of(share, all); }, at, before, total, goal, upto)) {
+        if (r.find_step([share](u64 all) { return share_of(share, all); }, at, before, total, goal)) {
             const int end = at < last_step ? at + 1 : last_step + 1;
             const float behind = end < BINS ? (float)end : INFINITY;
-            if (upto <= LIST || at > last_step) {
-                const uint32_t n = r.collect([within, behind](uint32_t, float l) { return within(l, behind); });
-                if (n <= LIST) return done(n, 0, total);
+            listed = r.collect([within, behind](uint32_t, float l) { return within(l, behind); });
+            if (listed && at <= last_step) {
+                cut = Row<T>::cut_in_list(r, at, before, goal, weigh, coarse);
+                listed = cut.key != 0u;
             }
-            cut = Row<T>::cut_in(r, at, before, goal, [](uint32_t, uint32_t key) { return key != 0u; }, weigh, coarse);
+            if (!listed)
+                cut = Row<T>::cut_in(r, at, before, goal, [](uint32_t, uint32_t key) { return key != 0u; }, weigh, coarse);
             cut_found = true;
         }
     } else if (rule.top_k == 0 && rule.least > 0) {
         const float behind = last_step + 1 < BINS ? (float)(last_step + 1) : INFINITY;
-        const uint32_t n = r.collect([within, behind](uint32_t, float l) { return within(l, behind); });
-        if (n <= LIST) return done(n, 0, 0);
+        listed = r.collect([within, behind](uint32_t, float l) { return within(l, behind); });
     }
     // many candidates: the cuts one after the other, then the draw over the row
     if (rule.top_k > 0) {
@@ -924,7 +980,7 @@ sample_kernel(const T* __restrict__ logits, const __grid_constant__ Job job, int
                   [p](u64 total) { return share_of(p, total); }, c))
             cut = c;
     }
-    // the draw: every warp sums a run of the slice, the run that holds the point is cut up again
+    // the draw: from the lists, if they hold all; else every warp sums a run of the slice, the run that holds the point is cut up again
     const u64 least = rule.least;
     const float border = cut.last == FULL ? -INFINITY : logit_of(cut.key);  // most logits are told by one comparison
     const auto kept = [&](uint32_t i, float l) {
@@ -933,8 +989,24 @@ sample_kernel(const T* __restrict__ logits, const __grid_constant__ Job job, int
     };
     uint32_t lo = from, hi = to;
     u64 point = 0;
+    if (listed) {
+        const auto drawn = Row<T>::draw_in_list(r, V, cut, least, rule.u, weigh);
+        lo = drawn.from;
+        hi = drawn.to;
+        point = drawn.point;
+    }
     __syncthreads();
-    for (int level = 0;; ++level) {
+    const bool here = !listed || rank == 0;
+    for (int level = listed ? 1 : 0; here; ++level) {
+        if (level > 0 && hi - lo <= 32) {
+            if (r.warp == 0) {
+                const u64 mine = lo + r.lane < hi ? kept(lo + r.lane, dl_to_float(r.logits[lo + r.lane])) : 0ull;
+                const u64 upto = warp_inclusive(mine, r.lane);
+                const uint32_t hit = __ballot_sync(FULL, upto > point);
+                if (r.lane == 0) job.out[row] = (int64_t)lo + __ffs(hit) - 1;
+            }
+            break;
+        }
         const uint32_t run = (hi - lo + WARPS - 1) / WARPS;
         const uint32_t begin = lo + r.warp * run < hi ? lo + r.warp * run : hi, end = begin + run < hi ? begin + run : hi;
         u64 sum = 0;
@@ -979,15 +1051,6 @@ sample_kernel(const T* __restrict__ logits, const __grid_constant__ Job job, int
         lo = lo + at * run;
         hi = lo + run < hi ? lo + run : hi;
         __syncthreads();
-        if (hi - lo <= 32) {
-            if (r.warp == 0) {
-                const u64 mine = lo + r.lane < hi ? kept(lo + r.lane, dl_to_float(r.logits[lo + r.lane])) : 0ull;
-                const u64 upto = warp_inclusive(mine, r.lane);
-                const uint32_t hit = __ballot_sync(FULL, upto > point);
-                if (r.lane == 0) job.out[row] = (int64_t)lo + __ffs(hit) - 1;
-            }
-            break;
-        }
     }
     r.barrier();  // nobody leaves while others read its numbers
 }
@@ -1004,8 +1067,8 @@ int launch_sample(const void* logits, const Job& job, cudaStream_t s) {
         else sample_small_kernel<T, 16><<<(unsigned)blocks, 128, 0, s>>>(src, job);
         return dl_launch_status();
     }
-    // more blocks per row while they have 8192 classes each and all are resident together: every block has its own
-    // histograms, lists and barriers to go through
+    // more blocks per row while they keep 8192 classes each and there is an SM for every one: each has its own histograms,
+    // lists and barriers to go through (64 x 32000, top-p: 35 us with two blocks a row; one row of 131072: 48 with eight)
     int ranks = 1;
     while (ranks < MAX_CLUSTER && job.V >= (int64_t)16384 * ranks && job.R * ranks <= DL_NUM_SMS) ranks *= 2;
     if (job.R * ranks > 0x7fffffff) return DL_ERR_TOO_LARGE;
