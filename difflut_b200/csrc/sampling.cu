@@ -23,7 +23,7 @@
 // eight when there are few rows.  Each pass reads the logits again: after the first they come from L2.
 //
 // Measured: 64 rows of 32000 bf16 logits, T .8: 5.8 us for the largest, 19 us to draw from all, 20 us with top-k 50 and top-p
-// .95, 35 us with top-p .95 alone.  Of the latter the histogram of the weights takes 11 us, the two searches in histograms
+// .95, 35 us with top-p .95 alone (8 rows: 31).  Of the latter the histogram of the weights takes 11 us, the two searches in histograms
 // 3 us each, collecting 6 us: latency of passes with one or two rounds of loads per thread, not bandwidth (the 4 MB are read
 // in a microsecond).  256 rows of 65536 fp32 logits with top-p .9 and min-p .01: 88 us, 43 of them the histogram, bound by
 // double precision and shared-memory atomics (the 67 MB take 10).
@@ -165,11 +165,15 @@ __device__ __forceinline__ u64 warp_inclusive(u64 v, int lane) {
 }
 
 // ------------------------------------------------------------------------------------------ one warp per row
-// Element j * 32 + lane sits in register j: index order is register, then lane.
+// Element j * 32 + lane sits in register j: index order is register, then lane.  The borders of top-k and top-p are found bit
+// by bit of the key: counting 256 keys takes 8 comparisons and one reduction.  What top-k leaves is moved together, since
+// every register of exponentials costs a row eighty double-precision issue slots.  Measured, 8192 rows of 256 fp32 logits,
+// top-k 40: 15.6 us (17.9 before moving; reading the logits takes 1.3): issue-bound, a third of it the search.
 template <typename T, int PER>
 __global__ void __launch_bounds__(128)
 sample_small_kernel(const T* __restrict__ logits, const __grid_constant__ Job job) {
     __shared__ double table[TABLE];
+    __shared__ uint2 moved[4][PER * 32];
     const int lane = threadIdx.x & 31;
     fill_table(table, job.shift, threadIdx.x, blockDim.x);
     __syncthreads();
@@ -191,6 +195,10 @@ sample_small_kernel(const T* __restrict__ logits, const __grid_constant__ Job jo
         return;
     }
     uint32_t member = 0;  // bit j: element j is still in
+    uint32_t index[PER];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) index[j] = j * 32 + lane;
+    int rounds = PER;  // registers that hold members
 #pragma unroll
     for (int j = 0; j < PER; ++j) member |= (key[j] != 0u) << j;
     if (rule.greedy) {
@@ -224,13 +232,27 @@ sample_small_kernel(const T* __restrict__ logits, const __grid_constant__ Job jo
 #pragma unroll
             for (int j = 0; j < PER; ++j) above += key[j] > t;
             int ties = (int)rule.top_k - __reduce_add_sync(FULL, above);  // of the keys equal to t these are in
-            member = 0;
+            // the members move up to the first registers, still in order of their indexes: they are few mostly
+            int kept = 0;
 #pragma unroll
             for (int j = 0; j < PER; ++j) {
                 const uint32_t equal = __ballot_sync(FULL, key[j] == t);
                 const bool in = key[j] > t || (key[j] == t && __popc(equal & ((1u << lane) - 1)) < ties);
                 ties -= __popc(equal);
-                member |= (uint32_t)in << j;
+                const uint32_t all = __ballot_sync(FULL, in);
+                if (in) moved[threadIdx.x >> 5][kept + __popc(all & ((1u << lane) - 1))] = make_uint2(key[j], j * 32 + lane);
+                kept += __popc(all);
+            }
+            __syncwarp();
+            rounds = (kept + 31) / 32;
+            member = 0;
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                const int i = j * 32 + lane;
+                const uint2 m = i < kept ? moved[threadIdx.x >> 5][i] : make_uint2(0u, 0u);
+                key[j] = m.x;
+                index[j] = m.y;
+                member |= (uint32_t)(i < kept) << j;
             }
         }
     }
@@ -238,7 +260,8 @@ sample_small_kernel(const T* __restrict__ logits, const __grid_constant__ Job jo
     u64 w[PER], mine = 0;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-        w[j] = member >> j & 1 ? weigh(key[j]) : 0ull;
+        w[j] = 0ull;
+        if (j < rounds) w[j] = member >> j & 1 ? weigh(key[j]) : 0ull;
         mine += w[j];
     }
     u64 total = warp_sum(mine);
@@ -292,7 +315,7 @@ sample_small_kernel(const T* __restrict__ logits, const __grid_constant__ Job jo
         const u64 upto = run + warp_inclusive(w[j], lane);
         const uint32_t hit = __ballot_sync(FULL, upto > point);
         if (hit) {
-            if (lane == 0) job.out[row] = j * 32 + __ffs(hit) - 1;
+            if (lane == __ffs(hit) - 1) job.out[row] = index[j];
             return;
         }
         run = __shfl_sync(FULL, upto, 31);
@@ -1067,10 +1090,11 @@ int launch_sample(const void* logits, const Job& job, cudaStream_t s) {
         else sample_small_kernel<T, 16><<<(unsigned)blocks, 128, 0, s>>>(src, job);
         return dl_launch_status();
     }
-    // more blocks per row while they keep 8192 classes each and there is an SM for every one: each has its own histograms,
-    // lists and barriers to go through (64 x 32000, top-p: 35 us with two blocks a row; one row of 131072: 48 with eight)
+    // twice as many blocks per row while they keep 6144 classes each and there is an SM for every one: each has its own
+    // histograms, lists and barriers to go through (top-p .95, 8 x 32000: 31 us with four blocks a row, 35 with two or eight;
+    // 64 x 32000: 35 us with two, 41 with four; 1 x 8192: 18 with one, 23 with two)
     int ranks = 1;
-    while (ranks < MAX_CLUSTER && job.V >= (int64_t)16384 * ranks && job.R * ranks <= DL_NUM_SMS) ranks *= 2;
+    while (ranks < MAX_CLUSTER && job.V >= (int64_t)12288 * ranks && job.R * ranks * 2 <= DL_NUM_SMS) ranks *= 2;
     if (job.R * ranks > 0x7fffffff) return DL_ERR_TOO_LARGE;
     const int vectors = dl_address(logits) % 16 == 0 && (job.R == 1 || job.pitch * (int64_t)sizeof(T) % 16 == 0);
     const uint32_t slice = (uint32_t)(dl_ceil_div(dl_ceil_div(job.V, ranks), 8) * 8);  // whole vectors
