@@ -130,6 +130,7 @@ DL_EXPORT int dl_dropout(const void* x, void* out, int64_t count, int64_t dtype,
     DL_REQUIRE(x && out);
     DL_REQUIRE_ALIGNED(x, dl_dtype_size(dtype));
     DL_REQUIRE_ALIGNED(out, dl_dtype_size(dtype));
+    DL_REQUIRE_ALIGNED(counter, 8);
     cudaStream_t s = dl_cast(stream);
     const uint64_t threshold = (uint64_t)(p * 4294967296.0 + 0.5);  // 0 .. 2^32
     if (threshold > 0xFFFFFFFFull)  // everything is dropped; 0.0 is all zero bits in every type
@@ -152,6 +153,8 @@ DL_EXPORT int dl_dropout(const void* x, void* out, int64_t count, int64_t dtype,
 
 DL_EXPORT int dl_counter_draw(int64_t* counter, int64_t* drawn, dl_stream_t stream) {
     DL_REQUIRE(counter && drawn && counter != drawn);
+    DL_REQUIRE_ALIGNED(counter, 8);
+    DL_REQUIRE_ALIGNED(drawn, 8);
     counter_draw_kernel<<<1, 1, 0, dl_cast(stream)>>>(counter, drawn);
     return dl_launch_status();
 }

@@ -903,6 +903,10 @@ DL_EXPORT int dl_group_norm(const void* x, const void* weight, const void* bias,
     DL_REQUIRE_ALIGNED(scratch, 16);
     DL_REQUIRE_ALIGNED(x, dl_dtype_size(dtype));
     DL_REQUIRE_ALIGNED(y, dl_dtype_size(dtype));
+    DL_REQUIRE_ALIGNED(weight, dl_dtype_size(param_dtype));
+    DL_REQUIRE_ALIGNED(bias, dl_dtype_size(param_dtype));
+    DL_REQUIRE_ALIGNED(mean, 4);
+    DL_REQUIRE_ALIGNED(rstd, 4);
     p.weight = weight;
     p.bias = bias;
     p.param_dtype = (int)param_dtype;
@@ -933,6 +937,12 @@ DL_EXPORT int dl_group_norm_bwd(const void* x, const void* g, const void* weight
     DL_REQUIRE_ALIGNED(x, dl_dtype_size(dtype));
     DL_REQUIRE_ALIGNED(g, dl_dtype_size(dtype));
     DL_REQUIRE_ALIGNED(gx, dl_dtype_size(dtype));
+    DL_REQUIRE_ALIGNED(weight, dl_dtype_size(param_dtype));
+    DL_REQUIRE_ALIGNED(bias, dl_dtype_size(param_dtype));
+    DL_REQUIRE_ALIGNED(gweight, dl_dtype_size(param_dtype));
+    DL_REQUIRE_ALIGNED(gbias, dl_dtype_size(param_dtype));
+    DL_REQUIRE_ALIGNED(mean, 4);
+    DL_REQUIRE_ALIGNED(rstd, 4);
     DL_REQUIRE_ALIGNED(scratch, 16);
     p.weight = weight;
     p.bias = bias;

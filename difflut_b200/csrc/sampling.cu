@@ -77,6 +77,7 @@ struct Rule {
         const int64_t k = j.set.top_k ? (int64_t)j.set.top_k[r] : j.set.top_k_all;
         top_k = k > 0 && k < j.V ? k : 0;
         top_p = j.set.top_p ? (double)j.set.top_p[r] : j.set.top_p_all;
+        if (top_p < 0.0) top_p = 0.0;  // NaN stays and keeps all
         double m = j.set.min_p ? (double)j.set.min_p[r] : j.set.min_p_all;
         m = m > 0.0 ? (m < 1.0 ? m : 1.0) : 0.0;
         least = (u64)ceil(m * (double)(1ull << j.shift));
@@ -168,7 +169,7 @@ __device__ __forceinline__ u64 warp_inclusive(u64 v, int lane) {
 // Element j * 32 + lane sits in register j: index order is register, then lane.  The borders of top-k and top-p are found bit
 // by bit of the key: counting 256 keys takes 8 comparisons and one reduction.  What top-k leaves is moved together, since
 // every register of exponentials costs a row eighty double-precision issue slots.  Measured, 8192 rows of 256 fp32 logits,
-// top-k 40: 15.6 us (17.9 before moving; reading the logits takes 1.3): issue-bound, a third of it the search.
+// top-k 40: 15.6 us (17.9 before moving; reading the logits takes 1.3): issue-bound.
 template <typename T, int PER>
 __global__ void __launch_bounds__(128)
 sample_small_kernel(const T* __restrict__ logits, const __grid_constant__ Job job) {
@@ -1128,6 +1129,11 @@ DL_EXPORT int dl_sample_rows(const void* logits, int64_t pitch, const void* u, i
     DL_REQUIRE(logits && u && out && (R == 1 || pitch >= 0));
     DL_REQUIRE_ALIGNED(logits, dl_dtype_size(dtype));
     DL_REQUIRE_ALIGNED(u, u_double ? 8 : 4);
+    DL_REQUIRE_ALIGNED(temperature, 4);
+    DL_REQUIRE_ALIGNED(top_k, 4);
+    DL_REQUIRE_ALIGNED(top_p, 4);
+    DL_REQUIRE_ALIGNED(min_p, 4);
+    DL_REQUIRE_ALIGNED(out, 8);
     Job job;
     job.u = u;
     job.u_double = u_double != 0;

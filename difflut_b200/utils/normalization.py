@@ -27,8 +27,11 @@ def _check_activation(activation) -> int:
 def _scratch_bytes(N, S, C, G, code):
     """Workspace of (the forward, the backward pass)."""
     lib = _native.lib()
-    return (int(lib.dl_group_norm_scratch_bytes(N, S, C, G, code)),
-            int(lib.dl_group_norm_bwd_scratch_bytes(N, S, C, G, code)))
+    sizes = (int(lib.dl_group_norm_scratch_bytes(N, S, C, G, code)),
+             int(lib.dl_group_norm_bwd_scratch_bytes(N, S, C, G, code)))
+    if min(sizes) < 0:
+        raise RuntimeError(f"group_norm of {N} x {S} x {C} values in {G} groups is not supported")
+    return sizes
 
 
 def _address(t):

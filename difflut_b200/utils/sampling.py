@@ -12,6 +12,10 @@ def _setting(name, value, rows, dtype, low, high, low_open=False):
     if isinstance(value, torch.Tensor):
         if value.shape != (rows,):
             raise ValueError(f"{name} must be a number or have shape ({rows},), got {tuple(value.shape)}")
+        if not dtype.is_floating_point:
+            if value.is_floating_point() or value.is_complex():
+                raise ValueError(f"{name} must hold integers, got {value.dtype}")
+            value = value.clamp(max=torch.iinfo(dtype).max) if value.dtype == torch.int64 else value
         return value.to(dtype).contiguous(), None
     number = isinstance(value, (int, float) if dtype.is_floating_point else int) and not isinstance(value, bool)
     if not number or not (low < value if low_open else low <= value) or not value <= high:
@@ -31,8 +35,8 @@ def sample_logits(logits: torch.Tensor, u: torch.Tensor, temperature: Union[floa
     ascending order whose running sum of kept weights exceeds u times their total.  Equal logits rank by index, lowest
     first.  NaN and -inf are never taken; a row without any other logit gives -1.
 
-    Every setting is a number or a tensor (R) of its own for each row (float32; int32 for top_k; other types are
-    converted).  u is float32 or float64.  logits (float32, bfloat16 or float16) may be a view with any distance between
+    Every setting is a number or a tensor (R) of its own for each row (float32; int32 for top_k; other float
+    or integer types are converted).  u is float32 or float64.  logits (float32, bfloat16 or float16) may be a view with any distance between
     its rows.  The result does not depend on the order of additions: the same id on every run."""
     code = _native.dtype_code(logits, "logits")
     if logits.dim() != 2 or logits.shape[1] == 0:

@@ -669,6 +669,31 @@ def test_sampling_settings_per_row(V):
     assert sample_logits(x, u, temperature=T.double(), top_k=k.long(), top_p=p, min_p=m).tolist() == got
 
 
+@pytest.mark.parametrize("V", [300, 2000])
+def test_sampling_settings_per_row_far_outside_their_range(V):
+    """A share far below 0 keeps the first class like 0 does, a count past 32 bits keeps all."""
+    x, u = _logits(4, V, torch.float32), _u(4)
+    p = torch.tensor([-1e9, -3e38, -math.inf, -0.5], device=DEV)
+    assert sample_logits(x, u, top_p=p).tolist() == x.argmax(1).tolist()
+    k = torch.tensor([2 ** 32 + 1, 2 ** 31, 2 ** 62, -2 ** 40], device=DEV)
+    assert sample_logits(x, u, top_k=k).tolist() == sample_logits(x, u).tolist()
+
+
+@pytest.mark.parametrize("V", [9000, 24600, 70000])
+@pytest.mark.parametrize("heavy", [1, 40, 512, 513, 1500, 2047, 2100, 5000, 8800])
+def test_sampling_candidates_around_the_lengths_of_the_lists(V, heavy):
+    """`heavy` logits stand out: equal ones, ones within a step of the histogram, ones over many steps.  Borders fall among
+    them, in lists that hold them in one block, only in several, or not at all."""
+    g = torch.Generator().manual_seed(V + heavy)
+    x = _normal(3, V, seed=V) - 30.0
+    places = torch.stack([torch.randperm(V, generator=g)[:heavy] for _ in range(3)]).to(DEV)
+    spread = torch.tensor([0.0, 0.02, 3.0], device=DEV)[:, None]
+    x.scatter_(1, places, spread * _normal(3, heavy, seed=heavy))
+    for i, (T, k, p, m) in enumerate([(1.0, 0, 0.63, 0.0), (1.0, 0, 0.999, 0.4), (1.0, 0, 1.0, 0.01), (1.0, 1000, 0.7, 0.0),
+                                      (1.0, 2048, 1.0, 0.0), (1.0, 2049, 0.9, 0.1), (0.9, 0, 1.0 - 1e-12, 0.0)]):
+        _check_samples(x, _u(3, i), T, k, p, m)
+
+
 @pytest.mark.parametrize("V", [200, 2000, 20000])
 def test_sampling_frequencies(V):
     """Random numbers on an even grid: every class comes up as often as its weight says, give or take one at each end."""

@@ -119,6 +119,7 @@ def test_dropout_entry_points_refuse():
     assert lib.dl_dropout(None, None, 0, 7, 0.5, 1, 0, None, None) == -1
     assert lib.dl_dropout(6, 8, 4, 0, 0.5, 1, 0, None, None) == -4
     assert lib.dl_counter_draw(None, None, None) == -1
+    assert lib.dl_dropout(8, 8, 4, 0, 0.5, 1, 0, 12, None) == -4 and lib.dl_counter_draw(8, 12, None) == -4
 
 
 # ---------------------------------------------------------------------------------------------- group norm
@@ -175,6 +176,22 @@ def test_group_norm_entry_points_refuse():
     assert lib.dl_group_norm_bwd(*([16] * 10), 2, 3, 8, 2, 0, 0, 9, None) == -1
     assert lib.dl_group_norm_bwd(16, 16, None, None, None, 16, 16, 16, 16, 16, 2, 3, 8, 2, 0, 0, 0, None) == -1
     assert lib.dl_group_norm_bwd(*([16] * 9), None, 2, 3, 8, 2, 0, 0, 0, None) == -1
+    for odd in (1, 2, 4, 5):  # weight, bias, mean, rstd
+        args = [16, 16, 16, 16, 16, 16, 16]
+        args[odd] = 18
+        assert lib.dl_group_norm(*args, 2, 3, 8, 2, 0, 0, 0, 1e-5, None) == -4
+    for odd in (2, 3, 4, 5, 7, 8):  # and the parameters' gradients
+        args = [16] * 10
+        args[odd] = 18
+        assert lib.dl_group_norm_bwd(*args, 2, 3, 8, 2, 0, 0, 0, None) == -4
+
+
+def test_group_norm_refuses_sizes_past_its_indexes():
+    from difflut_b200.utils.normalization import _scratch_bytes
+
+    for size in ((1, 1 << 30, 1, 1, 1), (1, 1, 1 << 30, 1, 1)):
+        with pytest.raises(RuntimeError, match="not supported"):
+            _scratch_bytes(*size)
 
 
 # ---------------------------------------------------------------------------------------------- sampling
@@ -194,6 +211,8 @@ def test_sample_logits_refuses():
         sample_logits(x, [0.0] * 3)
     with pytest.raises(ValueError, match="u must"):
         sample_logits(x, u[:2])
+    with pytest.raises(ValueError, match="integers"):
+        sample_logits(x, u, top_k=torch.ones(3))
     nan = float("nan")
     for name, values in (("temperature", (-1.0, nan, "1", True, torch.ones(2))), ("top_k", (-1, 1.5, True, torch.ones(3, 1))),
                          ("top_p", (0.0, 1.1, nan, -0.5)), ("min_p", (-0.1, 1.5, nan))):
@@ -212,7 +231,10 @@ def test_sample_entry_point_refuses():
     assert call(V=0) == -1 and call(R=-1) == -1 and call(dtype=3) == -1 and call(V=1 << 30) == -5
     assert call(T=-1.0) == -1 and call(T=float("nan")) == -1 and call(k=-1) == -1
     assert call(p=0.0) == -1 and call(p=float("nan")) == -1 and call(m=-1.0) == -1 and call(m=1.5) == -1
-    assert call(logits=18) == -4 and call(u=18) == -4
+    assert call(logits=18) == -4 and call(u=18) == -4 and call(out=20) == -4
+    for odd in range(4):
+        t, k, p, m = (18 if odd == i else None for i in range(4))
+        assert f(16, 4, 16, 0, t, 1.0, k, 0, p, 1.0, m, 0.0, 16, 2, 4, 0, None) == -4
 
 
 def test_plain_sampling_form_on_known_answers():
