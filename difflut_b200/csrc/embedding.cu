@@ -11,6 +11,14 @@
 //      every segment that begins in its range; among these blocks others write the zero rows of ids that do not
 //      occur, so each row of gW is written once;
 //   3. segments that go on far behind their range are joined from their fp32 partial sums, in range order.
+//
+// Measured, 65536 tokens of 1024 bf16 features (ids as in text: few frequent, many rare) into a table of 65536 rows:
+//   1. 53 us: the sort takes 36 alone (latency of two passes of a cluster of eight blocks), the lookup beside it reads 35 MB
+//      of rows and writes 134 MB from the other SMs;
+//   2. 52 us for 134 MB of gradients read and 134 MB of table written: 5.2 TB/s, 0.8 of the copy rate.  The rows on
+//      their way to shared memory instead of registers made 69 us 63, neighbouring warps on the slabs of a row 52;
+//   3. 12 us: most blocks find nothing to join, the others wait for a few hundred partial rows.
+// For one step of generation (32 tokens) the lookup is a launch of 1.8 us.
 #include <cooperative_groups.h>
 
 #include "elements.cuh"
@@ -26,7 +34,8 @@ constexpr int SORT_KEYS = 8;  // per thread and tile
 constexpr int SORT_TILE = SORT_KEYS * SORT_THREADS;
 constexpr int SORT_DIGIT_BITS = 9;  // two passes sort tables of up to 2^18 - 1 rows
 constexpr int SORT_BINS = 1 << SORT_DIGIT_BITS;
-constexpr int MAX_CLUSTER = 8;  // 16 (not portable) sort in 32 us instead of 36, but beside a lookup both take 51 us
+constexpr int MAX_CLUSTER = 8;  // 16 (not portable) sort in 32 us instead of 36, but beside a lookup both take as long
+
 // id as stored, or -1 when it is outside [0, V)
 template <typename I>
 __device__ __forceinline__ int64_t checked_id(const I* ids, int64_t t, int64_t V) {

@@ -9,13 +9,20 @@
 // one adds up its sample's (a few hundred numbers) and writes.  Where samples alone fill the GPU a chunk is a sample and
 // one launch does both.  The second reading comes from L2 as far as the tensor fits there.  (Holding a sample in the shared
 // memory of a cluster, so that it is read once, was slower: all blocks load, then all compute, then all store, and each
-// sample costs a cluster barrier: 51 us instead of 46 us forward, 90 instead of 80 us backward for 16 x 4096 x 512 bf16.)
+// sample costs a cluster barrier: 51 us instead of 43 us forward, 90 instead of 73 us backward for 16 x 4096 x 512 bf16.)
 // A thread keeps to its own channels (a vector of W).  Rows without positions (S = 1) take kernels of their own, in which a
 // group is a few lanes of a warp and stays in registers.
 //
 // A thread sums its values and their squares relative to its first one, which is a value of the group: the squares of these
 // offsets add up to no more than the group's own, so what cancels is at most (values per thread) * 2^-24 of the variance.
 // Threads and chunks are joined by their means and squares around them.  No atomics: the same bits on every run.
+//
+// Measured, 16 x 4096 x 512 bf16 with 32 groups and silu (67 MB a tensor): sums 16.5 us (4.1 TB/s), writing 26.7 us
+// (5.0 TB/s read and written; the exponential and the reciprocal keep their pipe 59 % busy); backward sums 34 us
+// (3.9 TB/s), writing 35 us (5.8 TB/s), the parameters' sums 4 us.  8192 rows of 1024 bf16 features, 32 groups, sigmoid
+// (17 MB a tensor, mostly in L2): 13.7 us forward and 21.6 + 3.6 us backward, bound by issue slots (51 %) and the wait for
+// one round of loads.  Maps of 128 x 576 x 32 fp32 (9 MB): 3.9 + 5.6 us forward, 6.7 + 6.2 + 2.2 us backward, mostly the
+// latency of the launches.
 #include <type_traits>
 
 #include "elements.cuh"
@@ -829,7 +836,8 @@ int launch_backward(const void* x, const void* g, const float* mean, const float
     }
     if (cudaPeekAtLastError() != cudaSuccess) return DL_ERR_LAUNCH;
     if (partial != nullptr)
-        norm_params_kernel<<<(unsigned)dl_ceil_div(p.C, PARAM_CHANNELS), PARAM_CHANNELS * PARAM_ROWS, 0, s>>>(partial, parts, p.C, gweight, gbias, p.param_dtype);
+        norm_params_kernel<<<(unsigned)dl_ceil_div(p.C, PARAM_CHANNELS), PARAM_CHANNELS * PARAM_ROWS, 0, s>>>(
+            partial, parts, p.C, gweight, gbias, p.param_dtype);
     return dl_launch_status();
 }
 

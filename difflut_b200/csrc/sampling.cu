@@ -7,26 +7,26 @@
 // Both cuts are one question: down to which (logit, index) does a running sum, of ones or of weights, stay below a
 // target?  It is answered without sorting the row: a histogram over (max - l) / T in 2048 steps of 1/32 finds the step in
 // which the target falls.  The logits in that step and above it are collected in lists in shared memory, and only those of
-// that one step are sorted.  The draw is a histogram as well, of the listed weights over the index, and the 1/2048 of the row
-// in which the point falls is read once more.  (Sorting the whole list by key and then by index took 34 of 48 us for 1900
-// logits.)  For top-k the list is short: it is sorted, and cuts and draw are prefix sums.  Should the lists not hold them,
-// the logits of the step are told apart by histograms over the bits of their keys and, for equal ones, over their index, and
-// the draw goes over the row.
+// that one step are sorted.  The draw is a histogram as well, of the listed weights over the index, and the 1/2048 of
+// the row in which the point falls is read once more.  (Sorting the whole list by key and then by index took 34 of 48 us
+// for 1900 logits.)  For top-k the list is short: it is sorted, and cuts and draw are prefix sums.  Should the lists not
+// hold them, the logits of the step are told apart by histograms over the bits of their keys and, for equal ones, over
+// their index, and the draw goes over the row.
 //
 // A class next to a border must not depend on the order of additions, so weights are whole numbers: exp in double
 // precision, as fixed point with up to 50 fractional bits, chosen so that the sum of a row fits 62 bits.  Integer sums are
-// exact in any order, so shared-memory atomics are harmless here.  The atomics of the weights are what a pass would spend
-// its time on; V classes that weigh less than (1 - p) / V of the largest each cannot hold the border of top-p, and go to a
-// register instead.
+// exact in any order, so shared-memory atomics are harmless here.  V classes that weigh less than (1 - p) / V of the
+// largest each cannot hold the border of top-p: they go to a register instead.
 //
 // Rows of up to 512 classes take one warp and registers; longer ones a block of 512 threads, or a cluster of up to
 // eight when there are few rows.  Each pass reads the logits again: after the first they come from L2.
 //
-// Measured: 64 rows of 32000 bf16 logits, T .8: 5.8 us for the largest, 19 us to draw from all, 20 us with top-k 50 and top-p
-// .95, 35 us with top-p .95 alone (8 rows: 31).  Of the latter the histogram of the weights takes 11 us, the two searches in histograms
-// 3 us each, collecting 6 us: latency of passes with one or two rounds of loads per thread, not bandwidth (the 4 MB are read
-// in a microsecond).  256 rows of 65536 fp32 logits with top-p .9 and min-p .01: 88 us, 43 of them the histogram, bound by
-// double precision and shared-memory atomics (the 67 MB take 10).
+// Measured: 64 rows of 32000 bf16 logits, T .8: 5.8 us for the largest, 19 us to draw from all, 20 us with top-k 50 and
+// top-p .95, 35 us with top-p .95 alone (8 rows: 31).  Of the latter the histogram of the weights takes 11 us, the two
+// searches in histograms 3 us each, collecting 6 us: latency of passes with few rounds of loads per thread, not bandwidth
+// (the 4 MB are read in a microsecond).  256 rows of 65536 fp32 logits with top-p .9 and min-p .01: 88 us, 43 of them the
+// histogram, bound by issue slots (51 % over all SMs, of which 108 hold two rows and 40 one; the double-precision pipe is
+// 12 % busy, the data pipe of shared memory 40 %); reading the 67 MB once takes 10.
 #include <cooperative_groups.h>
 
 #include "elements.cuh"
@@ -1004,7 +1004,8 @@ sample_kernel(const T* __restrict__ logits, const __grid_constant__ Job job, int
                   [p](u64 total) { return share_of(p, total); }, c))
             cut = c;
     }
-    // the draw: from the lists, if they hold all; else every warp sums a run of the slice, the run that holds the point is cut up again
+    // the draw: from the lists, if they hold all; else every warp sums a run of the slice, and the run that holds the point
+    // is cut up again
     const u64 least = rule.least;
     const float border = cut.last == FULL ? -INFINITY : logit_of(cut.key);  // most logits are told by one comparison
     const auto kept = [&](uint32_t i, float l) {
