@@ -100,7 +100,8 @@ struct SortShared {
     uint16_t warp_count[SORT_WARPS][SORT_BINS];  // first counts, then offsets inside the tile
     uint32_t totals[SORT_BINS];                  // of the block's run; read by the other blocks
     uint32_t base[SORT_BINS];                    // where the block's next token with this digit goes
-    uint32_t warp_sum[SORT_BINS / 32];
+    uint32_t start[SORT_BINS];                   // where its first one lies among the block's own, by digit
+    uint32_t warp_sum[2][SORT_BINS / 32];
 };
 
 // The lanes that hold the same digit (NO_KEY included), by one vote per bit: the match instruction walks the distinct
@@ -198,12 +199,28 @@ embedding_sorting_kernel(Lookup<T, I> lookup, int64_t padding, uint2* a, uint2* 
             for (int j = 0; j < SORT_KEYS; ++j)
                 if (digit[j] != NO_KEY) {
                     const uint32_t at = sh.base[digit[j]] + sh.warp_count[warp][digit[j]] + slot[j];
-                    if (one_tile && pass < passes - 1)
+                    if (one_tile)
                         cluster.map_shared_rank(sh.tile, at >> per_log2)[at & (uint32_t)(per - 1)] = entry[j];
                     else
                         dst[at] = entry[j];
                     if (pass == passes - 1 && entry[j].x < V) present[entry[j].x] = 1;
                 }
+        };
+        // the last pass of a run of one tile: put in order on the chip first, so that neighbouring threads write
+        // neighbouring entries, and only the first of equal ids marks it
+        auto write_tile = [&]() {
+#pragma unroll
+            for (int j = 0; j < SORT_KEYS; ++j)
+                if (digit[j] != NO_KEY)
+                    sh.tile[sh.start[digit[j]] + sh.warp_count[warp][digit[j]] + slot[j]] = entry[j];
+            __syncthreads();
+            const int n = (int)(hi - lo);
+            for (int i = tid; i < n; i += SORT_THREADS) {
+                const uint2 e = sh.tile[i];
+                const uint32_t d = (e.x >> shift) & mask;
+                dst[sh.base[d] + i - sh.start[d]] = e;
+                if (e.x < V && (i == 0 || sh.tile[i - 1].x != e.x)) present[e.x] = 1;
+            }
         };
 
         if (one_tile) {
@@ -221,7 +238,7 @@ embedding_sorting_kernel(Lookup<T, I> lookup, int64_t padding, uint2* a, uint2* 
             }
         }
         cluster.sync();
-        uint32_t all = 0, before = 0, inclusive = 0;
+        uint32_t all = 0, before = 0, inclusive = 0, own = 0, own_inclusive = 0;
         if (tid < SORT_BINS) {
             if (tid < bins) {
 #pragma unroll
@@ -230,23 +247,38 @@ embedding_sorting_kernel(Lookup<T, I> lookup, int64_t padding, uint2* a, uint2* 
                     all += c;
                     if (r < rank) before += c;
                 }
+                own = sh.totals[tid];
             }
             inclusive = all;
+            own_inclusive = own;
 #pragma unroll
             for (int s = 1; s < 32; s <<= 1) {
                 const uint32_t o = __shfl_up_sync(0xffffffffu, inclusive, s);
-                if (lane >= s) inclusive += o;
+                const uint32_t oo = __shfl_up_sync(0xffffffffu, own_inclusive, s);
+                if (lane >= s) {
+                    inclusive += o;
+                    own_inclusive += oo;
+                }
             }
-            if (lane == 31) sh.warp_sum[warp] = inclusive;
+            if (lane == 31) {
+                sh.warp_sum[0][warp] = inclusive;
+                sh.warp_sum[1][warp] = own_inclusive;
+            }
         }
         __syncthreads();
         if (tid < bins) {
-            uint32_t lower = 0;
-            for (int w = 0; w < warp; ++w) lower += sh.warp_sum[w];
+            uint32_t lower = 0, own_lower = 0;
+            for (int w = 0; w < warp; ++w) {
+                lower += sh.warp_sum[0][w];
+                own_lower += sh.warp_sum[1][w];
+            }
             sh.base[tid] = lower + inclusive - all + before;
+            sh.start[tid] = own_lower + own_inclusive - own;
         }
         __syncthreads();
-        if (one_tile) {
+        if (one_tile && pass == passes - 1) {
+            write_tile();
+        } else if (one_tile) {
             scatter_tile();
         } else {
             for (int64_t t0 = lo; t0 < hi; t0 += SORT_TILE) {
