@@ -13,8 +13,8 @@
 //   3. segments that go on far behind their range are joined from their fp32 partial sums, in range order.
 //
 // Measured, 65536 tokens of 1024 bf16 features (ids as in text: few frequent, many rare) into a table of 65536 rows:
-//   1. 53 us: the sort takes 36 alone (latency of two passes of a cluster of eight blocks), the lookup beside it reads 35 MB
-//      of rows and writes 134 MB from the other SMs;
+//   1. 38 us: the sort takes 31 alone (latency of two passes of a cluster of eight blocks), the lookup beside it reads 35 MB
+//      of rows and writes 134 MB from the other SMs, 4.5 TB/s;
 //   2. 52 us for 134 MB of gradients read and 134 MB of table written: 5.2 TB/s, 0.8 of the copy rate.  The rows on
 //      their way to shared memory instead of registers made 69 us 63, neighbouring warps on the slabs of a row 52;
 //   3. 12 us: most blocks find nothing to join, the others wait for a few hundred partial rows.
@@ -34,7 +34,7 @@ constexpr int SORT_KEYS = 8;  // per thread and tile
 constexpr int SORT_TILE = SORT_KEYS * SORT_THREADS;
 constexpr int SORT_DIGIT_BITS = 9;  // two passes sort tables of up to 2^18 - 1 rows
 constexpr int SORT_BINS = 1 << SORT_DIGIT_BITS;
-constexpr int MAX_CLUSTER = 8;  // 16 (not portable) sort in 32 us instead of 36, but beside a lookup both take as long
+constexpr int MAX_CLUSTER = 8;  // the largest portable one
 
 // id as stored, or -1 when it is outside [0, V)
 template <typename I>
@@ -601,10 +601,8 @@ int launch_forward(const void* ids, const void* weight, void* out, int64_t token
         per = dl_ceil_div(tokens, ranks);
         per_log2 = -1;
     }
-    // one block (of 1024 threads) on each SM that the sort leaves, as far as there are rows for them
-    const int64_t lookers = dl_min64(dl_ceil_div(tokens, SORT_THREADS >> look.lanes_log2), DL_NUM_SMS - ranks);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((1 + dl_ceil_div(lookers, ranks)) * ranks));
+    cfg.gridDim = dim3((unsigned)ranks);
     cfg.blockDim = dim3(SORT_THREADS);
     cfg.dynamicSmemBytes = sizeof(SortShared);
     cfg.stream = s;
@@ -617,6 +615,19 @@ int launch_forward(const void* ids, const void* weight, void* out, int64_t token
     const auto kernel = embedding_sorting_kernel<T, W, I>;
     static DlKernelLimits limits;
     if (!dl_allow(reinterpret_cast<const void*>(kernel), limits, sizeof(SortShared))) return DL_ERR_LAUNCH;
+    // as many clusters look up beside the one that sorts as are resident with it, as far as there are rows for them: a
+    // cluster that has to wait would start its share when the others have finished theirs (65536 rows of 2 KB: 52 us)
+    static std::atomic<int> resident[64][4];  // per device and log2 of the cluster; asked for once
+    int device = 0, log2 = 0;
+    while (1 << log2 < ranks) ++log2;
+    if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) return DL_ERR_LAUNCH;
+    int clusters = resident[device][log2].load(std::memory_order_relaxed);
+    if (clusters == 0) {
+        if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) != cudaSuccess || clusters < 1) return DL_ERR_LAUNCH;
+        resident[device][log2].store(clusters, std::memory_order_relaxed);
+    }
+    const int64_t lookers = dl_ceil_div(tokens, (int64_t)(SORT_THREADS >> look.lanes_log2) * ranks);
+    cfg.gridDim.x = (unsigned)((1 + dl_max64(dl_min64(lookers, clusters - 1), 1)) * ranks);
     const cudaError_t e = cudaLaunchKernelEx(
         &cfg, kernel, look, padding, reinterpret_cast<uint2*>(order), reinterpret_cast<uint2*>(order + p.off_b),
         reinterpret_cast<uint8_t*>(order + p.off_present), p.passes, p.digit_bits, per, per_log2);
