@@ -40,7 +40,7 @@ typedef unsigned long long u64;
 constexpr int THREADS = 512;
 constexpr int WARPS = THREADS / 32;
 constexpr int BINS = 2048;
-constexpr int LIST = 2048;  // most logits that are collected and sorted
+constexpr int LIST = 2048;  // most logits that a block collects, and that are sorted
 constexpr int MAX_CLUSTER = 8;
 constexpr int SMALL_V = 512;
 constexpr int TABLE = 128;
@@ -497,7 +497,7 @@ struct Row {
             }
             run += v[k];
         }
-        barrier();  // also: nobody clears a histogram that others still read
+        __syncthreads();  // the other blocks may still read this one's histogram
         at = (int)sh.found[0];
         before = sh.found[1];
         return at < BINS;
@@ -505,6 +505,7 @@ struct Row {
     // adds value(i, key) at step(i, key) wherever that is not negative, and finds the step of target(total)
     template <typename S, typename G>
     __device__ __forceinline__ bool crossing(S step, G target, int& at, u64& before, u64& total, u64& goal) {
+        barrier();  // nobody reads the last histogram any more
         clear_histogram();
         each_key([&](uint32_t i, uint32_t key) {
             u64 value;
@@ -514,9 +515,10 @@ struct Row {
         return find_step(target, at, before, total, goal);
     }
     // Collects the logits that wanted(index, logit) accepts in the blocks' lists.  False: a list was too short for them.
+    // Between one call and the next there is a barrier.
     template <typename F>
     __device__ __forceinline__ bool collect(F wanted) {
-        barrier();  // nobody reads the last list any more
+        __syncthreads();
         if (tid == 0) sh.list_count = 0;
         __syncthreads();
         each4([&](uint32_t i, uint32_t stride, const float (&l)[4]) {
@@ -544,6 +546,7 @@ struct Row {
         bool fits = true;
         for (int r = 0; r < ranks; ++r)
             fits &= (ranks > 1 ? *cluster.map_shared_rank(&sh.list_count, r) : sh.list_count) <= LIST;
+        if (!fits) barrier();
         return fits;
     }
     // Brings the entries of the blocks' lists (`part`: of their parts) to the first block and sorts them there, if there
@@ -734,7 +737,6 @@ struct Row {
         }
         barrier();
         const u64 last = ranks > 1 ? *cluster.map_shared_rank(&sh.found[3], 0) : sh.found[3];
-        barrier();
         return Cut{(uint32_t)(last >> 32), ~(uint32_t)last};
     }
     // cut_in among the logits in the blocks' lists, which hold step `at` and all above.  Key 0 when too many share the step.
