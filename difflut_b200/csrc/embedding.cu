@@ -17,7 +17,8 @@
 //      of rows and writes 134 MB from the other SMs, 4.5 TB/s;
 //   2. 52 us for 134 MB of gradients read and 134 MB of table written: 5.2 TB/s, 0.8 of the copy rate.  The rows on
 //      their way to shared memory instead of registers made 69 us 63, neighbouring warps on the slabs of a row 52;
-//   3. 12 us: most blocks find nothing to join, the others wait for a few hundred partial rows.
+//   3. 12 us: most blocks find nothing to join, the others wait for up to a few hundred partial rows.
+// 5003 tokens of 515 fp32 features: 11 + 17 + 4.5 us.
 // For one step of generation (32 tokens) the lookup is a launch of 1.8 us.
 #include <cooperative_groups.h>
 

@@ -22,8 +22,8 @@
 // eight when there are few rows.  Each pass reads the logits again: after the first they come from L2.
 //
 // Measured: 64 rows of 32000 bf16 logits, T .8: 5.8 us for the largest, 19 us to draw from all, 20 us with top-k 50 and
-// top-p .95, 35 us with top-p .95 alone (8 rows: 31).  Of the latter the histogram of the weights takes 11 us, the two
-// searches in histograms 3 us each, collecting 6 us: latency of passes with few rounds of loads per thread, not bandwidth
+// top-p .95, 34 us with top-p .95 alone (8 rows: 30).  Of the latter the histogram of the weights takes 7 us, the two
+// searches in histograms 3 to 4 us each, collecting 4, the cut 5: latency of passes with few rounds of loads per thread, not bandwidth
 // (the 4 MB are read in a microsecond).  256 rows of 65536 fp32 logits with top-p .9 and min-p .01: 88 us, 43 of them the
 // histogram, bound by issue slots (51 % over all SMs, of which 108 hold two rows and 40 one; the double-precision pipe is
 // 12 % busy, the data pipe of shared memory 40 %); reading the 67 MB once takes 10.
@@ -1096,7 +1096,7 @@ int launch_sample(const void* logits, const Job& job, cudaStream_t s) {
     }
     // twice as many blocks per row while they keep 6144 classes each and there is an SM for every one: each has its own
     // histograms, lists and barriers to go through (top-p .95, 8 x 32000: 31 us with four blocks a row, 35 with two or eight;
-    // 64 x 32000: 35 us with two, 41 with four; 1 x 8192: 18 with one, 23 with two)
+    // 64 x 32000: 34 us with two, 41 with four; 1 x 8192: 18 with one, 23 with two)
     int ranks = 1;
     while (ranks < MAX_CLUSTER && job.V >= (int64_t)12288 * ranks && job.R * ranks * 2 <= DL_NUM_SMS) ranks *= 2;
     if (job.R * ranks > 0x7fffffff) return DL_ERR_TOO_LARGE;

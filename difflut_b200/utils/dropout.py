@@ -79,7 +79,8 @@ class Dropout(nn.Module):
     Eager calls take a fresh seed from torch's CPU generator (reproducible under torch.manual_seed), as the layers'
     bit flip does.  While a CUDA graph is being captured the mask comes from a counter on the device instead, which
     every replay advances; it is created by an eager training call on that device, so run one before the capture (any
-    warm-up step does)."""
+    warm-up step does).  A block that a captured backward pass recomputes (checkpointing) would draw another mask: use
+    `dropout` with an offset there."""
 
     def __init__(self, p: Optional[float] = None) -> None:
         super().__init__()
