@@ -23,8 +23,8 @@
 //
 // Measured: 64 rows of 32000 bf16 logits, T .8: 5.8 us for the largest, 19 us to draw from all, 20 us with top-k 50 and
 // top-p .95, 34 us with top-p .95 alone (8 rows: 30).  Of the latter the histogram of the weights takes 7 us, the two
-// searches in histograms 3 to 4 us each, collecting 4, the cut 5: latency of passes with few rounds of loads per thread, not bandwidth
-// (the 4 MB are read in a microsecond).  256 rows of 65536 fp32 logits with top-p .9 and min-p .01: 88 us, 43 of them the
+// searches in histograms 3 to 4 us each, collecting 4, the cut 5: latency of passes with few rounds of loads per thread,
+// not bandwidth (the 4 MB are read in a microsecond).  256 rows of 65536 fp32 logits with top-p .9 and min-p .01: 88 us, 43 of them the
 // histogram, bound by issue slots (51 % over all SMs, of which 108 hold two rows and 40 one; the double-precision pipe is
 // 12 % busy, the data pipe of shared memory 40 %); reading the 67 MB once takes 10.
 #include <cooperative_groups.h>
@@ -1116,7 +1116,8 @@ int launch_sample(const void* logits, const Job& job, cudaStream_t s) {
     const auto kernel = sample_kernel<T>;
     static DlKernelLimits limits;
     if (!dl_allow(reinterpret_cast<const void*>(kernel), limits, sizeof(Shared))) return DL_ERR_LAUNCH;
-    return cudaLaunchKernelEx(&cfg, kernel, src, job, ranks, slice, vectors) == cudaSuccess ? dl_launch_status() : DL_ERR_LAUNCH;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, src, job, ranks, slice, vectors);
+    return e == cudaSuccess ? dl_launch_status() : DL_ERR_LAUNCH;
 }
 
 }  // namespace

@@ -103,9 +103,10 @@ class Dropout(nn.Module):
             capturing = torch.cuda.is_current_stream_capturing()
             held = self._counters.get(x.device)
             if not capturing:
+                seed = self._draw_seed()  # one draw per call, so that a recomputed call finds its own again
                 if held is None:
-                    self._counters[x.device] = (self._draw_seed(), torch.zeros(1, device=x.device, dtype=torch.int64))
-                return dropout(x, self.p, self._draw_seed())
+                    self._counters[x.device] = (seed ^ 1 << 61, torch.zeros(1, device=x.device, dtype=torch.int64))
+                return dropout(x, self.p, seed)
             if held is None:
                 raise RuntimeError("Dropout: run one training call on this device before capturing a CUDA graph")
             seed, counter = held

@@ -156,6 +156,17 @@ def test_dropout_module_in_a_captured_graph_draws_a_mask_per_replay():
     assert not torch.equal(seen[0], seen[1]) and not torch.equal(seen[1], seen[2])
 
 
+def test_dropout_module_in_a_checkpointed_block_recomputes_its_mask():
+    from torch.utils.checkpoint import checkpoint
+
+    drop = Dropout(0.5).train()
+    x = torch.full((4096,), 3.0, device=DEV, requires_grad=True)
+    y = checkpoint(lambda v: drop(v) * v, x, use_reentrant=False)
+    kept = y.detach() != 0
+    (g,) = torch.autograd.grad(y.sum(), x)
+    assert 1700 < int(kept.sum()) < 2400 and torch.equal(g, torch.where(kept, 12.0, 0.0))
+
+
 def test_dropout_on_another_stream():
     x = _normal(1 << 20)
     want = dropout(x, 0.5, seed=8)
