@@ -810,6 +810,34 @@ def test_token_model_equals_its_plain_form():
     close_normwise(model.norm.bias.grad, b.grad, "norm bias")
 
 
+def test_token_block_recomputed_expanded_and_repeated():
+    """The same gradients with checkpointing, from an expanded gradient of the output, and a second time from a kept graph."""
+    from torch.utils.checkpoint import checkpoint
+
+    emb = EmbeddingEncoder(50, num_bits=16, padding_idx=3, flatten=False).to(DEV)
+    norm, drop = GroupNorm(4, 16, activation="silu").to(DEV), Dropout(0.25).train()
+    ids = torch.randint(0, 50, (6, 40), generator=torch.Generator().manual_seed(5)).to(DEV)
+    leaves = [emb.weight, norm.weight, norm.bias]
+
+    def block(ids):
+        return drop(norm(emb(ids)))
+
+    def grads(y, g, **kwargs):
+        return torch.autograd.grad(y, leaves, g, **kwargs)
+
+    g = torch.full((1, 1, 1), 0.5, device=DEV).expand(6, 40, 16)
+    torch.manual_seed(11)
+    y = block(ids)
+    want = grads(y, g.contiguous(), retain_graph=True)
+    assert all(float(w.abs().max()) > 0 for w in want) and float(want[0][3].abs().max()) == 0.0
+    again, expanded = grads(y, g.contiguous(), retain_graph=True), grads(y, g)
+    torch.manual_seed(11)
+    recomputed = checkpoint(block, ids, use_reentrant=False)
+    assert torch.equal(recomputed, y)
+    for other in (again, expanded, grads(recomputed, g)):
+        assert all(torch.equal(a, b) for a, b in zip(want, other))
+
+
 def test_token_model_trains_captured_and_samples():
     """A captured step draws a new mask per replay and moves the parameters; ids are then sampled from the logits."""
     model, ids, labels = _token_model(p=0.5)
