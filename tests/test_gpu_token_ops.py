@@ -810,6 +810,70 @@ def test_token_model_equals_its_plain_form():
     close_normwise(model.norm.bias.grad, b.grad, "norm bias")
 
 
+def test_embedding_elements_past_32_bits():
+    """The last rows of a table of 2.3e9 elements, and as many tokens' elements as that."""
+    V, D = 140001, 16384
+    w = torch.zeros(V, D, device=DEV, dtype=torch.bfloat16)
+    ids = torch.tensor([V - 1, 0, V - 2, V - 1], device=DEV)
+    w[V - 2], w[V - 1] = 2.0, 3.0
+    w.requires_grad_()
+    out = embedding_lookup(ids, w, 2.0)
+    assert out[:, ::4095].tolist() == [[v] * 5 for v in (6.0, 0.0, 4.0, 6.0)]
+    (g,) = torch.autograd.grad(out, w, torch.ones_like(out))
+    assert g[[0, 1, V - 3, V - 2, V - 1], 7].tolist() == [2.0, 0.0, 0.0, 2.0, 4.0] and float(g[V - 1].sum()) == 4.0 * D
+    assert float(g[1: V - 2: 997].abs().max()) == 0.0
+    del w, g, out
+    small = _normal(9, D, dtype=torch.bfloat16).requires_grad_()
+    ids = torch.arange(V, device=DEV) % 9
+    out = embedding_lookup(ids, small)
+    assert all(torch.equal(out[t], small[t % 9]) for t in (0, 131071, 131072, V - 1))
+    g = torch.zeros_like(out)
+    g[V - 1] = 1.0
+    (gw,) = torch.autograd.grad(out, small, g)
+    assert float(gw[(V - 1) % 9].min()) == 1.0 and float(gw.sum()) == D
+
+
+def test_group_norm_elements_past_32_bits():
+    """Two samples of 1.2e9 values: the second one as if it stood alone (behind a short pass over the first)."""
+    S, C, G = 1200001, 1024, 8
+    x = torch.zeros(2, S, C, device=DEV, dtype=torch.bfloat16)
+    x[1, S - 5000:] = _normal(5000, C, dtype=torch.bfloat16)
+    g = torch.zeros_like(x)
+    g[1, S - 1] = 1.0
+    w = torch.ones(C, device=DEV, requires_grad=True)
+    x.requires_grad_()
+    y = group_norm(x, G, w)
+    tail = x.detach()[1, S - 5000:].double().view(5000, G, -1)
+    m = S * (C // G)
+    mean = tail.sum(dim=(0, 2)) / m
+    var = (tail * tail).sum(dim=(0, 2)) / m - mean * mean
+    want = ((tail[-1] - mean[:, None]) * torch.rsqrt(var + 1e-5)[:, None]).reshape(-1)
+    got = y.detach()[1, S - 1].double()
+    # one rounding to bf16's 8 significant bits (half a step is up to 2^-8 of the value: eps = 2^-7), and the statistics'
+    # fp32 sums: a thread adds up some 16000 values of a chunk, each addition off by 2^-24 of the sum at most: 2^-10 of the
+    # variance, 2^-11 of its root, and as much again for the mean and what joins the chunks
+    rounding = half_step(torch.bfloat16) + 2.0 ** -10
+    assert bool(((got - want).abs() <= want.abs() * rounding + 1e-5).all())
+    assert float(y.detach()[0].abs().max()) == 0.0
+    gx, gw = torch.autograd.grad(y, (x, w), g)
+    assert bool(((gw.double() - want).abs() <= want.abs() * 2.0 ** -10 + 1e-5).all())
+    rstd = torch.rsqrt(var + 1e-5)[:, None]
+    xh = (tail[-1] - mean[:, None]) * rstd
+    s2 = xh.sum(dim=1, keepdim=True) / m
+    last = (rstd * (1.0 - (C // G) / m - xh * s2)).reshape(-1)
+    assert bool(((gx[1, S - 1].double() - last).abs() <= last.abs() * rounding).all())
+
+
+def test_sampling_rows_past_32_bits():
+    R, V = 70001, 32768
+    x = torch.full((R, V), -40.0, device=DEV, dtype=torch.bfloat16)
+    hot = (torch.arange(R, device=DEV) * 7919) % V
+    x[torch.arange(R, device=DEV), hot] = 10.0
+    u = torch.rand(R, device=DEV, generator=torch.Generator(DEV).manual_seed(1))
+    for kw in ({"temperature": 0.0}, {"top_p": 0.9}, {"top_k": 5, "min_p": 0.5}):
+        assert torch.equal(sample_logits(x, u, **kw), hot)
+
+
 def test_token_block_recomputed_expanded_and_repeated():
     """The same gradients with checkpointing, from an expanded gradient of the output, and a second time from a kept graph."""
     from torch.utils.checkpoint import checkpoint
