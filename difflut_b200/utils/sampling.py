@@ -6,6 +6,9 @@ import torch
 
 from .. import _native
 
+# integer types with values that int32 does not have
+_WIDE = (torch.int64, torch.uint64, torch.uint32)
+
 
 def _setting(name, value, rows, dtype, low, high, low_open=False):
     """(per-row tensor or None, scalar) of one setting, checked; per-row values are not read on the host."""
@@ -15,7 +18,8 @@ def _setting(name, value, rows, dtype, low, high, low_open=False):
         if not dtype.is_floating_point:
             if value.is_floating_point() or value.is_complex():
                 raise ValueError(f"{name} must hold integers, got {value.dtype}")
-            value = value.clamp(max=torch.iinfo(dtype).max) if value.dtype == torch.int64 else value
+            # 64 bits that cannot hold the value make it negative: it keeps all classes, as a count that large does
+            value = value.to(torch.int64).clamp(0, torch.iinfo(dtype).max) if value.dtype in _WIDE else value
         return value.to(dtype).contiguous(), None
     number = isinstance(value, (int, float) if dtype.is_floating_point else int) and not isinstance(value, bool)
     if not number or not (low < value if low_open else low <= value) or not value <= high:

@@ -1,0 +1,50 @@
+"""Calls of the token path that the documentation allows, at its edges, without a GPU.
+
+Where a call would launch, the launches are replaced by functions that do nothing: what is looked at here is which
+calls are refused, what autograd is told and what reaches the entry points.
+"""
+
+import contextlib
+import subprocess
+import sys
+
+import pytest
+import torch
+import torch.autograd.forward_ad as forward_ad
+from torch.utils.checkpoint import checkpoint
+
+from difflut_b200 import _native
+from difflut_b200.build import LIB_PATH
+from difflut_b200.encoder import EmbeddingEncoder, embedding_lookup
+from difflut_b200.network import DWNNetwork
+from difflut_b200.utils import Dropout, GroupSum, dropout, group_norm
+from difflut_b200.utils import sampling
+
+
+@pytest.fixture
+def no_launches(monkeypatch):
+    """CPU tensors pass and nothing is launched; yields the names of the entry points called."""
+    called = []
+
+    def entry(name):
+        return lambda *args: called.append(name)
+
+    monkeypatch.setattr(_native, "require_cuda", lambda what, *tensors: None)
+    monkeypatch.setattr(_native, "entry", entry)
+    monkeypatch.setattr(_native, "call", lambda name, *args, **kwargs: called.append(name))
+    monkeypatch.setattr(_native, "device_of", lambda t: contextlib.nullcontext())
+    yield called
+
+
+# ---------------------------------------------------------------------------------------------- sampling
+@pytest.mark.parametrize("dtype", [torch.int64, torch.uint64, torch.uint32])
+def test_top_k_per_row_of_any_size_keeps_its_meaning(dtype):
+    """A count that is not positive or not below the number of classes keeps all, also past the 32 bits of the kernel."""
+    counts = {torch.int64: [-2 ** 32 + 5, -2 ** 33 + 1, -2 ** 31 - 1, -2 ** 63, -1, 0, 3, 2 ** 31, 2 ** 32 + 2, 2 ** 63 - 1],
+              torch.uint64: [0, 3, 2 ** 31, 2 ** 32 + 2, 2 ** 63, 2 ** 64 - 3],
+              torch.uint32: [0, 3, 2 ** 31, 2 ** 32 - 2]}[dtype]
+    rows, scalar = sampling._setting("top_k", torch.tensor(counts, dtype=dtype), len(counts), torch.int32, 0, 2 ** 62)
+    assert scalar is None and rows.dtype == torch.int32
+    V = 1 << 29  # more classes than this are refused
+    for count, row in zip(counts, rows.tolist()):
+        assert (row if 0 < row < V else 0) == (count if 0 < count < V else 0), (count, row)
