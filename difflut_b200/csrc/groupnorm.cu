@@ -741,7 +741,7 @@ bool grid_fits(const Norm& p, const Cut& k) { return p.N * k.blocks_c * (int64_t
 
 // W as the kernel takes it, at most ROW_WIDTH
 bool cut_rows(const Norm& p, int W, int items, int64_t most_blocks, RowCut& k) {
-    if (p.S != 1 || p.per_group / W > 32) return false;
+    if (p.S != 1 || p.N == 0 || p.per_group / W > 32) return false;  // without rows there is nothing to divide by
     k.lanes = p.per_group / W;
     k.lanes_log2 = 0;
     while ((1 << k.lanes_log2) < k.lanes) ++k.lanes_log2;

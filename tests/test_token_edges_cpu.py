@@ -48,3 +48,16 @@ def test_top_k_per_row_of_any_size_keeps_its_meaning(dtype):
     V = 1 << 29  # more classes than this are refused
     for count, row in zip(counts, rows.tolist()):
         assert (row if 0 < row < V else 0) == (count if 0 < count < V else 0), (count, row)
+
+
+# ---------------------------------------------------------------------------------------------- group norm
+@pytest.mark.parametrize("S", [1, 2, 1000])
+@pytest.mark.parametrize("C,G", [(8, 2), (1024, 1), (64, 64), (1, 1)])
+def test_group_norm_workspaces_of_no_samples(S, C, G):
+    """In a process of its own: a division by zero in a size function ends it."""
+    code = (f"import ctypes; lib = ctypes.CDLL({LIB_PATH!r})\n"
+            "for f in (lib.dl_group_norm_scratch_bytes, lib.dl_group_norm_bwd_scratch_bytes):\n"
+            "    f.argtypes, f.restype = [ctypes.c_int64] * 5, ctypes.c_int64\n"
+            f"    assert all(f(0, {S}, {C}, {G}, dtype) == 0 for dtype in range(3))\n")
+    done = subprocess.run([sys.executable, "-S", "-c", code], capture_output=True, text=True)
+    assert done.returncode == 0, done.stderr
