@@ -11,6 +11,7 @@ import ctypes
 import os
 
 import torch
+from torch.autograd import forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "_lib", "libdifflut_b200.so")
@@ -197,6 +198,25 @@ def require_cuda(what: str, *tensors) -> None:
             raise RuntimeError(f"difflut_b200.{what}: tensors are on devices {device} and {index}")
 
 
+def followed(*tensors) -> bool:
+    """Whether autograd follows a call on these tensors, so that it has to go through its Function (None is skipped).
+
+    A tensor with a forward-mode tangent need not require a gradient; the Function then says that it has no forward
+    derivative, where a bare launch would read as a tangent of zero."""
+    if forward_ad._current_level >= 0:
+        return True
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def refuse_tangents(*grads) -> None:
+    """For a backward pass by bare launches: its incoming gradients carry no forward-mode tangents."""
+    if forward_ad._current_level >= 0:
+        for g in grads:
+            if g is not None and forward_ad.unpack_dual(g).tangent is not None:
+                raise NotImplementedError("the backward pass has no forward derivative (jvp): it cannot take a gradient that "
+                                          "carries a tangent")
+
+
 def once_differentiable_backward(backward):
     """A Function's backward whose result cannot be differentiated again: an error says so if it is.  torch's own wrapper
     costs several microseconds a call and only matters while a graph of the backward pass is being built."""
@@ -205,6 +225,7 @@ def once_differentiable_backward(backward):
     guarded = once_differentiable(backward)
 
     def chosen(ctx, *grads):
+        refuse_tangents(*grads)
         return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
 
     return chosen

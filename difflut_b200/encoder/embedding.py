@@ -84,7 +84,7 @@ def embedding_lookup(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0
             raise ValueError(f"padding_idx must be within [-{V}, {V}), got {padding_idx}")
         padding = int(padding_idx) % V
     ids, weight = ids.contiguous(), weight.contiguous()
-    if weight.requires_grad and torch.is_grad_enabled():
+    if _native.followed(weight):
         return _EmbeddingFn.apply(ids, weight, float(scale), padding)
     return _forward(ids, weight, float(scale), padding, False)[0]
 

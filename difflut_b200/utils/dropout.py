@@ -48,6 +48,7 @@ class _DropoutFn(torch.autograd.Function):
         g = g.contiguous()
         if torch.is_grad_enabled():  # create_graph
             return _DropoutFn.apply(g, p, seed, offset, counter), None, None, None, None
+        _native.refuse_tangents(g)
         return _apply_mask(g, p, seed, offset, counter), None, None, None, None
 
 
@@ -68,7 +69,7 @@ def dropout(x: torch.Tensor, p: float = DEFAULT_DROPOUT_P, seed: int = 0, offset
     if counter is not None and (counter.dtype != torch.int64 or counter.numel() != 1):
         raise TypeError(f"counter must hold one int64, got {counter.numel()} x {counter.dtype}")
     x = x.contiguous()
-    if x.requires_grad and torch.is_grad_enabled():
+    if _native.followed(x):
         return _DropoutFn.apply(x, p, seed, offset, counter)
     return _apply_mask(x, p, seed, offset, counter)
 

@@ -120,8 +120,7 @@ def group_norm(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor] 
     weight = None if weight is None else weight.contiguous()
     bias = None if bias is None else bias.contiguous()
     dims = (N, S, C, num_groups, 0 if param_dtype is None else _native.DTYPE_CODES[param_dtype])
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
-                                    or (bias is not None and bias.requires_grad)):
+    if _native.followed(x, weight, bias):
         return _GroupNormFn.apply(x, weight, bias, dims, float(eps), act)
     return _forward(x, weight, bias, dims, float(eps), act, False)[0]
 

@@ -61,3 +61,37 @@ def test_group_norm_workspaces_of_no_samples(S, C, G):
             f"    assert all(f(0, {S}, {C}, {G}, dtype) == 0 for dtype in range(3))\n")
     done = subprocess.run([sys.executable, "-S", "-c", code], capture_output=True, text=True)
     assert done.returncode == 0, done.stderr
+
+
+# ---------------------------------------------------------------------------------------------- differentiation
+def test_forward_mode_differentiation_is_refused(no_launches):
+    x, w, ids = torch.ones(6, 16), torch.ones(16), torch.arange(6)
+    calls = [lambda t: dropout(t, 0.5), lambda t: embedding_lookup(ids, t), lambda t: group_norm(t, 4),
+             lambda t: group_norm(x, 4, t[0]), lambda t: group_norm(x, 4, w, t[0])]
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for call in calls:
+            with pytest.raises(NotImplementedError, match="jvp"):
+                call(dual)
+            with torch.no_grad(), pytest.raises(NotImplementedError, match="jvp"):
+                call(dual)
+        no_launches.clear()
+        for call in calls:  # tensors without a tangent are taken as ever
+            assert not call(x).requires_grad
+        assert len(no_launches) == len(calls)
+    assert not _native.followed(x, None) and _native.followed(None, w.clone().requires_grad_())
+
+
+def test_gradient_with_a_forward_mode_tangent_is_refused(no_launches):
+    """Forward over reverse: the operator's input has no tangent, what comes back to it has one."""
+    ids = torch.arange(6)
+    for call in (lambda t: dropout(t, 0.5), lambda t: embedding_lookup(ids, t), lambda t: group_norm(t, 4)):
+        x = torch.ones(6, 16, requires_grad=True)
+        y = call(x)
+        with forward_ad.dual_level():
+            g = forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y))
+            with pytest.raises(NotImplementedError, match="jvp"):
+                torch.autograd.grad(y, x, g, retain_graph=True)
+            with pytest.raises(NotImplementedError, match="jvp"):
+                torch.autograd.grad(y, x, g, retain_graph=True, create_graph=True)
+            torch.autograd.grad(y, x, torch.ones_like(y))
