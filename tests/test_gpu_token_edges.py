@@ -10,9 +10,11 @@ import torch.autograd.forward_ad as forward_ad
 
 from difflut_b200.encoder import embedding_lookup
 from difflut_b200.utils import dropout, group_norm, sample_logits
+from token_util import half_step
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
+U32 = 2.0 ** -24
 
 
 def _normal(*shape, dtype=torch.float32, seed=0):
@@ -71,3 +73,43 @@ def test_gradient_with_a_forward_mode_tangent_is_refused():
             with pytest.raises(NotImplementedError, match="jvp"):
                 torch.autograd.grad(y, x, g, retain_graph=True, create_graph=True)
             torch.autograd.grad(y, x, torch.ones_like(y))
+
+
+def _variance_bound(values, width, threads):
+    """Relative error of the variance of groups whose threads hold `values` values each, `width` per row.
+
+    A thread takes its values by runs, squares relative to the mean of what came before the run: these add up to no more
+    than twice the squares around the thread's mean (the first run's to nine times, its centre being the mean of one of
+    eight rows), and a run is at most 32 rows.  Runs are joined by one addition each, then the threads of a block, a
+    lane of a warp after the other."""
+    return (2 * 32 * width + 9 * 8 * width + values / (32 * width) + 8 + threads / 32 + 16) * U32
+
+
+@pytest.mark.parametrize("dtype,S,C", [(torch.float32, 524288, 4), (torch.bfloat16, 262144, 8), (torch.float32, 1048576, 2)])
+def test_group_norm_value_far_from_all_that_follow(dtype, S, C):
+    """Thousands of values per thread, the first one far away: the variance is what the other ones make it.
+
+    So many samples that each is one block of 256 threads, 8192 values a thread; the samples looked at have an outlier in
+    their first row and zeros behind it, small noise behind it, and noise without it."""
+    N, width = 600, C
+    x = torch.zeros(N, S, C, device=DEV, dtype=dtype)
+    noise = torch.randn(S, C, device=DEV, generator=torch.Generator(DEV).manual_seed(3))
+    x[0, 0, 0] = 1003.7
+    x[1] = (noise * 0.05).to(dtype)
+    x[1, 0, 0] = 1003.7
+    x[2] = noise.to(dtype)
+    y = group_norm(x, 1)
+    bound = _variance_bound(8192, width, 256)
+    for n in range(3):
+        v = x[n].double()
+        mean = v.mean()
+        var = (v - mean).square().mean()
+        want = (v - mean) / torch.sqrt(var + 1e-5)
+        # half the variance's error for its root, roundings of the linear form, the mean off by its roundings and the
+        # block's share of a thread's (one of 256 threads has the outlier)
+        off = bound / 2 + 8 * U32
+        size = v[0].abs().max() / torch.sqrt(var + 1e-5)
+        limit = want.abs() * (off + half_step(dtype) * 1.01) + 2 * U32 * (1 + size)
+        err = (y[n].double() - want).abs()
+        assert bool((err <= limit).all()), (n, float((err / limit).max()), float(err.max()))
+    assert float(y[3:].abs().max()) == 0.0
