@@ -80,8 +80,8 @@ class Dropout(nn.Module):
     Eager calls take a fresh seed from torch's CPU generator (reproducible under torch.manual_seed), as the layers'
     bit flip does.  While a CUDA graph is being captured the mask comes from a counter on the device instead, which
     every replay advances; it is created by an eager training call on that device, so run one before the capture (any
-    warm-up step does).  A block that a captured backward pass recomputes (checkpointing) would draw another mask: use
-    `dropout` with an offset there."""
+    warm-up step does).  In a block that a captured backward pass recomputes (checkpointing) the recomputation would draw
+    another mask than the forward pass: it raises RuntimeError, use `dropout` with a seed or counter of your own there."""
 
     def __init__(self, p: Optional[float] = None) -> None:
         super().__init__()
@@ -108,6 +108,9 @@ class Dropout(nn.Module):
                 if held is None:
                     self._counters[x.device] = (seed ^ 1 << 61, torch.zeros(1, device=x.device, dtype=torch.int64))
                 return dropout(x, self.p, seed)
+            if torch._C._current_graph_task_id() != -1:  # called by autograd, in a backward pass
+                raise RuntimeError("Dropout: a block recomputed while its backward pass is captured into a CUDA graph would draw "
+                                   "another mask than its forward pass; use dropout() with a seed or counter of your own")
             if held is None:
                 raise RuntimeError("Dropout: run one training call on this device before capturing a CUDA graph")
             seed, counter = held

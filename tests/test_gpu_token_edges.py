@@ -7,9 +7,10 @@ fp32 additions by n * 2^-24 of what it adds up.
 import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
+from torch.utils.checkpoint import checkpoint
 
 from difflut_b200.encoder import embedding_lookup
-from difflut_b200.utils import dropout, group_norm, sample_logits
+from difflut_b200.utils import Dropout, dropout, group_norm, sample_logits
 from token_util import half_step
 
 pytestmark = pytest.mark.gpu
@@ -113,3 +114,26 @@ def test_group_norm_value_far_from_all_that_follow(dtype, S, C):
         err = (y[n].double() - want).abs()
         assert bool((err <= limit).all()), (n, float((err / limit).max()), float(err.max()))
     assert float(y[3:].abs().max()) == 0.0
+
+
+# ---------------------------------------------------------------------------------------------- dropout
+def test_dropout_module_recomputed_while_capturing_is_refused():
+    """A captured mask is drawn on the device: a recomputation would draw another one than the forward pass used."""
+    drop, x = Dropout(0.5).train(), torch.ones(4096, device=DEV, requires_grad=True)
+    with torch.no_grad():
+        drop(x)
+    torch.cuda.synchronize()
+    graph, refused = torch.cuda.CUDAGraph(), None
+    with torch.cuda.graph(graph):
+        y = checkpoint(lambda v: drop(v) * v, x, use_reentrant=False, preserve_rng_state=False)
+        try:
+            torch.autograd.grad(y.sum(), x)
+        except RuntimeError as e:
+            refused = str(e)
+    assert refused is not None and "recomputed" in refused
+    graph.replay()
+    torch.cuda.synchronize()
+    kept = y.detach() != 0
+    assert 1700 < int(kept.sum()) < 2400 and torch.equal(y.detach(), torch.where(kept, 2.0, 0.0))
+    with torch.no_grad():
+        assert 1700 < int((drop(x) != 0).sum()) < 2400

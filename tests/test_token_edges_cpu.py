@@ -95,3 +95,23 @@ def test_gradient_with_a_forward_mode_tangent_is_refused(no_launches):
             with pytest.raises(NotImplementedError, match="jvp"):
                 torch.autograd.grad(y, x, g, retain_graph=True, create_graph=True)
             torch.autograd.grad(y, x, torch.ones_like(y))
+
+
+# ---------------------------------------------------------------------------------------------- dropout
+@pytest.mark.parametrize("use_reentrant", [False, True])
+def test_dropout_module_recomputed_while_capturing_is_refused(no_launches, monkeypatch, use_reentrant):
+    """A captured mask is drawn on the device: a recomputation would draw another one than the forward pass used."""
+    drop, x = Dropout(0.5).train(), torch.ones(64, requires_grad=True)
+
+    def gradient():
+        y = checkpoint(lambda v: drop(v) * v, x, use_reentrant=use_reentrant, preserve_rng_state=False)
+        y.sum().backward()
+
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    gradient()  # eager: also makes the counter
+    assert no_launches.count("dl_dropout") == 3
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="recomputed"):
+        gradient()
+    (drop(x) * x).sum().backward()  # without recomputation
+    assert no_launches.count("dl_counter_draw") == 2
