@@ -57,15 +57,15 @@ class _GroupNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, dims, eps, act):
         y, held, mean_at = _forward(x, weight, bias, dims, eps, act, True)
-        ctx.save_for_backward(x, weight, bias)
-        ctx.held, ctx.spec = held, (dims, act, mean_at)
+        ctx.save_for_backward(x, weight, bias, held)
+        ctx.spec = (dims, act, mean_at)
         return y
 
     @staticmethod
     @_native.once_differentiable_backward
     def backward(ctx, g):
-        x, weight, bias = ctx.saved_tensors
-        held, ((N, S, C, G, param_code), act, mean_at) = ctx.held, ctx.spec
+        x, weight, bias, held = ctx.saved_tensors
+        (N, S, C, G, param_code), act, mean_at = ctx.spec
         code = _native.DTYPE_CODES[x.dtype]
         g = g.contiguous()
         gx = torch.empty_like(x)

@@ -137,3 +137,46 @@ def test_dropout_module_recomputed_while_capturing_is_refused():
     assert 1700 < int(kept.sum()) < 2400 and torch.equal(y.detach(), torch.where(kept, 2.0, 0.0))
     with torch.no_grad():
         assert 1700 < int((drop(x) != 0).sum()) < 2400
+
+
+# ---------------------------------------------------------------------------------------------- what is kept
+def _training_calls():
+    ids = torch.randint(0, 500, (20000,), generator=torch.Generator().manual_seed(0)).to(DEV)
+    table, x = _normal(500, 8).requires_grad_(True), _normal(64, 3000, 8).requires_grad_(True)
+    counter = torch.zeros(1, device=DEV, dtype=torch.int64)
+    return {"embedding": (lambda: embedding_lookup(ids, table), table),
+            "group norm": (lambda: group_norm(x, 2), x),
+            "dropout": (lambda: dropout(x, 0.5, seed=1, counter=counter), x)}
+
+
+@pytest.mark.parametrize("name", ["embedding", "group norm", "dropout"])
+def test_second_backward_pass_needs_a_kept_graph(name):
+    call, leaf = _training_calls()[name]
+    y = call()
+    g = torch.ones_like(y)
+    first = torch.autograd.grad(y, leaf, g, retain_graph=True)[0]
+    assert torch.equal(torch.autograd.grad(y, leaf, g)[0], first)
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(y, leaf, g)
+
+
+@pytest.mark.parametrize("name", ["embedding", "group norm"])
+def test_what_the_backward_pass_needs_is_let_go_behind_it(name):
+    call, leaf = _training_calls()[name]
+    y = call()  # keeps the graph
+    g = torch.ones_like(y)
+    torch.cuda.synchronize()
+    held = torch.cuda.memory_allocated()
+    torch.autograd.grad(y, leaf, g)
+    torch.cuda.synchronize()
+    assert torch.cuda.memory_allocated() < held
+
+
+@pytest.mark.parametrize("name", ["embedding", "group norm", "dropout"])
+def test_what_the_backward_pass_needs_goes_through_saved_tensor_hooks(name):
+    call, leaf = _training_calls()[name]
+    plain = call()
+    want = torch.autograd.grad(plain, leaf, torch.ones_like(plain))[0]
+    with torch.autograd.graph.save_on_cpu():
+        y = call()
+    assert torch.equal(torch.autograd.grad(y, leaf, torch.ones_like(y))[0], want)

@@ -115,3 +115,25 @@ def test_dropout_module_recomputed_while_capturing_is_refused(no_launches, monke
         gradient()
     (drop(x) * x).sum().backward()  # without recomputation
     assert no_launches.count("dl_counter_draw") == 2
+
+
+# ---------------------------------------------------------------------------------------------- what is kept
+@pytest.mark.parametrize("saved,call", [
+    (1, lambda x: embedding_lookup(torch.arange(4), x)),
+    (2, lambda x: group_norm(x, 4)),  # and the statistics
+    (1, lambda x: dropout(x, 0.5, counter=torch.zeros(1, dtype=torch.int64)))])
+def test_what_the_backward_pass_needs_is_kept_by_autograd(no_launches, saved, call):
+    """Saved-tensor hooks see it, and it goes with the first backward pass that does not keep the graph."""
+    x, packed = torch.ones(8, 16, requires_grad=True), []
+
+    def pack(t):
+        packed.append(t)
+        return t
+
+    with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t):
+        y = call(x)
+    assert len(packed) == saved
+    torch.autograd.grad(y, x, torch.ones_like(y), retain_graph=True)
+    torch.autograd.grad(y, x, torch.ones_like(y))
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(y, x, torch.ones_like(y))
