@@ -123,7 +123,7 @@ class EmbeddingEncoder(BaseEncoder):
         out = embedding_lookup(ids, self.weight, self.scale, self.padding_idx)
         if not self.flatten:
             return out
-        return out.reshape(-1) if ids.dim() <= 1 else out.reshape(ids.shape[0], -1)
+        return out.reshape(-1) if ids.dim() <= 1 else out.flatten(1)
 
     def to(self, *args, **kwargs) -> "EmbeddingEncoder":
         return nn.Module.to(self, *args, **kwargs)  # the table is a parameter, not a plain attribute

@@ -137,3 +137,12 @@ def test_what_the_backward_pass_needs_is_kept_by_autograd(no_launches, saved, ca
     torch.autograd.grad(y, x, torch.ones_like(y))
     with pytest.raises(RuntimeError, match="second time"):
         torch.autograd.grad(y, x, torch.ones_like(y))
+
+
+# ---------------------------------------------------------------------------------------------- embedding encoder
+@pytest.mark.parametrize("shape,flat", [((0, 5), (0, 20)), ((3, 0), (3, 0)), ((0,), (0,)), ((0, 2, 5), (0, 40)), ((3, 5), (3, 20)),
+                                        ((3, 2, 5), (3, 40)), ((5,), (20,)), ((), (4,))])
+def test_embedding_encoder_shapes(no_launches, shape, flat):
+    ids = torch.zeros(shape, dtype=torch.int64)
+    assert EmbeddingEncoder(10, num_bits=4).encode(ids).shape == flat
+    assert EmbeddingEncoder(10, num_bits=4, flatten=False).encode(ids).shape == shape + (4,)
