@@ -39,6 +39,9 @@ class DWNNetwork:
                  fused_backward: bool = True, peer_optimizer: Optional[bool] = None, peer_status_every: int = 0):
         if not encoder.is_fitted:
             raise RuntimeError("DWNNetwork needs a fitted encoder")
+        if getattr(encoder, "thresholds", None) is None:
+            raise TypeError(f"DWNNetwork compares real features with its encoder's thresholds itself, which "
+                            f"{type(encoder).__name__} does not have; use the layer API behind it")
         if groupsum.use_randperm:
             raise ValueError("DWNNetwork does not support GroupSum(use_randperm=True)")
         for l in layers:

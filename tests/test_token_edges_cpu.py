@@ -146,3 +146,8 @@ def test_embedding_encoder_shapes(no_launches, shape, flat):
     ids = torch.zeros(shape, dtype=torch.int64)
     assert EmbeddingEncoder(10, num_bits=4).encode(ids).shape == flat
     assert EmbeddingEncoder(10, num_bits=4, flatten=False).encode(ids).shape == shape + (4,)
+
+
+def test_network_refuses_an_encoder_without_thresholds():
+    with pytest.raises(TypeError, match="thresholds.*EmbeddingEncoder.*layer API"):
+        DWNNetwork(EmbeddingEncoder(10, num_bits=4), [], GroupSum(k=2, tau=1.0, use_randperm=False))
