@@ -120,7 +120,7 @@ class Dropout(nn.Module):
 
     @staticmethod
     def _draw_seed() -> int:
-        return int(torch.randint(0, 2 ** 62, (1,), dtype=torch.int64).item())
+        return int(torch.randint(0, 2 ** 62, (1,), dtype=torch.int64, device="cpu").item())
 
     def extra_repr(self) -> str:
         return f"p={self.p}"

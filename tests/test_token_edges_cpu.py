@@ -151,3 +151,17 @@ def test_embedding_encoder_shapes(no_launches, shape, flat):
 def test_network_refuses_an_encoder_without_thresholds():
     with pytest.raises(TypeError, match="thresholds.*EmbeddingEncoder.*layer API"):
         DWNNetwork(EmbeddingEncoder(10, num_bits=4), [], GroupSum(k=2, tau=1.0, use_randperm=False))
+
+
+def test_dropout_module_seed_comes_from_the_cpu_generator(no_launches, monkeypatch):
+    """Whatever the default device is."""
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    seeds = []
+    monkeypatch.setattr(_native, "entry", lambda name: lambda *args: seeds.append(args[5]))
+    x, drop = torch.ones(8), Dropout(0.5).train()
+    for device in ("cpu", "meta"):
+        torch.manual_seed(3)
+        with torch.device(device):
+            drop(x)
+    torch.manual_seed(3)
+    assert seeds == [int(torch.randint(0, 2 ** 62, (1,), dtype=torch.int64))] * 2
