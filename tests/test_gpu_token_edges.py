@@ -4,14 +4,18 @@ Bounds as in test_gpu_token_ops.py: a rounding to type t is off by at most half 
 fp32 additions by n * 2^-24 of what it adds up.
 """
 
+import copy
+
+import numpy as np
 import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
 from torch.utils.checkpoint import checkpoint
 
+from difflut_b200 import _native
 from difflut_b200.encoder import embedding_lookup
 from difflut_b200.utils import Dropout, dropout, group_norm, sample_logits
-from token_util import half_step
+from token_util import half_step, philox
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -180,3 +184,40 @@ def test_what_the_backward_pass_needs_goes_through_saved_tensor_hooks(name):
     with torch.autograd.graph.save_on_cpu():
         y = call()
     assert torch.equal(torch.autograd.grad(y, leaf, torch.ones_like(y))[0], want)
+
+
+def test_dropout_module_masks_repeat_under_a_seed():
+    x = torch.ones(4096, device=DEV)
+    called = Dropout(0.5).train()
+    called(x)  # has a counter from here on
+    for module in (Dropout(0.5).train(), called, copy.deepcopy(called)):
+        masks = []
+        for _ in range(2):
+            torch.manual_seed(11)
+            masks.append((module(x), module(x), module(x)))
+        for a, b in zip(*masks):
+            assert torch.equal(a, b)
+        assert not torch.equal(masks[0][0], masks[0][1]) and not torch.equal(masks[0][1], masks[0][2])
+    torch.manual_seed(11)
+    assert torch.equal(copy.deepcopy(called)(x), masks[0][0])
+    assert called._counters and not copy.deepcopy(called)._counters
+
+
+def test_dropout_elements_past_2_34():
+    """There the counter's second word, the high one of element index / 4, is no longer zero."""
+    behind = 4096 + 8 * 123 + 5
+    count = (1 << 34) + behind
+    if torch.cuda.mem_get_info()[0] < 2 * count + (8 << 30):
+        pytest.skip("needs 42 GB of free device memory")
+    x = torch.empty(count, device=DEV, dtype=torch.bfloat16)
+    first = (1 << 34) - 4096
+    x[first:] = 1.0
+    _native.call("dl_dropout", x, x, count, 1, 0.5, 5, 3, None)  # in place
+    got = x[first:].float().cpu()
+    del x
+    q = np.arange(first // 4, (count + 3) // 4, dtype=np.uint64)
+    low, high = q & np.uint64(0xFFFFFFFF), q >> np.uint64(32)
+    assert high[0] == 0 and high[-1] == 1
+    words = philox(np.stack([low, high, np.full_like(q, 3), np.zeros_like(q)], axis=1), (5, 0)).reshape(-1)
+    want = torch.from_numpy(np.where(words[:count - first] < 2 ** 31, 0.0, 2.0).astype(np.float32))
+    assert torch.equal(got, want)
