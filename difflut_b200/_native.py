@@ -205,7 +205,11 @@ def followed(*tensors) -> bool:
     derivative, where a bare launch would read as a tangent of zero."""
     if forward_ad._current_level >= 0:
         return True
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def refuse_tangents(*grads) -> None:
