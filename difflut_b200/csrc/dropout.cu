@@ -5,10 +5,11 @@
 // as easy as 1, 2, 3", 2011) computes for the counter (i / 4, offset) under the key `seed`, and is dropped when that
 // word is below p * 2^32: the mask depends neither on the type nor on the launch.
 //
-// Every element is read and written once.  The generator is what bounds 16-bit types: 18 wide products per four elements
-// keep the pipe that multiplies wide 65 % busy (59 % of the issue slots): 65.5 M bf16 elements, 262 MB, take 63 us or
-// 4.2 TB/s.  The fp32 kernel moves twice the bytes per product and runs at the copy rate of 6.5 TB/s.  A thread takes whole
-// Philox blocks: two accesses of 16 bytes, so that the loads of the second are under way during the rounds of the first.
+// Every element is read and written once.  16-bit types wait for the generator: 18 wide products per four elements keep the
+// pipe that multiplies wide 65 % busy, DRAM 45 %, and a thread loads, computes and stores once, so that the two overlap only
+// across blocks: 65.5 M bf16 elements, 262 MB, take 63 us or 4.2 TB/s.  The fp32 kernel moves twice the bytes per product and
+// runs at the copy rate of 6.5 TB/s.  A thread takes whole Philox blocks: two accesses of 16 bytes, so that the loads of the
+// second are under way during the rounds of the first.
 #include "elements.cuh"
 
 namespace {

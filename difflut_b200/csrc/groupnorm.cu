@@ -19,12 +19,14 @@
 // run of 8 rows is taken relative to the mean of its first row: 9 n.)  Runs, threads and chunks are joined by their means and
 // their squares, moved to the joint mean: only additions.  No atomics: the same bits on every call.
 //
-// Measured, 16 x 4096 x 512 bf16 with 32 groups and silu (67 MB a tensor): sums 16.5 us (4.1 TB/s), writing 26.7 us
-// (5.0 TB/s read and written; the exponential and the reciprocal keep their pipe 59 % busy); backward sums 34 us
-// (3.9 TB/s), writing 35 us (5.8 TB/s), the parameters' sums 4 us.  8192 rows of 1024 bf16 features, 32 groups, sigmoid
-// (17 MB a tensor, mostly in L2): 13.7 us forward and 21.6 + 3.6 us backward, bound by issue slots (51 %) and the wait for
-// one round of loads.  Maps of 128 x 576 x 32 fp32 (9 MB): 3.9 + 5.6 us forward, 6.7 + 6.2 + 2.2 us backward, mostly the
-// latency of the launches.
+// Measured with nothing of the inputs in L2, 16 x 4096 x 512 bf16 with 32 groups and silu (67 MB a tensor): sums 19.9 us
+// (3.4 TB/s; without the runs 19.8), writing 28.4 us (4.7 TB/s read and written; the exponential and the reciprocal keep
+// their pipe 60 % busy); backward sums 34 us (3.9 TB/s), writing 35 us (5.7 TB/s), the parameters' sums 4 us.  8192 rows of
+// 1024 bf16 features, 32 groups, sigmoid (17 MB a tensor): 15.2 us forward and 24.1 + 3.6 us backward: a round of loads,
+// shuffles and stores after the other, no unit above half of its rate (issue slots 51 %).  Maps of 128 x 576 x 32 fp32
+// (9 MB): 5.9 + 5.6 us forward, 7.7 + 6.3 + 2.4 us backward, mostly the latency of the launches.  Many samples of few
+// positions are slow for their size: 8192 x 6 x 16 fp32 (3 MB) 37.9 us forward, 49.8 + 12.4 backward, as every sample is
+// a block of one warp here, which holds the shared memory of eight.
 #include <type_traits>
 
 #include "elements.cuh"

@@ -25,8 +25,9 @@
 // top-p .95, 34 us with top-p .95 alone (8 rows: 30).  Of the latter the histogram of the weights takes 7 us, the two
 // searches in histograms 3 to 4 us each, collecting 4, the cut 5: latency of passes with few rounds of loads per thread,
 // not bandwidth (the 4 MB are read in a microsecond).  256 rows of 65536 fp32 logits with top-p .9 and min-p .01: 88 us, 43 of them the
-// histogram, bound by issue slots (51 % over all SMs, of which 108 hold two rows and 40 one; the double-precision pipe is
-// 12 % busy, the data pipe of shared memory 40 %); reading the 67 MB once takes 10.
+// histogram: no unit is at its limit (issue slots 51 % over all SMs, of which 108 hold two rows and 40 one, the data pipe of
+// shared memory 40 %, double precision 12 %); what a logit costs is an exponential and two atomics, also below the reach of
+// min-p, where they are not needed.  Reading the 67 MB once takes 10.
 #include <cooperative_groups.h>
 
 #include "elements.cuh"
@@ -169,7 +170,8 @@ __device__ __forceinline__ u64 warp_inclusive(u64 v, int lane) {
 // Element j * 32 + lane sits in register j: index order is register, then lane.  The borders of top-k and top-p are found bit
 // by bit of the key: counting 256 keys takes 8 comparisons and one reduction.  What top-k leaves is moved together, since
 // every register of exponentials costs a row eighty double-precision issue slots.  Measured, 8192 rows of 256 fp32 logits,
-// top-k 40: 15.6 us (17.9 before moving; reading the logits takes 1.3): issue-bound.
+// top-k 40: 15.6 us (17.9 before moving; reading the logits takes 1.3), 56 % of the issue slots: about 16 rounds of counting
+// that follow one another.
 template <typename T, int PER>
 __global__ void __launch_bounds__(128)
 sample_small_kernel(const T* __restrict__ logits, const __grid_constant__ Job job) {

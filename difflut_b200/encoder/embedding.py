@@ -70,7 +70,8 @@ def embedding_lookup(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0
 
     The gradient of `weight` sums the rows of equal ids in the order of their positions, in fp32, rounded once: the
     same bits on every run.  `padding_idx` takes no gradient.  An id outside [0, V) gives a NaN row and takes no
-    gradient (torch raises a device assertion; nothing is read outside the table here)."""
+    gradient (torch raises a device assertion; nothing is read outside the table here).  Differentiable once, in reverse
+    mode."""
     if not isinstance(ids, torch.Tensor) or ids.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"ids must be an int32 or int64 tensor, got {getattr(ids, 'dtype', type(ids))}")
     if weight.dim() != 2 or weight.shape[0] == 0 or weight.shape[1] == 0:

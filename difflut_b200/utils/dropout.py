@@ -59,7 +59,8 @@ def dropout(x: torch.Tensor, p: float = DEFAULT_DROPOUT_P, seed: int = 0, offset
     Element i (row-major) is dropped when word i % 4 of Philox4x32-10 with counter (i // 4, offset) and key `seed` is
     below p * 2^32 (rounded).  The same (p, seed, offset) drops the same elements: use another `offset` per call.
     `counter` (one int64 on x's device) is added to `offset` when the kernel runs, which lets a captured graph draw
-    another mask per replay; it must keep its value until the backward pass has run."""
+    another mask per replay; it must keep its value until the backward pass has run.  Differentiable any number of times, in
+    reverse mode."""
     p = _check_p(p)
     for name, value in (("seed", seed), ("offset", offset)):
         if isinstance(value, bool) or not isinstance(value, int) or not 0 <= value < _WORD:

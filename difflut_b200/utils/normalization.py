@@ -87,7 +87,8 @@ def group_norm(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor] 
     over all positions in between, by its mean and biased variance.
 
     x is float32, bfloat16 or float16; weight and bias (C) are float32 or of x's type.  Statistics and sums are fp32, the
-    result is rounded once.  activation: "none", "relu", "silu" or "sigmoid"."""
+    result is rounded once (sigmoids below 2^-126 are 0).  activation: "none", "relu", "silu" or "sigmoid".  Differentiable
+    once, in reverse mode."""
     act = _check_activation(activation)
     _native.dtype_code(x, "group_norm input")
     if x.dim() < 2:

@@ -37,11 +37,13 @@ def sample_logits(logits: torch.Tensor, u: torch.Tensor, temperature: Union[floa
     logits (0: all), of these in descending order those with less than `top_p` of their total weight before them (1:
     all), of these the ones that weigh at least `min_p` times the largest (0: all).  The id is the first one in
     ascending order whose running sum of kept weights exceeds u times their total.  Equal logits rank by index, lowest
-    first.  NaN and -inf are never taken; a row without any other logit gives -1.
+    first.  NaN and -inf are never taken; a row without any other logit gives -1.  Weights are whole numbers of 2^-50 of the
+    largest (above 4096 classes of 2^(log2 V - 62)): a class that weighs less than half of that is never drawn.
 
-    Every setting is a number or a tensor (R) of its own for each row (float32; int32 for top_k; other float
-    or integer types are converted).  u is float32 or float64.  logits (float32, bfloat16 or float16) may be a view with any distance between
-    its rows.  The result does not depend on the order of additions: the same id on every run."""
+    Every setting is a number or a tensor (R) of its own for each row (float32; int32 for top_k; other float or integer
+    types are converted, and counts that int32 does not hold keep all).  u is float32 or float64.  logits (float32,
+    bfloat16 or float16) may be a view with any distance between its rows.  The result does not depend on the order of
+    additions: the same id on every run."""
     code = _native.dtype_code(logits, "logits")
     if logits.dim() != 2 or logits.shape[1] == 0:
         raise ValueError(f"logits must have shape (rows, classes) with at least one class, got {tuple(logits.shape)}")
